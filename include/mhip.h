@@ -262,6 +262,64 @@ int mhip_flash_attention_ws(void* stream, const void* q, const void* k, const vo
                             int64_t mask_stride_b, int64_t mask_stride_h, int dtype, const int64_t* strides,
                             void* workspace, int64_t workspace_bytes);
 
+/* Serving: a cache in pages -------------------------------------------------- */
+
+/* Keys and values of many sequences in pages of `page_size` tokens (a power of two, 16 .. 256):
+ *   keys    [pages, heads, page_size, head_size]
+ *   values  [pages, heads, page_size / 16, head_size, 16]   (blocks of 16 tokens, token innermost)
+ * in the queries' type (scales NULL), or as OCP e4m3 bytes with a scale 2^(byte - 127) for each page and head, [pages, heads] bytes.
+ * head_size 32, 64, 96 or 128; 16-byte aligned.  The reference has no cache (its attention takes packed [B,H,S,D],
+ * Runtime/MetalExecutor.swift:502-564). */
+typedef struct {
+    void* keys;
+    void* values;
+    uint8_t* key_scales;
+    uint8_t* value_scales;
+    int64_t pages, heads, page_size, head_size;
+} mhip_paged_cache;
+
+/* The sequences of a call, all of it device memory, so that a captured launch takes what is there when it is replayed:
+ *   starts  [sequences + 1]      sequence b's new tokens are rows starts[b] .. starts[b + 1] of the call's tensors, in order; rows behind the last one
+ *                                (a padded batch) are neither read nor written
+ *   lengths [sequences]          its keys in all, the new tokens' among them (they are the last ones)
+ *   table   [sequences, width]   the pages of its keys; an entry outside [0, pages) holds no keys and takes none
+ * `tokens` is the number of rows of the tensors.  A sequence may have no new tokens.  Pages may be shared for reading; a page that takes tokens
+ * belongs to one sequence, once.  Up to 65536 sequences, 2^24 tokens and 2^24 keys a sequence. */
+typedef struct {
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* starts;
+    int64_t sequences, width, tokens;
+} mhip_sequences;
+
+/* Stores the new tokens' k and v [tokens, heads, head_size] in the cache.  With `rotated` > 0 (a multiple of 16) the first `rotated` elements of k, and of q [tokens, q_heads,
+ * head_size] if that is given, are turned as mhip_rope turns them, by row `position` of freqs [positions, rotated] in fp32 (cosines, then sines); q_out gets the
+ * turned queries and may be q.  A token whose position lies outside of freqs is passed over.  8 bits: a page's scale is the least power of two under which the
+ * page's largest value is within 448; it never shrinks while the page holds older tokens, whose values are rounded anew where it grows.  What is not finite is stored as NaN there.
+ * strides: {token, head} in elements of k, v, q, q_out (the last two where q is given), multiples of 8, the last axis contiguous; 16-byte aligned tensors.
+ * BF16, F16; fp32 arithmetic, one rounding (CustomCallHandlers.swift:720-846 for the rotation). */
+int mhip_paged_append(void* stream, const mhip_paged_cache* cache, const mhip_sequences* seqs, const void* k, const void* v, const void* q, void* q_out,
+                      int64_t q_heads, const float* freqs, int64_t positions, int64_t rotated, const int64_t* strides, int dtype);
+
+/* o = softmax(scale * q K^T, causal) V over each sequence's keys, q and o [tokens, q_heads, head_size], q_heads a multiple of the cache's heads (query head h reads
+ * head h / (q_heads / heads)).  Causal: a token sees the keys up to its own position.  A token without keys yields zeros.
+ * fp32 softmax state and accumulation; the last bits of a row may depend on the other sequences of the call, whose lengths decide over how many
+ * parts its keys are dealt.  strides: {token, head} of q and o in elements, multiples of 8; 16-byte aligned tensors.  BF16, F16.
+ * The workspace (mhip_paged_attention_workspace bytes, 16-byte aligned, overwritten) lets keys be dealt over the whole device; with less, or none, they are not. */
+int64_t mhip_paged_attention_workspace(const mhip_paged_cache* cache, const mhip_sequences* seqs, int64_t q_heads);
+int mhip_paged_attention(void* stream, const mhip_paged_cache* cache, const mhip_sequences* seqs, const void* q, void* o, int64_t q_heads, float scale,
+                         int is_causal, const int64_t* strides, int dtype, void* workspace, int64_t workspace_bytes);
+
+/* Of each row of logits [rows, vocab]: the log probability of tokens[row] (NaN for one outside [0, vocab)), the distribution's entropy in nats (may be NULL), and
+ * its `top` most likely tokens (up to 64; 0: none, NULL) with their log probabilities [rows, top], the most likely first and the lowest index among equals.  A -inf logit has
+ * probability zero; a row that holds a NaN or +inf, or nothing but -inf, yields NaN log probabilities and entropy, and its alternatives in the order of its
+ * logits, a NaN above all (as mhip_argmax).  BF16, F16, F32 logits of any alignment of their type, I32 or I64 tokens; fp32 arithmetic and results.
+ * The workspace (mhip_token_log_probs_workspace bytes, 0: of no use; 16-byte aligned, overwritten) lets few rows be dealt over the whole device.
+ * The reference has softmax only (Metal/Kernels/SoftmaxKernel.swift:16-215). */
+int64_t mhip_token_log_probs_workspace(int64_t rows, int64_t vocab, int top);
+int mhip_token_log_probs(void* stream, const void* logits, const void* tokens, float* log_probs, float* entropy, float* top_log_probs, int32_t* top_ids,
+                         int64_t rows, int64_t vocab, int top, int dtype, int token_dtype, void* workspace, int64_t workspace_bytes);
+
 /* Glue operators (index / data movement; integer results are bit-exact) ---- */
 
 /* out[i, :] = table[clamp(idx[i], 0, n_rows-1), :], rows of `row_elems` elements.

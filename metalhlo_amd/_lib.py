@@ -57,6 +57,11 @@ SIGNATURES = {
     "mhip_flash_attention_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i32, _i32]),
     "mhip_flash_attention_ws": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                                        _f32, _i32, _i64, _i64, _i32, _vp, _vp, _i64]),
+    "mhip_paged_append": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _i32]),
+    "mhip_paged_attention_workspace": (_i64, [_vp, _vp, _i64]),
+    "mhip_paged_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _f32, _i32, _vp, _i32, _vp, _i64]),
+    "mhip_token_log_probs_workspace": (_i64, [_i64, _i64, _i32]),
+    "mhip_token_log_probs": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _i64]),
     "mhip_copy": (_i32, [_vp, _vp, _vp, _i64]),
     "mhip_gather_rows": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32]),
     "mhip_embed_tokens": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32]),

@@ -8,6 +8,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -471,6 +472,177 @@ FUNCTION(flash_attention) {
     });
 }
 
+// ---- a cache in pages
+
+// On the device that the call runs on: a launch goes to the current device's stream.
+void on_current_device(const at::Tensor& t) {
+    if (!t.is_cuda()) raise(PyExc_RuntimeError, "metalhlo_amd kernels need device tensors (no CPU path exists)");
+    if (t.device().index() != c10::hip::current_device()) raise(PyExc_ValueError, "tensors must be on the current device");
+}
+
+// (keys, values, key_scales, value_scales) of a PagedCache, checked against one another
+struct Cache {
+    mhip_paged_cache c{};
+    at::ScalarType type = at::kBFloat16;           // of keys and values
+    bool eight = false;
+};
+Cache cache_of(PyObject* o) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) raise(PyExc_TypeError, "expected a PagedCache");
+    const at::Tensor &k = dense(PyTuple_GET_ITEM(o, 0)), &v = dense(PyTuple_GET_ITEM(o, 1));
+    const at::Tensor *ks = optional_dense(PyTuple_GET_ITEM(o, 2)), *vs = optional_dense(PyTuple_GET_ITEM(o, 3));
+    if (k.dim() != 4 || v.dim() != 5) raise(PyExc_ValueError, "keys must be [pages, heads, page, D] and values [pages, heads, page / 16, D, 16]");
+    if (v.size(0) != k.size(0) || v.size(1) != k.size(1) || v.size(2) * 16 != k.size(2) || v.size(3) != k.size(3) || v.size(4) != 16)
+        raise(PyExc_ValueError, "keys [pages, heads, page, D] and values [pages, heads, page / 16, D, 16] do not belong together");
+    if (k.scalar_type() != v.scalar_type()) raise(PyExc_TypeError, "keys and values must have one element type");
+    Cache r;
+    r.type = k.scalar_type();
+    r.eight = r.type == at::kFloat8_e4m3fn;
+    if (r.eight != (ks != nullptr) || r.eight != (vs != nullptr)) raise(PyExc_ValueError, "a cache in float8_e4m3fn has scales, one in 16 bits has none");
+    for (const at::Tensor* s : {ks, vs})
+        if (s && (s->scalar_type() != at::kByte || s->dim() != 2 || s->size(0) != k.size(0) || s->size(1) != k.size(1)))
+            raise(PyExc_ValueError, "scales must be uint8 [pages, heads]");
+    for (const at::Tensor* t : {&k, &v, ks, vs})
+        if (t) on_current_device(*t);
+    r.c = {k.data_ptr(), v.data_ptr(), ks ? static_cast<uint8_t*>(ks->data_ptr()) : nullptr, vs ? static_cast<uint8_t*>(vs->data_ptr()) : nullptr,
+           k.size(0), k.size(1), k.size(2), k.size(3)};
+    return r;
+}
+
+mhip_sequences sequences_of(PyObject* table_o, PyObject* lengths_o, PyObject* starts_o, int64_t tokens) {
+    const at::Tensor &table = dense(table_o), &lengths = dense(lengths_o), &starts = dense(starts_o);
+    for (const at::Tensor* t : {&table, &lengths, &starts}) {
+        on_current_device(*t);
+        if (t->scalar_type() != at::kInt) raise(PyExc_TypeError, "table, lengths and starts must be int32");
+    }
+    if (table.dim() != 2 || lengths.dim() != 1 || starts.dim() != 1 || lengths.size(0) != table.size(0) || starts.size(0) != table.size(0) + 1)
+        raise(PyExc_ValueError, "table must be [sequences, width], lengths [sequences] and starts [sequences + 1]");
+    return {table.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), starts.data_ptr<int32_t>(), table.size(0), table.size(1), tokens};
+}
+
+// A device tensor [tokens, heads, D] of a 16-bit type that belongs to the cache; writes its token and head strides.
+const at::Tensor& head_rows(PyObject* o, const Cache& cache, int64_t* strides) {
+    const at::Tensor& t = tensor(o);
+    on_current_device(t);
+    if (t.dim() != 3 || t.size(2) != cache.c.head_size) raise(PyExc_ValueError, "q, k and v must be [tokens, heads, D] with the cache's D");
+    if (cache.eight ? t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kHalf : t.scalar_type() != cache.type)
+        raise(PyExc_TypeError, "q, k and v must be bfloat16 or float16, of the type of a cache in 16 bits");
+    if (t.stride(2) != 1) raise(PyExc_ValueError, "the last axis must be contiguous");
+    strides[0] = t.size(0) > 1 ? t.stride(0) : 0;      // (of an axis of one element the stride says nothing)
+    strides[1] = t.size(1) > 1 ? t.stride(1) : 0;
+    return t;
+}
+
+void no_overlap(const at::Tensor& t, const char* msg) {
+    const int64_t D = t.size(2);
+    const int64_t ts = t.size(0) > 1 ? t.stride(0) : INT64_MAX, hs = t.size(1) > 1 ? t.stride(1) : INT64_MAX;
+    const bool ok = t.numel() == 0 || (ts >= D && hs >= D && (t.size(0) <= 1 || t.size(1) <= 1 || (ts > hs ? ts >= hs * (t.size(1) - 1) + D : hs >= ts * (t.size(0) - 1) + D)));
+    if (!ok) raise(PyExc_ValueError, msg);
+}
+
+// paged_append(cache, k, v, table, lengths, starts, q, freqs, out) -> turned queries or None
+FUNCTION(paged_append) {
+    return guarded(n, 9, [&]() -> PyObject* {
+        const Cache cache = cache_of(arg[0]);
+        int64_t strides[8] = {};
+        const at::Tensor &k = head_rows(arg[1], cache, strides), &v = head_rows(arg[2], cache, strides + 2);
+        if (k.size(1) != cache.c.heads || v.size(1) != cache.c.heads || v.size(0) != k.size(0)) raise(PyExc_ValueError, "k and v must be [tokens, the cache's heads, D]");
+        if (v.scalar_type() != k.scalar_type()) raise(PyExc_TypeError, "q, k and v must have one element type");
+        const mhip_sequences seqs = sequences_of(arg[3], arg[4], arg[5], k.size(0));
+        const at::Tensor* freqs = optional_dense(arg[7]);
+        if (freqs) {
+            on_current_device(*freqs);
+            if (freqs->scalar_type() != at::kFloat || freqs->dim() != 2 || freqs->size(1) > cache.c.head_size || freqs->size(1) == 0)
+                raise(PyExc_ValueError, "freqs must be fp32 [positions, R], R up to D: cosines, then sines");
+        }
+        at::Tensor out;
+        const at::Tensor* q = nullptr;
+        if (arg[6] != Py_None) {
+            q = &head_rows(arg[6], cache, strides + 4);
+            if (q->size(0) != k.size(0) || q->size(1) == 0) raise(PyExc_ValueError, "q must have k's tokens");
+            if (q->scalar_type() != k.scalar_type()) raise(PyExc_TypeError, "q, k and v must have one element type");
+            if (!freqs) raise(PyExc_ValueError, "queries are turned by freqs: without them they stay what they are");
+            if (arg[8] == Py_None) out = empty({q->size(0), q->size(1), q->size(2)}, q->scalar_type(), *q);
+            else out = tensor(arg[8]);
+            head_rows(arg[8] == Py_None ? arg[6] : arg[8], cache, strides + 6);
+            if (arg[8] == Py_None) { strides[6] = q->size(1) * q->size(2); strides[7] = q->size(2); }
+            if (out.sizes() != q->sizes() || out.scalar_type() != q->scalar_type()) raise(PyExc_ValueError, "out must have q's shape and type");
+            no_overlap(out, "out must not overlap itself");
+        } else if (arg[8] != Py_None) {
+            raise(PyExc_ValueError, "out without queries");
+        }
+        const int dt = dtype_code(k.scalar_type());
+        check([&] { return mhip_paged_append(stream_of(k), &cache.c, &seqs, k.data_ptr(), v.data_ptr(), q ? q->data_ptr() : nullptr, q ? out.data_ptr() : nullptr,
+                                             q ? q->size(1) : 0, f32(freqs), freqs ? freqs->size(0) : 0, freqs ? freqs->size(1) : 0, strides, dt); });
+        if (q) return THPVariable_Wrap(std::move(out));
+        Py_RETURN_NONE;
+    });
+}
+
+// paged_attention(q, cache, table, lengths, starts, scale or None, is_causal, out)
+FUNCTION(paged_attention) {
+    return guarded(n, 8, [&] {
+        const Cache cache = cache_of(arg[1]);
+        int64_t strides[4];
+        const at::Tensor& q = head_rows(arg[0], cache, strides);
+        const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
+        if (H == 0 || cache.c.heads == 0 || H % cache.c.heads) raise(PyExc_ValueError, "the query heads must be a multiple of the cache's heads");
+        const mhip_sequences seqs = sequences_of(arg[2], arg[3], arg[4], T);
+        const float scale = arg[5] == Py_None ? 1.f / std::sqrt((float)D) : (float)number(arg[5]);
+        const bool causal = truth(arg[6]);
+        at::Tensor out;
+        if (arg[7] == Py_None) {
+            out = empty({T, H, D}, q.scalar_type(), q);
+            strides[2] = H * D;
+            strides[3] = D;
+        } else {
+            out = head_rows(arg[7], cache, strides + 2);
+            if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type()) raise(PyExc_ValueError, "out must have q's shape and type");
+            no_overlap(out, "out must not overlap itself");
+        }
+        const int dt = dtype_code(q.scalar_type());
+        const at::Tensor work = workspace(mhip_paged_attention_workspace(&cache.c, &seqs, H), q);
+        check([&] { return mhip_paged_attention(stream_of(q), &cache.c, &seqs, q.data_ptr(), out.data_ptr(), H, scale, causal, strides, dt,
+                                                work.defined() ? work.data_ptr() : nullptr, work.defined() ? work.numel() : 0); });
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// token_log_probs(logits, tokens, top) -> (log probabilities, entropy[, top log probabilities, top ids])
+FUNCTION(token_log_probs) {
+    return guarded(n, 3, [&] {
+        const at::Tensor &x = dense(arg[0]), &tokens = dense(arg[1]);
+        on_current_device(x);
+        on_current_device(tokens);
+        if (x.dim() < 1) raise(PyExc_ValueError, "logits must be [.., vocab]");
+        const int64_t vocab = x.size(-1), top = integer(arg[2]);
+        c10::SmallVector<int64_t, 8> lead(x.sizes().begin(), x.sizes().end() - 1);
+        if (tokens.sizes() != at::IntArrayRef(lead)) raise(PyExc_ValueError, "tokens must have logits' leading axes");
+        if (vocab < 1) raise(PyExc_ValueError, "logits without a vocabulary");
+        if (top < 0 || top > 64 || top > vocab) raise(PyExc_ValueError, "top must lie between 0 and 64, and within the vocabulary");
+        const int dt = dtype_code(x.scalar_type()), tt = dtype_code(tokens.scalar_type());
+        const int64_t rows = x.numel() / vocab;
+        at::Tensor p = empty(lead, at::kFloat, x), entropy = empty(lead, at::kFloat, x), tp, ti;
+        if (top) {
+            lead.push_back(top);
+            tp = empty(lead, at::kFloat, x);
+            ti = empty(lead, at::kInt, x);
+        }
+        const at::Tensor work = workspace(mhip_token_log_probs_workspace(rows, vocab, (int)top), x);
+        check([&] { return mhip_token_log_probs(stream_of(x), x.data_ptr(), tokens.data_ptr(), p.data_ptr<float>(), entropy.data_ptr<float>(), top ? tp.data_ptr<float>() : nullptr,
+                                                top ? ti.data_ptr<int32_t>() : nullptr, rows, vocab, (int)top, dt, tt, work.defined() ? work.data_ptr() : nullptr,
+                                                work.defined() ? work.numel() : 0); });
+        PyObject* r = PyTuple_New(top ? 4 : 2);
+        if (!r) throw Failed();
+        PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(p)));
+        PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(entropy)));
+        if (top) {
+            PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(std::move(tp)));
+            PyTuple_SET_ITEM(r, 3, THPVariable_Wrap(std::move(ti)));
+        }
+        return r;
+    });
+}
+
 // argmax(x, 64-bit indices?, with values?)
 FUNCTION(argmax) {
     return guarded(n, 3, [&]() -> PyObject* {
@@ -503,7 +675,8 @@ FUNCTION(bind) {
 
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {ENTRY(softmax), ENTRY(layer_norm), ENTRY(rms_norm), ENTRY(bias_gelu), ENTRY(matmul), ENTRY(linear), ENTRY(linear_layer), ENTRY(matmul_sums), ENTRY(tied_head), ENTRY(finish_norm), ENTRY(causal_attention), ENTRY(attend_project), ENTRY(attend_project_layer),
-                          ENTRY(flash_attention), ENTRY(argmax), ENTRY(bind), {nullptr, nullptr, 0, nullptr}};
+                          ENTRY(flash_attention), ENTRY(argmax), ENTRY(paged_append), ENTRY(paged_attention), ENTRY(token_log_probs),
+                          ENTRY(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -175,6 +175,54 @@ def attend_project_layer(qkv, weight, bias, residual, batch: int, n_head: int, a
 
 def attend_project_layer_served(batch: int, length: int, n_head: int, head_size: int, N: int, dtype) -> bool:
     return bool(_lib.load().mhip_attend_project_layer_ok(batch, length, n_head, head_size, N, DTYPE_CODE[dtype]))
+
+
+# ---- serving: a cache in pages --------------------------------------------------
+class PagedCache(NamedTuple):
+    """Keys and values of many sequences in pages of 16 to 256 tokens (a power of two), head sizes 32, 64, 96 and 128: `keys`
+    [pages, heads, page, D], `values` [pages, heads, page / 16, D, 16] (blocks of sixteen tokens, the token innermost).  In bfloat16 or float16, or in
+    float8_e4m3fn with a scale 2 ** (byte - 127) a page and head (`key_scales`, `value_scales`, uint8 [pages, heads]).
+
+    The calls on it take what describes the sequences from device memory (all int32): `table` [sequences, width], the pages of each (an entry outside the
+    cache holds no keys and takes none); `lengths` [sequences], its keys, those of the call's tokens among them, which are the last; `starts` [sequences + 1], where its
+    tokens begin among the rows of q, k and v.  Rows behind the last sequence stay as they are.  A page that takes tokens belongs to one sequence, once."""
+    keys: torch.Tensor
+    values: torch.Tensor
+    key_scales: Optional[torch.Tensor] = None
+    value_scales: Optional[torch.Tensor] = None
+
+
+def paged_cache(pages: int, heads: int, page_size: int, head_size: int, dtype, device="cuda") -> PagedCache:
+    """An empty PagedCache; its memory holds anything until tokens are appended."""
+    if page_size % 16:
+        raise ValueError("a page holds blocks of 16 tokens")
+    keys = torch.empty(pages, heads, page_size, head_size, dtype=dtype, device=device)
+    values = torch.empty(pages, heads, page_size // 16, head_size, 16, dtype=dtype, device=device)
+    if dtype != torch.float8_e4m3fn:
+        return PagedCache(keys, values)
+    return PagedCache(keys, values, *(torch.zeros(pages, heads, dtype=torch.uint8, device=device) for _ in range(2)))
+
+
+def paged_append(cache: PagedCache, k, v, table, lengths, starts, q=None, freqs=None, out=None):
+    """Stores k and v [tokens, heads, D] (views with a contiguous last axis) of each sequence's new tokens in the cache.  With `freqs` [positions, R] in fp32 (R / 2
+    cosines, then sines; R a multiple of 16) the first R elements of k, and of q [tokens, query heads, D], are turned on the way as `rope` turns them; returns the
+    turned q (`out`, which may be q, or a new tensor).  A token whose position lies outside of freqs is passed over.  8 bits: a page's scale is the least
+    that its largest value needs and only grows while the page holds older tokens, whose values are then rounded anew; what is not finite becomes NaN."""
+    return (_native or _host()).paged_append(cache, k, v, table, lengths, starts, q, freqs, out)
+
+
+def paged_attention(q, cache: PagedCache, table, lengths, starts, scale: Optional[float] = None, is_causal: bool = True,
+                    out: Optional[torch.Tensor] = None):
+    """softmax(scale * q k^T, causal) v over each sequence's keys in the cache: q [tokens, query heads, D], query heads a multiple of the cache's heads.  Causal: a
+    token sees the keys up to its own position.  A token without keys yields zeros.  Default scale 1/sqrt(D).  The last bits of a row may depend on the
+    lengths of the other sequences, as mhip.h says."""
+    return (_native or _host()).paged_attention(q, cache, table, lengths, starts, scale, is_causal, out)
+
+
+def token_log_probs(logits, tokens, top: int = 0):
+    """(log probability of each token, entropy of each row's distribution) of logits [.., vocab] and tokens [..] (int32 or int64; one outside the vocabulary yields NaN),
+    and with `top` (up to 64) also (log probabilities, ids) of the most likely tokens [.., top], the lowest id among equals.  fp32 results."""
+    return (_native or _host()).token_log_probs(logits, tokens, top)
 
 
 # ---- glue -------------------------------------------------------------------
