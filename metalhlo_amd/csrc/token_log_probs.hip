@@ -42,27 +42,59 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 __device__ __forceinline__ float value_of(uint32_t o) { return __builtin_bit_cast(float, o == ~0u ? 0x7FC00000u : (o >> 31) ? o & 0x7FFFFFFFu : ~o); }
 __device__ __forceinline__ uint64_t key_of(float v, uint32_t index) { return (uint64_t)ordered(v) << 32 | (uint32_t)~index; }
 
-__device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane) {
-    return (uint64_t)(uint32_t)__shfl((int)(v >> 32), lane, 64) << 32 | (uint32_t)__shfl((int)v, lane, 64);
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xF, 0xF, false); }
+// the word of lane ^ J, in the register file
+template <int J>
+__device__ __forceinline__ uint32_t word_of(uint32_t v) {
+    if constexpr (J == 1) return moved<0xB1>(v);                          // quad_perm
+    else if constexpr (J == 2) return moved<0x4E>(v);
+    else if constexpr (J == 3) return moved<0x1B>(v);
+    else if constexpr (J == 7) return moved<0x141>(v);                    // row_half_mirror
+    else if constexpr (J == 4) return moved<0x1B>(moved<0x141>(v));
+    else if constexpr (J == 8) return moved<0x128>(v);                    // row_ror
+    else if constexpr (J == 15) return moved<0x140>(v);                   // row_mirror
+    else if constexpr (J == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (threadIdx.x & 16) ? r[0] : r[1];
+    } else if constexpr (J == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return (threadIdx.x & 32) ? r[0] : r[1];
+    } else if constexpr (J == 31) return word_of<16>(word_of<15>(v));
+    else return word_of<32>(word_of<31>(v));                              // 63
 }
-__device__ __forceinline__ uint64_t exchange(uint64_t v, int lane, int j, bool greater) {
-    const uint64_t w = lane_key(v, lane ^ j);
-    return (w > v) == greater ? w : v;
+template <int J>
+__device__ __forceinline__ uint64_t key_at(uint64_t v) { return (uint64_t)word_of<J>((uint32_t)(v >> 32)) << 32 | word_of<J>((uint32_t)v); }
+template <int J>
+__device__ __forceinline__ uint64_t greater(uint64_t v) {
+    const uint64_t w = key_at<J>(v);
+    return w > v ? w : v;
 }
-// a wave's keys, the greatest in lane 0
-__device__ inline uint64_t sorted(uint64_t v, int lane) {
-#pragma unroll
-    for (int k = 2; k <= 64; k *= 2)
-#pragma unroll
-        for (int j = k / 2; j; j /= 2) v = exchange(v, lane, j, ((lane & k) == 0) == ((lane & j) == 0));
-    return v;
+// lanes i and i ^ J: the one whose `bit` is clear has the greater key afterwards
+template <int J>
+__device__ __forceinline__ void order(uint64_t& v, int lane, int bit) {
+    const uint64_t w = key_at<J>(v);
+    v = (w > v) == ((lane & bit) == 0) ? w : v;
+}
+// groups of 2 J lanes whose keys rise and fall once, each sorted
+template <int J>
+__device__ __forceinline__ void settle(uint64_t& v, int lane) {
+    order<J>(v, lane, J);
+    if constexpr (J > 1) settle<J / 2>(v, lane);
+}
+// a wave's keys, the greatest in lane 0: sorted groups of K lanes are mirrored against one another, which leaves both halves such groups
+template <int K = 2>
+__device__ __forceinline__ uint64_t sorted(uint64_t v, int lane) {
+    order<K - 1>(v, lane, K / 2);
+    if constexpr (K > 2) settle<K / 4>(v, lane);
+    if constexpr (K < 64) return sorted<2 * K>(v, lane);
+    else return v;
 }
 // the 64 greatest of two sorted lists, sorted
-__device__ inline uint64_t merged(uint64_t a, uint64_t b, int lane) {
-    const uint64_t r = lane_key(b, 63 - lane);
+__device__ __forceinline__ uint64_t merged(uint64_t a, uint64_t b, int lane) {
+    const uint64_t r = key_at<63>(b);
     uint64_t v = a > r ? a : r;
-#pragma unroll
-    for (int j = 32; j; j /= 2) v = exchange(v, lane, j, (lane & j) == 0);
+    settle<32>(v, lane);
     return v;
 }
 
@@ -81,67 +113,97 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
     __shared__ uint64_t found[kMost];
     __shared__ Sums wave_sums[kWaves];
     __shared__ uint64_t groups[64], bound, best[kWaves];
-    __shared__ int count, last;
+    __shared__ uint16_t holders[kThreads];
+    __shared__ int count, holding, last;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int part = blockIdx.x % a.parts;
     const int64_t row = blockIdx.x / a.parts;
     uint64_t seen = 0;
     if (a.parts > 1 && threadIdx.x == 0) seen = arrive_look(a.words + row);
     const T* x = static_cast<const T*>(a.x) + row * a.vocab;
-    // pieces of sixteen aligned bytes; the row begins `off` values into the first one
+    // pieces of sixteen aligned bytes; the row begins `off` values into piece 0.  Pieces [whole0, whole1) lie inside the row; one in front of them and one behind are read value by value
     const int off = (int)((uintptr_t)x & 15) / (int)sizeof(T);
     const int pieces = (int)((a.vocab + off + EPV - 1) / EPV);
     const int p0 = (int)min((int64_t)part * a.pieces, (int64_t)pieces), p1 = (int)min((int64_t)p0 + a.pieces, (int64_t)pieces);
+    const int whole0 = max(p0, off ? 1 : 0), whole1 = min(p1, (int)((a.vocab + off) / EPV));
+    const bool head = p0 == 0 && p1 > 0 && (off || whole1 == 0), tail = p1 == pieces && p1 - 1 >= whole1 && !(head && p1 == 1);
     const u32x4* base = reinterpret_cast<const u32x4*>(x - off);
-    auto read = [&](int p, float (&v)[EPV]) __attribute__((always_inline)) {
+    auto whole = [&](int p, float (&v)[EPV]) __attribute__((always_inline)) {
+        const Vec16<T> w = __builtin_bit_cast(Vec16<T>, base[p]);
+#pragma unroll
+        for (int e = 0; e < EPV; e++) v[e] = Elem<T>::to_f32(w.v[e]);
+    };
+    auto broken = [&](int p, float (&v)[EPV]) __attribute__((always_inline)) {
         const int64_t i0 = (int64_t)p * EPV - off;
-        if (i0 >= 0 && i0 + EPV <= a.vocab) {
-            const Vec16<T> w = __builtin_bit_cast(Vec16<T>, base[p]);
 #pragma unroll
-            for (int e = 0; e < EPV; e++) v[e] = Elem<T>::to_f32(w.v[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < EPV; e++) v[e] = i0 + e >= 0 && i0 + e < a.vocab ? Elem<T>::to_f32(x[i0 + e]) : -INFINITY;
-        }
+        for (int e = 0; e < EPV; e++) v[e] = i0 + e >= 0 && i0 + e < a.vocab ? Elem<T>::to_f32(x[i0 + e]) : -INFINITY;
     };
 
-    // ---- the sums, and each lane's greatest value
+    // ---- the sums, and each lane's greatest value.  Weights are 2^(x log2(e) - c) with c = ref log2(e) rounded; `slip` is what the rounding took (2^-8 at most), and
+    // leaves the sums with the reference that it belongs to.  References beyond 2^16 are subtracted before the multiplication
     Sums s{-INFINITY, 0.f, 0.f};
-    float most = -INFINITY;
-    int where = p0 + (int)threadIdx.x;
+    float c = 0.f, slip = 0.f, most = -INFINITY;
+    int where = -1;
+    auto settled = [&](Sums& s) __attribute__((always_inline)) {
+        const float f = __builtin_amdgcn_exp2f(-slip);
+        s.t = f * (s.t - slip * s.l);
+        s.l *= f;
+    };
     auto take = [&](const float (&v)[EPV], int p) __attribute__((always_inline)) {
-        float m = v[0];
+        float m = fmaxf(v[0], v[1]);
 #pragma unroll
-        for (int e = 1; e < EPV; e++) m = fmaxf(m, v[e]);
-        if (m > most) { most = m; where = p; }
+        for (int e = 2; e < EPV; e += 2) m = fmaxf(fmaxf(m, v[e]), v[e + 1]);
+        if (m > most || where < 0) { most = m; where = p; }
         if (m > s.ref + 8.f) {                                            // (from -inf on: any number)
+            settled(s);
             const float d = fmaxf((s.ref - m) * kLog2eT, -300.f), f = __builtin_amdgcn_exp2f(d);
             s.t = f * (s.t + s.l * d);
             s.l *= f;
             s.ref = m;
+            c = m * kLog2eT;
+            slip = fabsf(m) <= 65536.f ? fmaf(m, kLog2eT, -c) : 0.f;
         }
-        const float ref = s.ref == -INFINITY ? 0.f : s.ref;
+        if (s.ref > 65536.f || (s.ref < -65536.f && s.ref != -INFINITY)) {
+#pragma unroll
+            for (int e = 0; e < EPV; e++) {
+                const float d = (v[e] - s.ref) * kLog2eT, f = __builtin_amdgcn_exp2f(d);
+                s.l += f;
+                s.t = fmaf(f, fmaxf(d, -300.f), s.t);
+            }
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < EPV; e++) {
-            // (2^-300 is zero, and so is its product: a masked value adds nothing)
-            const float raw = (v[e] - ref) * kLog2eT, d = raw < -300.f ? -300.f : raw, f = __builtin_amdgcn_exp2f(d);
+            // (the weight of a masked value is zero, and so is its product with -300; a NaN stays one)
+            const float d = fmaf(v[e], kLog2eT, -c), f = __builtin_amdgcn_exp2f(d);
             s.l += f;
-            s.t = fmaf(f, d, s.t);
+            s.t = fmaf(f, fmaxf(d, -300.f), s.t);
         }
     };
-    int p = p0 + threadIdx.x;
-    for (; p + 3 * kThreads < p1; p += 4 * kThreads) {
+    if (head && threadIdx.x == kThreads - 1) {
+        float v[EPV];
+        broken(0, v);
+        take(v, 0);
+    }
+    int p = whole0 + threadIdx.x;
+    for (; p + 3 * kThreads < whole1; p += 4 * kThreads) {
         float v[4][EPV];
 #pragma unroll
-        for (int i = 0; i < 4; i++) read(p + i * kThreads, v[i]);
+        for (int i = 0; i < 4; i++) whole(p + i * kThreads, v[i]);
 #pragma unroll
         for (int i = 0; i < 4; i++) take(v[i], p + i * kThreads);
     }
-    for (; p < p1; p += kThreads) {
+    for (; p < whole1; p += kThreads) {
         float v[EPV];
-        read(p, v);
+        whole(p, v);
         take(v, p);
     }
+    if (tail && threadIdx.x == 0) {
+        float v[EPV];
+        broken(p1 - 1, v);
+        take(v, p1 - 1);
+    }
+    settled(s);
     if (a.parts > 1 && threadIdx.x == 0) arrive_claim(a.words + row, seen, a.tag);
     const bool not_a_number = s.l != s.l;
 #pragma unroll
@@ -151,51 +213,51 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
     // ---- the alternatives of this part
     uint64_t list = 0;
     if (a.top) {
-        uint64_t key = 0;
-        if (p0 + (int)threadIdx.x < p1) {
-            if (not_a_number) {                                           // (or an infinity: its sums are no numbers either)
-                for (int q = p0 + threadIdx.x; q < p1 && most == most; q += kThreads) {
-                    float v[EPV];
-                    read(q, v);
+        auto each_of = [&](int q, auto each) __attribute__((always_inline)) {
+            float v[EPV];
+            if (q >= whole0 && q < whole1) whole(q, v);
+            else broken(q, v);
 #pragma unroll
-                    for (int e = 0; e < EPV; e++)
-                        if (v[e] != v[e]) { most = v[e]; where = q; }
-                }
+            for (int e = 0; e < EPV; e++) {
+                const int64_t i = (int64_t)q * EPV - off + e;
+                if (i >= 0 && i < a.vocab) each(v[e], (uint32_t)i);
             }
-            key = key_of(most, (uint32_t)where);
+        };
+        if (not_a_number) {                                               // (or an infinity: its sums are no numbers either)
+            auto look = [&](int q) __attribute__((always_inline)) {
+                each_of(q, [&](float v, uint32_t) __attribute__((always_inline)) {
+                    if (v != v && most == most) { most = v; where = q; }
+                });
+            };
+            if (head && threadIdx.x == kThreads - 1) look(0);
+            for (int q = whole0 + threadIdx.x; q < whole1; q += kThreads) look(q);
+            if (tail && threadIdx.x == 0) look(p1 - 1);
         }
-        uint64_t group = key;
-#pragma unroll
-        for (int j = 1; j < kGroup; j *= 2) {
-            const uint64_t w = lane_key(group, lane ^ j);
-            group = w > group ? w : group;
-        }
+        const uint64_t key = where >= 0 ? key_of(most, (uint32_t)where) : 0;
+        const uint64_t group = greater<4>(greater<2>(greater<1>(key)));
         if (lane % kGroup == 0) groups[threadIdx.x / kGroup] = group;
-        if (threadIdx.x == 0) count = 0;
+        if (threadIdx.x == 0) count = holding = 0;
         __syncthreads();
         if (wave == 0) {
-            const uint64_t v = sorted(groups[lane], lane), b = lane_key(v, a.top - 1);
-            if (lane == 0) bound = b;
+            const uint64_t v = sorted(groups[lane], lane);
+            if (lane == a.top - 1) bound = v;
         }
         __syncthreads();
         const uint64_t limit = bound;
-        auto look = [&](auto each) __attribute__((always_inline)) {
-            for (int q = p0 + threadIdx.x; q < p1; q += kThreads) {
-                float v[EPV];
-                read(q, v);
-#pragma unroll
-                for (int e = 0; e < EPV; e++) {
-                    const int64_t i = (int64_t)q * EPV - off + e;
-                    if (i >= 0 && i < a.vocab) each(v[e], q, (uint32_t)i);
-                }
-            }
-        };
-        if (key >= limit)
-            look([&](float v, int q, uint32_t i) __attribute__((always_inline)) {
-                if (key_of(v, (uint32_t)q) < limit) return;
+        if (key >= limit && where >= 0) holders[atomicAdd(&holding, 1)] = (uint16_t)threadIdx.x;
+        __syncthreads();
+        // every piece of the lanes whose own maximum reaches the bound, dealt over the workgroup, and the two that are broken
+        const int lanes = holding, turns = (whole1 - whole0 + kThreads - 1) / kThreads, items = lanes * max(turns, 0);
+        const float least = value_of((uint32_t)(limit >> 32));
+        for (int i = threadIdx.x; i < items + 2; i += kThreads) {
+            const int q = i < items ? whole0 + holders[i % lanes] + i / lanes * kThreads : i == items ? (head ? 0 : -1) : (tail ? p1 - 1 : -1);
+            if (q < 0 || (i < items && q >= whole1)) continue;
+            each_of(q, [&](float v, uint32_t i) __attribute__((always_inline)) {
+                if (v < least || key_of(v, (uint32_t)q) < limit) return;
                 const int n = atomicAdd(&count, 1);
                 if (n < kMost) found[n] = key_of(v, i);
             });
+        }
         __syncthreads();
         const int n = count;
         if (n <= kMost) {
@@ -215,15 +277,12 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
             uint64_t before = ~(uint64_t)0;
             for (int r = 0; r < a.top; r++) {
                 uint64_t mine = 0;
-                look([&](float v, int, uint32_t i) __attribute__((always_inline)) {
-                    const uint64_t k = key_of(v, i);
-                    if (k < before && k > mine) mine = k;
-                });
-#pragma unroll
-                for (int j = 1; j < 64; j *= 2) {
-                    const uint64_t w = lane_key(mine, lane ^ j);
-                    mine = w > mine ? w : mine;
-                }
+                for (int q = p0 + threadIdx.x; q < p1; q += kThreads)
+                    each_of(q, [&](float v, uint32_t i) __attribute__((always_inline)) {
+                        const uint64_t k = key_of(v, i);
+                        if (k < before && k > mine) mine = k;
+                    });
+                mine = greater<32>(greater<16>(greater<8>(greater<4>(greater<2>(greater<1>(mine))))));
                 if (lane == 0) best[wave] = mine;
                 __syncthreads();
                 before = 0;
