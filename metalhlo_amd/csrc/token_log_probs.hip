@@ -11,13 +11,15 @@
 // the way, a piece's index standing for its values', so that the bound is one among equals too.  Where a row is built so that more than kMost values reach the bound, the row is read once for each alternative.
 //
 // Few rows are dealt over several workgroups each, and the last one to arrive puts the parts together (arrive.h).
+#include <type_traits>
+
 #include "arrive.h"
 #include "common.h"
 
 namespace mhip {
 namespace {
 
-constexpr int kThreads = 512, kWaves = kThreads / 64, kGroup = kThreads / 64, kMost = 4096, kMaxTop = 64, kMaxParts = 64;
+constexpr int kThreads = 256, kWaves = kThreads / 64, kGroup = kThreads / 64, kMost = 2048, kMaxTop = 64, kMaxParts = 64;
 constexpr float kLn2 = 0.69314718055994531f, kLog2eT = 1.4426950408889634f;
 
 struct LogProbArgs {
@@ -100,11 +102,11 @@ __device__ __forceinline__ uint64_t merged(uint64_t a, uint64_t b, int lane) {
 
 // sums under a reference: l = sum 2^d, t = sum 2^d d, d = log2(e) (x - ref)
 struct Sums { float ref, l, t; };
-__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
-    const float m = fmaxf(a.ref, b.ref), use = m == -INFINITY ? 0.f : m;
-    const float da = fmaxf((a.ref - use) * kLog2eT, -300.f), db = fmaxf((b.ref - use) * kLog2eT, -300.f);
-    const float ea = __builtin_amdgcn_exp2f(da), eb = __builtin_amdgcn_exp2f(db);
-    return {m, a.l * ea + b.l * eb, ea * (a.t + a.l * da) + eb * (b.t + b.l * db)};
+// of the wave's lanes, under the greatest of their references
+__device__ __forceinline__ Sums joined(Sums s) {
+    const float m = wave_max(s.ref);
+    const float d = fmaxf((s.ref - (m == -INFINITY ? 0.f : m)) * kLog2eT, -300.f), f = __builtin_amdgcn_exp2f(d);
+    return {m, wave_sum(s.l * f), wave_sum(f * (s.t + s.l * d))};
 }
 
 template <typename T>
@@ -134,80 +136,110 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
         for (int e = 0; e < EPV; e++) v[e] = Elem<T>::to_f32(w.v[e]);
     };
     auto broken = [&](int p, float (&v)[EPV]) __attribute__((always_inline)) {
-        const int64_t i0 = (int64_t)p * EPV - off;
+        const int i0 = p * EPV - off, n = (int)a.vocab;
+        T t[EPV];
 #pragma unroll
-        for (int e = 0; e < EPV; e++) v[e] = i0 + e >= 0 && i0 + e < a.vocab ? Elem<T>::to_f32(x[i0 + e]) : -INFINITY;
+        for (int e = 0; e < EPV; e++) t[e] = x[min(max(i0 + e, 0), n - 1)];       // (all on their way before the first is used)
+#pragma unroll
+        for (int e = 0; e < EPV; e++) v[e] = i0 + e >= 0 && i0 + e < n ? Elem<T>::to_f32(t[e]) : -INFINITY;
     };
 
-    // ---- the sums, and each lane's greatest value.  Weights are 2^(x log2(e) - c) with c = ref log2(e) rounded; `slip` is what the rounding took (2^-8 at most), and
-    // leaves the sums with the reference that it belongs to.  References beyond 2^16 are subtracted before the multiplication
+    // ---- the sums, and each lane's greatest value.  Weights are 2^(x log2(e) - c) with c = ref log2(e) rounded: 2^slip times what they are to be, `slip` being what the
+    // rounding took (2^-8 at most).  Where a lane of the wave has a reference beyond 2^16 it is subtracted before the multiplication
     Sums s{-INFINITY, 0.f, 0.f};
     float c = 0.f, slip = 0.f, most = -INFINITY;
     int where = -1;
-    auto settled = [&](Sums& s) __attribute__((always_inline)) {
-        const float f = __builtin_amdgcn_exp2f(-slip);
-        s.t = f * (s.t - slip * s.l);
-        s.l *= f;
-    };
+    bool far = false;
     auto take = [&](const float (&v)[EPV], int p) __attribute__((always_inline)) {
         float m = fmaxf(v[0], v[1]);
 #pragma unroll
         for (int e = 2; e < EPV; e += 2) m = fmaxf(fmaxf(m, v[e]), v[e + 1]);
-        if (m > most || where < 0) { most = m; where = p; }
-        if (m > s.ref + 8.f) {                                            // (from -inf on: any number)
-            settled(s);
-            const float d = fmaxf((s.ref - m) * kLog2eT, -300.f), f = __builtin_amdgcn_exp2f(d);
+        where = m > most ? p : where;
+        most = fmaxf(m, most);
+        if (__builtin_expect(__any(m > s.ref + 8.f), 0)) {                // (from -inf on: any number)
+            const float to = m > s.ref + 8.f ? m : s.ref;
+            const bool none = to == -INFINITY;
+            c = none ? 0.f : to * kLog2eT;
+            const float slips = !none && fabsf(to) <= 65536.f ? fmaf(to, kLog2eT, -c) : 0.f;
+            const float d = none ? 0.f : fmaxf((s.ref - to) * kLog2eT - slip + slips, -300.f), f = __builtin_amdgcn_exp2f(d);
             s.t = f * (s.t + s.l * d);
             s.l *= f;
-            s.ref = m;
-            c = m * kLog2eT;
-            slip = fabsf(m) <= 65536.f ? fmaf(m, kLog2eT, -c) : 0.f;
+            s.ref = to;
+            slip = slips;
+            far = __any(fabsf(to) > 65536.f && !none);
         }
-        if (s.ref > 65536.f || (s.ref < -65536.f && s.ref != -INFINITY)) {
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(far), 0)) {
+            const float ref = s.ref == -INFINITY ? 0.f : s.ref;
 #pragma unroll
             for (int e = 0; e < EPV; e++) {
-                const float d = (v[e] - s.ref) * kLog2eT, f = __builtin_amdgcn_exp2f(d);
+                const float d = fmaf(v[e] - ref, kLog2eT, slip), f = __builtin_amdgcn_exp2f(d);
                 s.l += f;
                 s.t = fmaf(f, fmaxf(d, -300.f), s.t);
             }
-            return;
-        }
+        } else {
 #pragma unroll
-        for (int e = 0; e < EPV; e++) {
-            // (the weight of a masked value is zero, and so is its product with -300; a NaN stays one)
-            const float d = fmaf(v[e], kLog2eT, -c), f = __builtin_amdgcn_exp2f(d);
-            s.l += f;
-            s.t = fmaf(f, fmaxf(d, -300.f), s.t);
+            for (int e = 0; e < EPV; e++) {
+                // (the weight of a masked value is zero, and so is its product with -300; a NaN stays one)
+                const float d = fmaf(v[e], kLog2eT, -c), f = __builtin_amdgcn_exp2f(d);
+                s.l += f;
+                s.t = fmaf(f, fmaxf(d, -300.f), s.t);
+            }
         }
     };
     if (head && threadIdx.x == kThreads - 1) {
         float v[EPV];
         broken(0, v);
+        where = 0;
         take(v, 0);
     }
-    int p = whole0 + threadIdx.x;
-    for (; p + 3 * kThreads < whole1; p += 4 * kThreads) {
-        float v[4][EPV];
+    constexpr int kAhead = 4;                                             // pieces that are asked for together
+    auto widened = [&](const u32x4& w, float (&v)[EPV]) __attribute__((always_inline)) {
+        const Vec16<T> t = __builtin_bit_cast(Vec16<T>, w);
 #pragma unroll
-        for (int i = 0; i < 4; i++) whole(p + i * kThreads, v[i]);
+        for (int e = 0; e < EPV; e++) v[e] = Elem<T>::to_f32(t.v[e]);
+    };
+    where = whole0 + (int)threadIdx.x < whole1 && where < 0 ? whole0 + threadIdx.x : where;
+    int p = whole0;                                                       // (the same in all lanes: an address is a scalar and a lane's own offset)
+    u32x4 w[kAhead];
+    for (; p <= whole1 - kAhead * kThreads; p += kAhead * kThreads) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) take(v[i], p + i * kThreads);
+        for (int i = 0; i < kAhead; i++) w[i] = (base + p + i * kThreads)[threadIdx.x];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            float v[EPV];
+            widened(w[i], v);
+            take(v, p + i * kThreads + threadIdx.x);
+        }
     }
-    for (; p < whole1; p += kThreads) {
-        float v[EPV];
-        whole(p, v);
-        take(v, p);
+    if (p < whole1) {
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) w[i] = (base + p)[min((int)threadIdx.x + i * kThreads, whole1 - 1 - p)];
+        auto rest = [&](auto which) __attribute__((always_inline)) {
+            constexpr int i = decltype(which)::value;
+            if (p + i * kThreads + (int)threadIdx.x < whole1) {
+                float v[EPV];
+                widened(w[i], v);
+                take(v, p + i * kThreads + threadIdx.x);
+            }
+        };
+        static_assert(kAhead == 4, "a call each");
+        rest(std::integral_constant<int, 0>{});
+        rest(std::integral_constant<int, 1>{});
+        rest(std::integral_constant<int, 2>{});
+        rest(std::integral_constant<int, 3>{});
     }
     if (tail && threadIdx.x == 0) {
         float v[EPV];
         broken(p1 - 1, v);
+        if (where < 0) where = p1 - 1;
         take(v, p1 - 1);
     }
-    settled(s);
+    const float unslipped = __builtin_amdgcn_exp2f(-slip);
+    s.t = unslipped * (s.t - slip * s.l);
+    s.l *= unslipped;
     if (a.parts > 1 && threadIdx.x == 0) arrive_claim(a.words + row, seen, a.tag);
     const bool not_a_number = s.l != s.l;
-#pragma unroll
-    for (int j = 1; j < 64; j *= 2) s = joined(s, Sums{__shfl_xor(s.ref, j, 64), __shfl_xor(s.l, j, 64), __shfl_xor(s.t, j, 64)});
+    s = joined(s);
     if (lane == 0) wave_sums[wave] = s;
 
     // ---- the alternatives of this part
@@ -219,8 +251,8 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
             else broken(q, v);
 #pragma unroll
             for (int e = 0; e < EPV; e++) {
-                const int64_t i = (int64_t)q * EPV - off + e;
-                if (i >= 0 && i < a.vocab) each(v[e], (uint32_t)i);
+                const int i = q * EPV - off + e;
+                if (i >= 0 && i < (int)a.vocab) each(v[e], (uint32_t)i);
             }
         };
         if (not_a_number) {                                               // (or an infinity: its sums are no numbers either)
@@ -234,7 +266,8 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
             if (tail && threadIdx.x == 0) look(p1 - 1);
         }
         const uint64_t key = where >= 0 ? key_of(most, (uint32_t)where) : 0;
-        const uint64_t group = greater<4>(greater<2>(greater<1>(key)));
+        uint64_t group = greater<2>(greater<1>(key));
+        if (kGroup == 8) group = greater<4>(group);
         if (lane % kGroup == 0) groups[threadIdx.x / kGroup] = group;
         if (threadIdx.x == 0) count = holding = 0;
         __syncthreads();
@@ -246,17 +279,36 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
         const uint64_t limit = bound;
         if (key >= limit && where >= 0) holders[atomicAdd(&holding, 1)] = (uint16_t)threadIdx.x;
         __syncthreads();
-        // every piece of the lanes whose own maximum reaches the bound, dealt over the workgroup, and the two that are broken
-        const int lanes = holding, turns = (whole1 - whole0 + kThreads - 1) / kThreads, items = lanes * max(turns, 0);
+        // every piece of the lanes whose own maximum reaches the bound, dealt over the workgroup (2^shift items a lane), and the two that are broken
+        const int turns = (whole1 - whole0 + kThreads - 1) / kThreads, shift = turns > 1 ? 32 - __builtin_clz(turns - 1) : 0, items = turns > 0 ? holding << shift : 0;
         const float least = value_of((uint32_t)(limit >> 32));
-        for (int i = threadIdx.x; i < items + 2; i += kThreads) {
-            const int q = i < items ? whole0 + holders[i % lanes] + i / lanes * kThreads : i == items ? (head ? 0 : -1) : (tail ? p1 - 1 : -1);
-            if (q < 0 || (i < items && q >= whole1)) continue;
-            each_of(q, [&](float v, uint32_t i) __attribute__((always_inline)) {
-                if (v < least || key_of(v, (uint32_t)q) < limit) return;
-                const int n = atomicAdd(&count, 1);
-                if (n < kMost) found[n] = key_of(v, i);
-            });
+        auto keep = [&](float v, int q, uint32_t i) __attribute__((always_inline)) {
+            if (v < least || key_of(v, (uint32_t)q) < limit) return;
+            const int n = atomicAdd(&count, 1);
+            if (n < kMost) found[n] = key_of(v, i);
+        };
+        for (int i0 = 0; i0 < items; i0 += 2 * kThreads) {
+            u32x4 w[2];
+            int q[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int i = min(i0 + j * kThreads + (int)threadIdx.x, items - 1);
+                q[j] = whole0 + holders[i >> shift] + (i & ((1 << shift) - 1)) * kThreads;
+                w[j] = base[min(q[j], whole1 - 1)];
+            }
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                if (i0 + j * kThreads >= items) break;
+                if (i0 + j * kThreads + (int)threadIdx.x >= items || q[j] >= whole1) continue;
+                float v[EPV];
+                widened(w[j], v);
+#pragma unroll
+                for (int e = 0; e < EPV; e++) keep(v[e], q[j], (uint32_t)(q[j] * EPV - off + e));
+            }
+        }
+        if ((head && threadIdx.x == 0) || (tail && threadIdx.x == 64)) {
+            const int q = threadIdx.x ? p1 - 1 : 0;
+            each_of(q, [&](float v, uint32_t i) __attribute__((always_inline)) { keep(v, q, i); });
         }
         __syncthreads();
         const int n = count;
@@ -294,9 +346,7 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
         }
     }
     __syncthreads();
-    s = wave_sums[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; w++) s = joined(s, wave_sums[w]);
+    if (wave == 0) s = joined(lane < kWaves ? wave_sums[lane] : Sums{-INFINITY, 0.f, 0.f});
 
     if (a.parts > 1) {
         float* to = reinterpret_cast<float*>(a.state + row * a.parts);
@@ -308,8 +358,11 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
         }
         if (a.top && wave == 0) __hip_atomic_store(lists + part * 64 + lane, list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (!arrive_last(a.words + row, a.parts, &last)) return;
-        s = Sums{-INFINITY, 0.f, 0.f};
-        for (int q = 0; q < a.parts; q++) s = joined(s, Sums{load_part(to + 4 * q), load_part(to + 4 * q + 1), load_part(to + 4 * q + 2)});
+        if (wave == 0) {
+            s = Sums{-INFINITY, 0.f, 0.f};
+            if (lane < a.parts) s = Sums{load_part(to + 4 * lane), load_part(to + 4 * lane + 1), load_part(to + 4 * lane + 2)};
+            s = joined(s);
+        }
         if (a.top) {
             list = 0;
             for (int q = wave; q < a.parts; q += kWaves) {
@@ -357,7 +410,7 @@ extern "C" int64_t mhip_token_log_probs_workspace(int64_t rows, int64_t vocab, i
 
 extern "C" int mhip_token_log_probs(void* stream, const void* logits, const void* tokens, float* log_probs, float* entropy, float* top_log_probs, int32_t* top_ids,
                                     int64_t rows, int64_t vocab, int top, int dtype, int token_dtype, void* workspace, int64_t workspace_bytes) {
-    if (rows < 0 || vocab <= 0 || vocab > (1 << 30)) return fail(MHIP_ERR_INVALID_ARGUMENT, "token_log_probs: %lld rows of %lld", (long long)rows, (long long)vocab);
+    if (rows < 0 || vocab <= 0 || vocab > (1 << 28)) return fail(MHIP_ERR_INVALID_ARGUMENT, "token_log_probs: %lld rows of %lld", (long long)rows, (long long)vocab);
     if (top < 0 || top > kMaxTop || top > vocab) return fail(MHIP_ERR_INVALID_ARGUMENT, "token_log_probs: %d alternatives of %lld (up to 64)", top, (long long)vocab);
     if (dtype != MHIP_BF16 && dtype != MHIP_F16 && dtype != MHIP_F32) return fail(MHIP_ERR_UNSUPPORTED, "token_log_probs: dtype %d (need bf16, f16 or f32)", dtype);
     if (token_dtype != MHIP_I32 && token_dtype != MHIP_I64) return fail(MHIP_ERR_UNSUPPORTED, "token_log_probs: token dtype %d (need i32 or i64)", token_dtype);
