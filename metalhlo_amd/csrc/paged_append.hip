@@ -82,6 +82,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
     if (b < 0) return;
     const int n = a.s.tokens(b), end = a.s.keys(b), begin = max(end - n, 0);          // (more tokens than keys: the first ones have no place)
     const int at = (begin >> shift) + (int)blockIdx.x - first;
+    if (at < begin >> shift || at << shift >= end) return;                            // (starts that are no starts: their sums may have wrapped)
     const int p0 = max(begin, at << shift), p1 = min(min(end, (at + 1) << shift), a.R ? a.positions : end);
     const int page_no = a.s.table[(int64_t)b * a.s.width + at];
     if (p0 >= p1) return;
@@ -298,7 +299,7 @@ int check_paged(const char* what, const mhip_paged_cache* c, const mhip_sequence
     if (c->head_size < 32 || c->head_size > 128 || c->head_size % 32) return fail(MHIP_ERR_UNSUPPORTED, "%s: head size %lld (need 32, 64, 96 or 128)", what, (long long)c->head_size);
     if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
         return fail(MHIP_ERR_UNSUPPORTED, "%s: page size %lld (need a power of two from 16 to 256)", what, (long long)c->page_size);
-    if (c->pages > INT32_MAX || c->heads > 1024 || s->sequences > 65536 || s->tokens > (1 << 24) || s->width > (1 << 20) || s->width * c->page_size > (1 << 24))
+    if (c->pages * c->heads > INT32_MAX || c->pages > INT32_MAX || c->heads > 1024 || s->sequences > 65536 || s->tokens > (1 << 24) || s->width > (1 << 20) || s->width * c->page_size > (1 << 24))
         return fail(MHIP_ERR_UNSUPPORTED, "%s: more than 65536 sequences, 2^24 tokens, 2^24 keys a sequence or 1024 heads", what);
     if (!c->key_scales != !c->value_scales) return fail(MHIP_ERR_INVALID_ARGUMENT, "%s: scales of keys without scales of values", what);
     if (s->sequences == 0 || s->tokens == 0) { *empty = true; return MHIP_OK; }
