@@ -12,6 +12,8 @@
 // fp32 sums, softmax state and scores (a key's scale is applied to its score in the first kernel, while it is converted in the second); probabilities are rounded to the queries' type in front of the second product,
 // whose error of half a step each (2^-9 for bf16) is below the result's own rounding once it is averaged over keys.  Values in 8 bits become the queries' type exactly,
 // scale and all, except that f16 ends at 65504 and at 2^-24.
+#include <algorithm>
+
 #include "arrive.h"
 #include "attention_common.h"
 #include "paged.h"
@@ -37,64 +39,79 @@ struct PagedArgs {
     const char *keys, *values;
     const uint8_t *key_scales, *value_scales;
     Sequences s;
-    int pages, KV, G, is_causal, target;
+    int pages, KV, G, is_causal, shares;
     float c;                                  // scale * log2(e)
     int64_t qs[2], os[2];                     // token and head strides in elements
     float* part;                              // workspace, NULL: keys are not dealt
     uint64_t* words;
     uint64_t tag;
-    Divider by_group, by_heads, by_shares;    // G, KV, target
-    int step_shift;                           // log2 of the keys of a step (few rows)
+    Divider by_group, by_heads, by_shares;    // G, KV, shares
+    int unit_shift;                           // log2 of the keys that one unit of the line stands for
 };
-
-// What a workgroup computes.
-struct Task { int b, tile, part, parts, k0, k1, first, tokens, keys; };
 
 constexpr int kMostParts = 64;
 
-// Unit u of the launch: tiles of ROWS rows of every sequence, times the parts of its keys.  Parts are a multiple of STEP keys.
-template <int ROWS, int STEP>
-__device__ __forceinline__ bool task_of(const PagedArgs& a, int u, Task& t) {
-    const int lane = threadIdx.x & 63;
-    int per = 1 << 28;                                                  // keys a part
-    auto tiles = [&](int b) __attribute__((always_inline)) { return (a.s.tokens(b) * a.G + ROWS - 1) / ROWS; };
-    if (a.part) {
-        float all = 0.f;
-        int most = 0;
-        for (int b = lane; b < a.s.B; b += 64) {
-            const int keys = a.s.keys(b);
-            all += (float)tiles(b) * (float)keys;
-            most = max(most, keys);
+// The work of a launch is one line: sequence by sequence, each head's and tile's own stretch as long as the work it stands for, and workgroup w takes the w-th share, which may be a part of one
+// tile's keys, or the end of one, several whole ones and the beginning of another.  Every workgroup has the same to do whatever the lengths, and leaves two parts at most.
+// The first `more` shares are per + 1 long, the others per.
+struct Line {
+    int per, more;
+    // `all`: the line's length; `longest`: a tile's stretch (one that were dealt over more than kMostParts workgroups would keep the last of them too long)
+    __device__ __forceinline__ Line(const Divider& by_shares, int shares, int all, int longest) {
+        per = by_shares(all);
+        more = all - per * shares;
+        if (per < 1 || longest > (kMostParts - 1) * per) {
+            per = (longest + kMostParts - 2) / (kMostParts - 1);
+            more = 0;
         }
-        all = wave_sum(all);
-        const int longest = (int)wave_max((float)most);
-        const float share = fminf(all * (float)a.KV / (float)a.target, (float)(1 << 27));
-        per = max((int)share, longest / kMostParts);
-        per = max((per + STEP) / STEP * STEP, 4 * STEP);
     }
-    auto parts_of = [&](int keys) __attribute__((always_inline)) { return max((keys + per - 1) / per, 1); };
-    auto units = [&](int b) __attribute__((always_inline)) { return tiles(b) * parts_of(a.s.keys(b)); };
-    int before;
-    t.b = sequence_of(a.s.B, u, units, before);
-    if (t.b < 0) return false;
-    t.tokens = __builtin_amdgcn_readfirstlane(a.s.tokens(t.b));
-    t.keys = __builtin_amdgcn_readfirstlane(a.s.keys(t.b));
-    t.first = __builtin_amdgcn_readfirstlane(a.s.start(t.b));
-    const int dealt = parts_of(t.keys), count = tiles(t.b), r = u - before;
-    if (r < 0 || r >= dealt * count) return false;                      // (starts that are no starts: their sums may have wrapped)
-    t.tile = count - 1 - r / dealt;                                     // (the longest first where the causal rule shortens them)
-    t.part = r % dealt;
-    int end = t.keys;                                                   // of the keys that the tile's last row sees
-    if (a.is_causal) {
-        const int last = a.by_group(min((t.tile + 1) * ROWS - 1, t.tokens * a.G - 1));
-        end = max(t.keys - t.tokens + last + 1, 0);
-    }
-    t.parts = parts_of(end);
-    if (t.part >= t.parts) return false;
-    t.k0 = t.part * per;
-    t.k1 = min(end, t.k0 + per);
-    return true;
+    __device__ __forceinline__ int begin(int w) const { return w * per + min(w, more); }
+    __device__ __forceinline__ int owner(int g) const { return g < more * (per + 1) ? g / (per + 1) : more + (g - more * (per + 1)) / per; }
+};
+
+// The first 64 sequences, in a wave's own LDS.
+struct Known { int start[64], tokens[64], keys[64]; };
+struct Found { int b, before, start, tokens, keys; };
+__device__ __forceinline__ void known_of(const Sequences& s, Known& known, int lane) {
+    known.start[lane] = lane < s.B ? s.start(lane) : 0;
+    known.tokens[lane] = lane < s.B ? s.tokens(lane) : 0;
+    known.keys[lane] = lane < s.B ? s.keys(lane) : 0;
 }
+// The sequence that place g of the line lies in, when one has stretch(tokens, keys) of it; `before`: where it begins.  False behind the last.
+template <typename F>
+__device__ __forceinline__ bool found_at(const Sequences& s, const Known& known, int lane, int g, F stretch, Found& at) {
+    const int mine = stretch(known.tokens[lane], known.keys[lane]), sum = wave_scan(mine);
+    int length;
+    if (const uint64_t m = __ballot(sum > g)) {
+        at.b = __builtin_ctzll(m);
+        at.before = __builtin_amdgcn_readlane(sum - mine, at.b);
+        length = __builtin_amdgcn_readlane(mine, at.b);
+        at.start = __builtin_amdgcn_readfirstlane(known.start[at.b]);
+        at.tokens = __builtin_amdgcn_readfirstlane(known.tokens[at.b]);
+        at.keys = __builtin_amdgcn_readfirstlane(known.keys[at.b]);
+    } else {
+        at.before = __builtin_amdgcn_readlane(sum, 63);
+        int further;
+        at.b = 64 + sequence_of(s.B - 64, g - at.before, [&](int i) { return stretch(s.tokens(64 + i), s.keys(64 + i)); }, further);
+        if (at.b < 64) return false;
+        at.before += further;
+        at.start = __builtin_amdgcn_readfirstlane(s.start(at.b));
+        at.tokens = __builtin_amdgcn_readfirstlane(s.tokens(at.b));
+        at.keys = __builtin_amdgcn_readfirstlane(s.keys(at.b));
+        length = stretch(at.tokens, at.keys);
+    }
+    return g >= at.before && g - at.before < length;                       // (starts that are no starts: their sums may have wrapped)
+}
+
+// The parts of a tile that is split: in workgroups `first` to first + parts - 1, the first one's at slot 2 first + 1 (the end of its share), the others' at 2 w (the beginning).
+struct Split { int first, parts; };
+__device__ __forceinline__ Split split_of(const Line& line, int shares, int share, int origin, int length) {
+    const int first = min(max(line.owner(origin), 0), share);
+    return {first, min(line.owner(origin + length - 1) - first + 1, min(kMostParts, shares - first))};
+}
+
+// Words at an address that is the same in all lanes, and that no launch writes while another reads them: read by scalar loads.
+typedef const __attribute__((address_space(4))) int32_t* uniform_words;
 
 // The page that holds key 16 `block` of sequence b, clamped to one that exists; `ok`: whether the table names it.
 __device__ __forceinline__ int page_of(const PagedArgs& a, const int32_t* table, int block, bool& ok) {
@@ -122,6 +139,32 @@ __device__ __forceinline__ u32x4 widen(u32x2 w, float scale) {
     return r;
 }
 
+// A key's value that is not finite makes the results of the rows that see it so, and of no others, but zero times it is no zero: where a result is not finite, the keys are
+// gone through once more with such values left out of the second product where some rows see them and others do not, and they are added to the rows behind it, one by one.
+template <typename T, bool EIGHT>
+__device__ __forceinline__ uint32_t tamed(uint32_t w, bool& any) {
+    uint32_t wild;                                                         // the top bit of each that is not finite
+    if constexpr (EIGHT) wild = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+    else if constexpr (std::is_same<T, bf16_t>::value) wild = ((w & 0x7FFF7FFFu) + 0x00800080u) & 0x80008000u;
+    else wild = ((w & 0x7FFF7FFFu) + 0x04000400u) & 0x80008000u;
+    any |= wild != 0;
+    return w & ~(EIGHT ? (wild >> 7) * 0xFFu : (wild >> 15) * 0xFFFFu);
+}
+// what a value adds to a result besides
+template <typename T, bool EIGHT>
+__device__ __forceinline__ float wild_of(const char* p) {
+    if constexpr (EIGHT) return (*reinterpret_cast<const uint8_t*>(p) & 0x7F) == 0x7F ? __builtin_nanf("") : 0.f;
+    const float x = Elem<T>::to_f32(*reinterpret_cast<const T*>(p));
+    return fabsf(x) < INFINITY ? 0.f : x;
+}
+// where key `key` of head `head` has its d = 0 in the values, NULL where the table names no page; from one d to the next it is sixteen values
+template <int D, int SIZE>
+__device__ __forceinline__ const char* value_at(const PagedArgs& a, const int32_t* table, int head, int key) {
+    bool ok;
+    const int page = page_of(a, table, key >> 4, ok), blocks = a.s.page_shift - 4;
+    return ok ? a.values + (((((int64_t)page * a.KV + head) << blocks) + ((key >> 4) & ((1 << blocks) - 1))) * (16 * D) + (key & 15)) * SIZE : nullptr;
+}
+
 template <typename T> struct Mfma16P;
 template <> struct Mfma16P<bf16_t> {
     __device__ static f32x4 run(u32x4 a, u32x4 b, f32x4 c) {
@@ -134,11 +177,11 @@ template <> struct Mfma16P<f16_t> {
     }
 };
 
-// Parts of a tile of ROWS rows: [unit * KV + head][ROWS][D] sums, then [..][ROWS] pairs of reference maximum and sum.
+// Parts of a tile of ROWS rows: [slot][ROWS][D] sums, then [slot][ROWS] pairs of reference maximum and sum; two slots a workgroup.
 template <int ROWS, int D>
 struct Parts {
     float *sums, *state;
-    __device__ Parts(const PagedArgs& a, int slot, int64_t slots) : sums(a.part + (int64_t)slot * ROWS * D), state(a.part + slots * ROWS * D + (int64_t)slot * ROWS * 2) {}
+    __device__ __forceinline__ Parts(const PagedArgs& a, int slot) : sums(a.part + (int64_t)slot * ROWS * D), state(a.part + 2 * (int64_t)a.shares * ROWS * D + (int64_t)slot * ROWS * 2) {}
 };
 
 __device__ __forceinline__ void store_two(float* p, float x, float y) {
@@ -149,11 +192,10 @@ __device__ __forceinline__ u32x2 load_two(const float* p) {
     return u32x2{(uint32_t)v, (uint32_t)(v >> 32)};
 }
 
-// By the last workgroup of a tile: its parts put together in order; part i is at slot `slot0` + `apart` i, from the second on `shift` further.
+// By the last workgroup of a tile: its parts put together in order.  `rows`: of the tile, from row `row0` of the sequence that starts at token `start`.
 template <typename T, int ROWS, int D, int THREADS>
-__device__ __forceinline__ void join(const PagedArgs& a, const Task& t, int head, int slot0, int apart, int shift, int64_t slots) {
+__device__ __forceinline__ void join(const PagedArgs& a, const Split& split, int start, int head, int row0, int rows) {
     constexpr int kFours = D / 4;
-    const int rows = min(ROWS, t.tokens * a.G - t.tile * ROWS);
     // AHEAD parts are asked for at once: up to 16 of them arrive after one latency
     auto put = [&](auto ahead) __attribute__((always_inline)) {
         constexpr int AHEAD = decltype(ahead)::value;
@@ -161,40 +203,39 @@ __device__ __forceinline__ void join(const PagedArgs& a, const Task& t, int head
             const int row = idx / kFours, four = idx % kFours;
             float m = -INFINITY, l = 0.f;
             f32x4 o = {0.f, 0.f, 0.f, 0.f};
-            for (int p0 = 0; p0 < t.parts; p0 += AHEAD) {
+            for (int p0 = 0; p0 < split.parts; p0 += AHEAD) {
                 u32x2 st[AHEAD];
                 f32x4 v[AHEAD];
 #pragma unroll
                 for (int p = 0; p < AHEAD; p++) {
-                    const int q = min(p0 + p, t.parts - 1);
-                    const Parts<ROWS, D> at(a, slot0 + q * apart + (q ? shift : 0), slots);
+                    const int q = min(p0 + p, split.parts - 1);
+                    const Parts<ROWS, D> at(a, 2 * (split.first + q) + (q ? 0 : 1));
                     st[p] = load_two(at.state + 2 * row);
                     v[p] = load_part(parts_rsrc(at.sums), (uint32_t)((row * kFours + four) * 16));
                 }
                 float top = m;
 #pragma unroll
-                for (int p = 0; p < AHEAD; p++) top = fmaxf(top, p0 + p < t.parts ? __builtin_bit_cast(float, (uint32_t)st[p].x) : -INFINITY);
+                for (int p = 0; p < AHEAD; p++) top = fmaxf(top, p0 + p < split.parts ? __builtin_bit_cast(float, (uint32_t)st[p].x) : -INFINITY);
                 const float use = top == -INFINITY ? 0.f : top, old = weight(m, use);
                 m = top;
                 l *= old;
                 o *= old;
 #pragma unroll
                 for (int p = 0; p < AHEAD; p++) {
-                    const float al = p0 + p < t.parts ? weight(__builtin_bit_cast(float, (uint32_t)st[p].x), use) : 0.f;
+                    const float al = p0 + p < split.parts ? weight(__builtin_bit_cast(float, (uint32_t)st[p].x), use) : 0.f;
                     l = fmaf(__builtin_bit_cast(float, (uint32_t)st[p].y), al, l);
 #pragma unroll
                     for (int e = 0; e < 4; e++) o[e] = fmaf(v[p][e], al, o[e]);
                 }
             }
             const float inv = l != 0.f ? 1.f / l : 0.f;
-            const int r = t.tile * ROWS + row;
-            const int token = a.by_group(r);
-            T* out = static_cast<T*>(a.o) + (int64_t)(t.first + token) * a.os[0] + (int64_t)(head * a.G + r - token * a.G) * a.os[1] + 4 * four;
+            const int r = row0 + row, token = a.by_group(r);
+            T* out = static_cast<T*>(a.o) + (int64_t)(start + token) * a.os[0] + (int64_t)(head * a.G + r - token * a.G) * a.os[1] + 4 * four;
             *reinterpret_cast<u32x2*>(out) = u32x2{Mfma32A<T>::pack2(o[0] * inv, o[1] * inv), Mfma32A<T>::pack2(o[2] * inv, o[3] * inv)};
         }
     };
-    if (t.parts <= 4) put(std::integral_constant<int, 4>{});
-    else if (t.parts <= 8 || ROWS > 32) put(std::integral_constant<int, 8>{});
+    if (split.parts <= 4) put(std::integral_constant<int, 4>{});
+    else if (split.parts <= 8 || ROWS > 32) put(std::integral_constant<int, 8>{});
     else put(std::integral_constant<int, 16>{});
 }
 
@@ -207,87 +248,57 @@ __device__ __forceinline__ void join(const PagedArgs& a, const Task& t, int head
 //                  they are those whose probabilities the lane has just computed.
 // Two blocks are in registers or on their way; K of the next but one is asked for behind this one's scores, V behind its second product.
 //
-// The keys of the launch are one line of steps of 256 keys (more where there were over 2^29 of them): sequence by sequence, tile by tile, head by head.  Workgroup w takes the w-th share of the line, which may be a part of one
-// head's keys, or the end of one, several whole ones and the beginning of another: every workgroup has the same to read, whatever the lengths.
+// SINGLE: no sequence has more tokens than its place among as many others suggests, one, and a tile is one token's G rows, which see the same keys; else the rows of a tile may see
+// different numbers of them.
+//
+// The line is in steps of 256 keys (more where there were over 2^29 of them), tile by tile and head by head.
 constexpr int kStepShift = 8;
 
 // Workgroups of a unit: what the registers allow, and what the launch counts on.
-constexpr int rows_kernel_workgroups(int tiles, int64_t D) { return tiles == 1 ? 2 : (D <= 64 ? 2 : 1); }
+constexpr int rows_kernel_workgroups(int tiles, int64_t D, bool single) { return tiles == 1 ? (D <= 64 && single ? 3 : 2) : (D <= 64 ? 2 : 1); }
 
-// The line and its shares: the first `more` workgroups have per + 1 steps, the others per.
-struct Line {
-    int per, more;
-    __device__ __forceinline__ int begin(int w) const { return w * per + min(w, more); }
-    __device__ __forceinline__ int owner(int g) const { return g < more * (per + 1) ? g / (per + 1) : more + (g - more * (per + 1)) / per; }
-};
-
-template <typename T, int D, bool EIGHT, int TILES, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void paged_rows_kernel(PagedArgs a) {
+template <typename T, int D, bool EIGHT, int TILES, int WAVES, bool SINGLE>
+__global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE)) void paged_rows_kernel(PagedArgs a) {
     constexpr int ROWS = 16 * TILES, kLane = EIGHT ? 16 : 8, NT = kLane / 4, kKeys = 4 * kLane, kBlocks = kKeys / kBlock;
     constexpr int NS = D / 32, NF = D / 16, SIZE = EIGHT ? 1 : 2;
     constexpr int KD = D * SIZE / 16;                       // dwords of a key that a lane holds
     static_assert((1 << kStepShift) % (WAVES * kKeys) == 0, "a step is the same number of blocks for every wave");
     __shared__ __attribute__((aligned(16))) float sums[WAVES][TILES][NF][64][4];
     __shared__ float ml[2][WAVES][ROWS];
+    constexpr bool kQueriesInLds = TILES == 1 && (EIGHT || !SINGLE);      // (what else does not fit the registers)
+    __shared__ __attribute__((aligned(16))) u32x4 queries[kQueriesInLds ? WAVES : 1][NS][64];
     __shared__ int last;
-    // (read by scalar loads)
-    typedef const __attribute__((address_space(4))) int32_t* uniform_words;
     auto scale_word = [](const uint8_t* scales, int at) __attribute__((always_inline)) { return (uint32_t)*(uniform_words)((uintptr_t)(scales + at) & ~(uintptr_t)3); };
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, lg = lane >> 4;
 
-    // ---- this workgroup's share of the line.  A wave keeps the first 64 sequences in LDS
-    __shared__ int known[WAVES][3][64];                                       // (a wave's own copy: nobody waits)
-    auto tiles_of = [&](int tokens) __attribute__((always_inline)) { return (tokens * a.G + ROWS - 1) / ROWS; };
-    auto steps_of = [&](int keys) __attribute__((always_inline)) { return max((keys + (1 << a.step_shift) - 1) >> a.step_shift, 1); };
-    const int own_start = lane < a.s.B ? a.s.start(lane) : 0, own_tokens = lane < a.s.B ? a.s.tokens(lane) : 0, own_keys = lane < a.s.B ? a.s.keys(lane) : 0;
-    known[wave][0][lane] = own_start;
-    known[wave][1][lane] = own_tokens;
-    known[wave][2][lane] = own_keys;
-    int longest = own_tokens ? steps_of(own_keys) : 1, steps = own_tokens ? tiles_of(own_tokens) * steps_of(own_keys) : 0;
-    for (int b = 64 + lane; b < a.s.B; b += 64)
-        if (const int tokens = a.s.tokens(b)) {
-            const int n = steps_of(a.s.keys(b));
-            longest = max(longest, n);
-            steps += tiles_of(tokens) * n;
-        }
+    // ---- this workgroup's share of the line
+    __shared__ Known known[WAVES];
+    known_of(a.s, known[wave], lane);
+    const int tile_rows = SINGLE ? a.G : ROWS;
+    auto tiles_of = [&](int tokens) __attribute__((always_inline)) { return SINGLE ? tokens : (tokens * a.G + ROWS - 1) / ROWS; };
+    auto steps_of = [&](int keys) __attribute__((always_inline)) { return max((keys + (1 << a.unit_shift) - 1) >> a.unit_shift, 1); };
+    int longest = 1, steps = 0;
+    auto count = [&](int tokens, int keys) __attribute__((always_inline)) {
+        const int n = steps_of(keys);
+        if (tokens) longest = max(longest, n);
+        steps += tiles_of(tokens) * n;
+    };
+    count(known[wave].tokens[lane], known[wave].keys[lane]);
+    for (int b = 64 + lane; b < a.s.B; b += 64) count(a.s.tokens(b), a.s.keys(b));
     longest = (int)wave_max((float)longest);                                  // of one sequence (exact: at most 2^16)
     steps = __builtin_amdgcn_readlane(wave_scan(steps), 63) * a.KV;           // of all heads
-    Line line;
-    line.per = a.by_shares(steps);
-    line.more = steps - line.per * a.target;
-    if (line.per < 1 || longest > (kMostParts - 1) * line.per) {
-        line.per = (longest + kMostParts - 2) / (kMostParts - 1);
-        line.more = 0;
-    }
+    const Line line(a.by_shares, a.shares, steps, longest);
     int g = line.begin(blockIdx.x);
     const int stop = min(line.begin(blockIdx.x + 1), steps);
     const int page_bytes = (D * SIZE) << a.s.page_shift;
 
     for (int segment = 0; g < stop; segment++) {
         // ---- the head that step g belongs to
-        int before, b, tokens, keys, first;
-        {
-            const int n = known[wave][1][lane], units = n ? tiles_of(n) * a.KV * steps_of(known[wave][2][lane]) : 0, sum = wave_scan(units);
-            if (const uint64_t m = __ballot(sum > g)) {
-                b = __builtin_ctzll(m);
-                before = __builtin_amdgcn_readlane(sum - units, b);
-                first = __builtin_amdgcn_readfirstlane(known[wave][0][b]);
-                tokens = __builtin_amdgcn_readfirstlane(known[wave][1][b]);
-                keys = __builtin_amdgcn_readfirstlane(known[wave][2][b]);
-            } else {
-                before = __builtin_amdgcn_readlane(sum, 63);
-                int further;
-                b = 64 + sequence_of(a.s.B - 64, g - before, [&](int i) { return a.s.tokens(64 + i) ? tiles_of(a.s.tokens(64 + i)) * a.KV * steps_of(a.s.keys(64 + i)) : 0; }, further);
-                if (b < 64) return;
-                before += further;
-                first = __builtin_amdgcn_readfirstlane(a.s.start(b));
-                tokens = __builtin_amdgcn_readfirstlane(a.s.tokens(b));
-                keys = __builtin_amdgcn_readfirstlane(a.s.keys(b));
-            }
-        }
-        if (g < before || g - before >= tiles_of(tokens) * a.KV * steps_of(keys)) return;     // (starts that are no starts: their sums may have wrapped)
-        const int mine = steps_of(keys), pair = (g - before) / mine, s0 = g - before - pair * mine;
+        Found at;
+        if (!found_at(a.s, known[wave], lane, g, [&](int tokens, int keys) { return tiles_of(tokens) * a.KV * steps_of(keys); }, at)) return;
+        const int b = at.b, tokens = at.tokens, keys = at.keys, first = at.start;
+        const int mine = steps_of(keys), pair = (g - at.before) / mine, s0 = g - at.before - pair * mine;
         if (!a.part && s0) {                                                  // without a workspace a head is its beginning's, whole
             g += mine - s0;
             continue;
@@ -297,18 +308,12 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
         g += s1 - s0;
         const int rows = tokens * a.G;
         int end = keys;                                                       // of the keys that the tile's last row sees
-        if (a.is_causal) end = max(keys - tokens + a.by_group(min((tile + 1) * ROWS, rows) - 1) + 1, 0);
-        const int k0 = s0 << a.step_shift, k1 = min(end, s1 << a.step_shift);
-        const bool split = s1 - s0 < mine;
-        const int owner0 = split ? min(max(line.owner(origin), 0), (int)blockIdx.x) : 0;
-        const int parts = split ? min(line.owner(origin + mine - 1) - owner0 + 1, min(kMostParts, (int)gridDim.x - owner0)) : 1;
-        uint64_t* word = nullptr;
+        if (a.is_causal) end = max(keys - tokens + a.by_group(min((tile + 1) * tile_rows, rows) - 1) + 1, 0);
+        const int k0 = s0 << a.unit_shift, k1 = min(end, s1 << a.unit_shift);
+        const bool parted = s1 - s0 < mine;
+        const Split split = parted ? split_of(line, a.shares, blockIdx.x, origin, mine) : Split{0, 1};
         uint64_t seen = 0;
-        if (split) {
-            // a split head begins in workgroup owner0 and is the only one to do so without ending there
-            word = a.words + owner0;
-            if (threadIdx.x == 0) seen = arrive_look(word);
-        }
+        if (parted && threadIdx.x == 0) seen = arrive_look(a.words + split.first);
 
         // ---- queries: row li of each tile.  d of step s: see d_of
         auto d_of = [&](int s) __attribute__((always_inline)) {
@@ -320,14 +325,23 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
         int open = k1;                                                       // the least of them: blocks in front of it need no mask
 #pragma unroll
         for (int x = 0; x < TILES; x++) {
-            const int row = tile * ROWS + 16 * x + li, token = a.by_group(row);
+            const int row = tile * tile_rows + 16 * x + li, token = a.by_group(row);
+            const bool mine = row < rows && (!SINGLE || 16 * x + li < a.G);
             const T* qp = static_cast<const T*>(a.q) + (int64_t)(first + token) * a.qs[0] + (int64_t)(head * a.G + row - token * a.G) * a.qs[1];
 #pragma unroll
-            for (int s = 0; s < NS; s++) qf[x][s] = row < rows ? *reinterpret_cast<const u32x4*>(qp + d_of(s)) : u32x4{0, 0, 0, 0};
-            limit[x] = min(a.is_causal ? keys - tokens + token + 1 : keys, k1);
-            open = min(open, row < rows ? limit[x] : k1);
+            for (int s = 0; s < NS; s++) qf[x][s] = mine ? *reinterpret_cast<const u32x4*>(qp + d_of(s)) : u32x4{0, 0, 0, 0};
+            limit[x] = SINGLE ? k1 : min(a.is_causal ? keys - tokens + token + 1 : keys, k1);
+            open = min(open, mine ? limit[x] : k1);
         }
-        open = -(int)wave_max((float)-open);
+        if (!SINGLE) open = -(int)wave_max((float)-open);
+        if constexpr (kQueriesInLds) {
+#pragma unroll
+            for (int s = 0; s < NS; s++) queries[wave][s][lane] = qf[0][s];
+        }
+        auto query = [&](int x, int s) __attribute__((always_inline)) {
+            if constexpr (kQueriesInLds) return queries[wave][s][lane];
+            else return qf[x][s];
+        };
 
         uniform_words table = (uniform_words)(uintptr_t)(a.s.table + (int64_t)b * a.s.width);
         // where the sixteen-token blocks of a block of keys lie, in keys and in values alike; bit i of `absent`: the table names no page for block i
@@ -341,7 +355,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
                 const bool ok = (uint32_t)p.page[i] < (uint32_t)a.pages;
                 p.absent |= ok ? 0u : 1u << i;
                 p.page[i] = (ok ? p.page[i] : 0) * a.KV + head;
-                if (EIGHT) {                                                    // the aligned words that hold the two bytes; taken apart where they are used, so that nothing waits for them here
+                if (EIGHT) {                                                    // the aligned words that hold the two bytes; nothing waits for them here
                     p.ks[i] = scale_word(a.key_scales, p.page[i]);
                     p.vs[i] = scale_word(a.value_scales, p.page[i]);
                 }
@@ -355,7 +369,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
         };
         const int key_block = kLane * (li >> 2) / kBlock, value_block = kLane * lg / kBlock;
         const int key_off = ((kLane * (li >> 2) % kBlock) + (li & 3)) * (D * SIZE) + 16 * lg, value_off = li * (16 * SIZE) + kLane * lg % kBlock * SIZE;
-        struct Block { uint32_t k[NT][KD], v[NF][4]; Place p; };
+        struct Block { uint32_t k[NT][KD], v[NF][4], ks, vs, absent; };           // (scales: a byte for each of its kBlocks)
         auto load_k = [&](Block& blk, const Place& p) __attribute__((always_inline)) {
             const char* kp = a.keys + chosen(p.at, key_block) + key_off;
 #pragma unroll
@@ -374,7 +388,15 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
                     blk.k[j][KD - 1] = w.y;
                 }
             }
-            blk.p = p;
+            blk.ks = blk.vs = 0;
+            if (EIGHT) {
+#pragma unroll
+                for (int i = 0; i < kBlocks; i++) {
+                    blk.ks |= (p.ks[i] >> 8 * ((uint32_t)(uintptr_t)(a.key_scales + p.page[i]) & 3) & 255) << 8 * i;
+                    blk.vs |= (p.vs[i] >> 8 * ((uint32_t)(uintptr_t)(a.value_scales + p.page[i]) & 3) & 255) << 8 * i;
+                }
+            }
+            blk.absent = p.absent;
         };
         auto load_v = [&](Block& blk, const Place& p) __attribute__((always_inline)) {
             const char* vp = a.values + chosen(p.at, value_block) + value_off;
@@ -388,26 +410,25 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
 
         f32x4 oacc[TILES][NF];
         float m_run[TILES], l_run[TILES];
+        auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int x = 0; x < TILES; x++) {
-            m_run[x] = -INFINITY;
-            l_run[x] = 0.f;
+            for (int x = 0; x < TILES; x++) {
+                m_run[x] = -INFINITY;
+                l_run[x] = 0.f;
 #pragma unroll
-            for (int f = 0; f < NF; f++) oacc[x][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        // the scale of this quarter's keys or values
-        auto scale_at = [&](const Place& p, const uint32_t (&words)[kBlocks], const uint8_t* scales) __attribute__((always_inline)) {
-            uint32_t bytes[kBlocks];
-#pragma unroll
-            for (int i = 0; i < kBlocks; i++) bytes[i] = max(words[i] >> 8 * ((uint32_t)(uintptr_t)(scales + p.page[i]) & 3) & 255, 1u) << 23;
-            return __builtin_bit_cast(float, chosen(bytes, value_block));
+                for (int f = 0; f < NF; f++) oacc[x][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
         };
+        clear();
+        bool tame = false;
+        // the scale of this quarter's keys or values
+        auto scale_at = [&](uint32_t bytes) __attribute__((always_inline)) { return scale_of(bytes >> 8 * value_block & 255); };
         // scores and probabilities of a block
         auto scored = [&](const Block& blk, int key, u32x4 (&pb)[TILES][NT / 2]) __attribute__((always_inline)) {
             const int at = key + kLane * lg;                                // first key of this quarter
-            const bool masked = key + kKeys > open || blk.p.absent;
-            const bool ok = !(blk.p.absent >> value_block & 1);
-            const float c = EIGHT ? a.c * scale_at(blk.p, blk.p.ks, a.key_scales) : a.c;
+            const bool masked = key + kKeys > open || blk.absent;
+            const bool ok = !(blk.absent >> value_block & 1);
+            const float c = EIGHT ? a.c * scale_at(blk.ks) : a.c;
             float sv[TILES][4 * NT];
 #pragma unroll
             for (int j = 0; j < NT; j++) {
@@ -421,7 +442,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
                 for (int x = 0; x < TILES; x++) {
                     f32x4 s4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int s = 0; s < NS; s++) s4 = Mfma16P<T>::run(kf[s], qf[x][s], s4);
+                    for (int s = 0; s < NS; s++) s4 = Mfma16P<T>::run(kf[s], query(x, s), s4);
 #pragma unroll
                     for (int r = 0; r < 4; r++) sv[x][4 * j + r] = s4[r] * c;
                 }
@@ -457,10 +478,10 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
                 for (int e = 0; e < 2 * NT; e++) pb[x][e >> 2][e & 3] = Mfma32A<T>::pack2(sv[x][2 * e], sv[x][2 * e + 1]);
             }
         };
-        auto added = [&](Block& blk, int key, const u32x4 (&pb)[TILES][NT / 2], const Place& p) __attribute__((always_inline)) {
-            if (key + kKeys > k1 || p.absent) {
+        auto added = [&](Block& blk, int key, const u32x4 (&pb)[TILES][NT / 2], uint32_t vs8, uint32_t absent) __attribute__((always_inline)) {
+            if (key + kKeys > k1 || absent) {
                 // values that no key of this part stands for may hold anything, a NaN among it
-                const int n = p.absent >> value_block & 1 ? 0 : k1 - key - kLane * lg;
+                const int n = absent >> value_block & 1 ? 0 : k1 - key - kLane * lg;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     constexpr int kPer = 4 / SIZE;
@@ -470,7 +491,14 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
                     for (int f = 0; f < NF; f++) blk.v[f][e] &= keep;
                 }
             }
-            const float vs = EIGHT ? scale_at(p, p.vs, a.value_scales) : 1.f;
+            if (!SINGLE && tame && key + kKeys > open) {
+                bool wild = false;
+#pragma unroll
+                for (int f = 0; f < NF; f++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) blk.v[f][e] = tamed<T, EIGHT>(blk.v[f][e], wild);
+            }
+            const float vs = EIGHT ? scale_at(vs8) : 1.f;
 #pragma unroll
             for (int f = 0; f < NF; f++)
 #pragma unroll
@@ -493,28 +521,60 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
                 if (next) ask(p, key_of(min(i + 2, blocks - 1)));             // (a block behind the last is the last again)
                 scored(blk, key_of(i), pb);
                 __builtin_amdgcn_sched_barrier(0);
-                const Place was = blk.p;
+                const uint32_t vs8 = blk.vs, absent = blk.absent;
                 if (next) load_k(blk, p);
-                added(blk, key_of(i), pb, was);
+                added(blk, key_of(i), pb, vs8, absent);
                 __builtin_amdgcn_sched_barrier(0);
                 if (next) load_v(blk, p);
             };
-            ask(p, start);
-            load_k(one, p);
-            load_v(one, p);
-            ask(p, key_of(min(1, blocks - 1)));
-            load_k(two, p);
-            load_v(two, p);
-            int i = 0;
-            for (; i + 2 < blocks; i += 2) {
-                attend(one, i, 1);
-                attend(two, i + 1, 1);
+            for (;;) {
+                ask(p, start);
+                load_k(one, p);
+                load_v(one, p);
+                ask(p, key_of(min(1, blocks - 1)));
+                load_k(two, p);
+                load_v(two, p);
+                int i = 0;
+                for (; i + 2 < blocks; i += 2) {
+                    attend(one, i, 1);
+                    attend(two, i + 1, 1);
+                }
+                attend(one, i, 0);
+                if (i + 1 < blocks) attend(two, i + 1, 0);
+                if (SINGLE || open >= k1 || tame) break;
+                bool odd = false;
+#pragma unroll
+                for (int x = 0; x < TILES; x++)
+#pragma unroll
+                    for (int f = 0; f < NF; f++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) odd |= !(fabsf(oacc[x][f][r]) < INFINITY);
+                if (!__any(odd)) break;
+                tame = true;                                                  // (see `tamed`)
+                clear();
             }
-            attend(one, i, 0);
-            if (i + 1 < blocks) attend(two, i + 1, 0);
+            if (!SINGLE && tame) {
+#pragma unroll 1
+                for (int i = 0; i < blocks; i++) {
+                    if (key_of(i) + kKeys <= open) continue;
+#pragma unroll 1
+                    for (int kk = key_of(i); kk < min(key_of(i) + kKeys, k1); kk++) {
+                        const char* vp = value_at<D, SIZE>(a, a.s.table + (int64_t)b * a.s.width, head, kk);
+                        if (!vp) continue;
+#pragma unroll
+                        for (int f = 0; f < NF; f++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                const float w = wild_of<T, EIGHT>(vp + (16 * f + 4 * lg + r) * (16 * SIZE));
+#pragma unroll
+                                for (int x = 0; x < TILES; x++) oacc[x][f][r] += kk < limit[x] ? w : 0.f;
+                            }
+                    }
+                }
+            }
         }
 
-        if (split && threadIdx.x == 0) arrive_claim(word, seen, a.tag);
+        if (parted && threadIdx.x == 0) arrive_claim(a.words + split.first, seen, a.tag);
         // ---- the waves' states, four sums a thread: O^T tile f holds d = 16 f + 4 g + e of group g
         if (segment) __syncthreads();                                        // (the segment before has been read)
 #pragma unroll
@@ -528,9 +588,8 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
         }
         __syncthreads();
         constexpr int kFours = D / 4;
-        const int here = min(ROWS, rows - tile * ROWS);
-        // a workgroup leaves at most two parts: the end of a head that began in front of its share, and the beginning of one that ends behind it
-        const Parts<ROWS, D> own(a, 2 * (int)blockIdx.x + (s0 ? 0 : 1), 2 * (int64_t)gridDim.x);
+        const int here = min(tile_rows, rows - tile * tile_rows);
+        const Parts<ROWS, D> own(a, 2 * (int)blockIdx.x + (s0 ? 0 : 1));
         for (int idx = threadIdx.x; idx < here * kFours; idx += 64 * WAVES) {
             const int row = idx / kFours, four = idx % kFours;
             float m = -INFINITY, l = 0.f;
@@ -546,9 +605,9 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[e] = fmaf(v[e], al, o[e]);
             }
-            if (!split) {
+            if (!parted) {
                 const float inv = l != 0.f ? 1.f / l : 0.f;
-                const int r = tile * ROWS + row, token = a.by_group(r);
+                const int r = tile * tile_rows + row, token = a.by_group(r);
                 T* out = static_cast<T*>(a.o) + (int64_t)(first + token) * a.os[0] + (int64_t)(head * a.G + r - token * a.G) * a.os[1] + 4 * four;
                 *reinterpret_cast<u32x2*>(out) = u32x2{Mfma32A<T>::pack2(o[0] * inv, o[1] * inv), Mfma32A<T>::pack2(o[2] * inv, o[3] * inv)};
             } else {
@@ -556,9 +615,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D)) void 
                 if (four == 0) store_two(own.state + 2 * row, m, l);
             }
         }
-        if (!split || !arrive_last(word, parts, &last)) continue;
-        const Task t{b, tile, 0, parts, 0, 0, first, tokens, keys};
-        join<T, ROWS, D, 64 * WAVES>(a, t, head, 2 * owner0 + 1, 2, -1, 2 * (int64_t)gridDim.x);
+        if (parted && arrive_last(a.words + split.first, split.parts, &last)) join<T, ROWS, D, 64 * WAVES>(a, split, first, head, tile * tile_rows, here);
     }
 }
 
@@ -579,92 +636,196 @@ __device__ __forceinline__ uint32_t tv_off(int d, int chunk) {            // V^T
     return (uint32_t)(d * 128 + ((chunk ^ ((d >> 1) & 7)) << 4));
 }
 
+// The line's stretches: a tile's is its keys and what a tile costs besides (kTileCost keys' worth), which grows from tile to tile by the tokens of one where the causal rule holds; head by head.
+constexpr int kTileCost = 128;
+struct Stretch {
+    int tiles, first, grows;
+    __device__ __forceinline__ Stretch(const PagedArgs& a, int tokens, int keys) {
+        const int wide = (kTileRows + a.G - 1) / a.G;
+        tiles = (tokens * a.G + kTileRows - 1) / kTileRows;
+        first = (((a.is_causal ? max(keys - tokens, 0) + wide : keys) + kTileCost) >> a.unit_shift) + 1;
+        grows = a.is_causal ? wide >> a.unit_shift : 0;
+    }
+    __device__ __forceinline__ int before(int t) const { return t * first + grows * (t * (t - 1) / 2); }
+    __device__ __forceinline__ int length(int t) const { return first + grows * t; }
+    // the tile that place x lies in
+    __device__ __forceinline__ int tile(int x) const {
+        const float f = (float)first - 0.5f * (float)grows;
+        int t = grows ? (int)((__builtin_sqrtf(f * f + 2.f * (float)grows * (float)x) - f) / (float)grows) : x / first;
+        t = min(max(t, 0), tiles - 1);
+        while (t > 0 && before(t) > x) t--;
+        while (t < tiles - 1 && before(t + 1) <= x) t++;
+        return __builtin_amdgcn_readfirstlane(t);
+    }
+};
+
 template <typename T, int D, bool EIGHT>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
     constexpr int NS = D / 16, NF = D / 32, SIZE = EIGHT ? 1 : 2;
     constexpr int kKBytes = D == 96 ? 64 * 208 : 64 * D * 2, kVBytes = D * 128;
     constexpr int kPieces = 64 * D * SIZE / 16, kMine = (kPieces + 255) / 256;      // pieces of sixteen bytes of K, and of V, of a stage; a thread's
     __shared__ __attribute__((aligned(16))) char lds[2][kKBytes + kVBytes];
+    __shared__ Known known[4];
     __shared__ int last;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 31, lh = lane >> 5;
-    const int unit = a.by_heads(blockIdx.x), head = blockIdx.x - unit * a.KV;
-    Task t;
-    if (!task_of<kTileRows, kStage>(a, unit, t)) return;
-    const int slot0 = (unit - t.part) * a.KV + head;
-    uint64_t seen = 0;
-    if (t.parts > 1 && threadIdx.x == 0) seen = arrive_look(a.words + slot0);
 
-    const int rows = t.tokens * a.G, row = t.tile * kTileRows + 32 * wave + li, token = a.by_group(row);
+    // ---- this workgroup's share of the line.  Eight neighbours of the launch, which are on eight XCDs, take shares an eighth of the line apart: what an XCD's workgroups read at a time belongs to few heads
+    known_of(a.s, known[wave], lane);
+    int longest = 1, shortest = 1 << 30, all = 0, count = 0;
+    auto add = [&](int tokens, int keys) __attribute__((always_inline)) {
+        const Stretch st(a, tokens, keys);
+        if (!st.tiles) return;
+        longest = max(longest, st.length(st.tiles - 1));
+        shortest = min(shortest, st.first);
+        all += st.before(st.tiles);
+        count += st.tiles;
+    };
+    add(known[wave].tokens[lane], known[wave].keys[lane]);
+    for (int b = 64 + lane; b < a.s.B; b += 64) add(a.s.tokens(b), a.s.keys(b));
+    longest = (int)(wave_max((float)longest) * 1.00001f) + 1;
+    shortest = -(int)wave_max((float)-shortest);
+    all = __builtin_amdgcn_readlane(wave_scan(all), 63) * a.KV;
+    count = __builtin_amdgcn_readlane(wave_scan(count), 63) * a.KV;
+    // Where there is a tile for every share, and short ones that come last and fill the gaps (a prompt from its beginning), a workgroup takes one whole tile instead, and none is joined; so it does
+    // without a workspace.  us, shares | tiles: four prompts of 2048 tokens 270 | 196, one of 4000 199 | 180; three pieces of 550 to 930 tokens behind 5000 to 7000 304 | 480
+    const bool tiles = !a.part || (count >= a.shares && shortest <= 5 * kTileCost >> a.unit_shift);
+    const Line line(a.by_shares, a.shares, all, longest);
+    if ((int)blockIdx.x >= (tiles ? count : a.shares)) return;
+    const int share = a.shares & 7 ? blockIdx.x : (blockIdx.x & 7) * (a.shares >> 3) + (blockIdx.x >> 3);
+    int g = tiles ? 0 : line.begin(share);
+    const int stop = tiles ? 1 : min(line.begin(share + 1), all);
+
+    for (int segment = 0; g < stop; segment++) {
+    Found found;
+    int tile, head, off0 = 0, off1, length, origin = 0;
+    if (tiles) {
+        const int unit = a.by_heads(blockIdx.x);
+        head = blockIdx.x - unit * a.KV;
+        if (!found_at(a.s, known[wave], lane, unit, [&](int tokens, int keys) { return Stretch(a, tokens, keys).tiles; }, found)) return;
+        const Stretch st(a, found.tokens, found.keys);
+        tile = st.tiles - 1 - (unit - found.before);
+        off1 = length = st.length(tile);
+        g = stop;
+    } else {
+        if (!found_at(a.s, known[wave], lane, g, [&](int tokens, int keys) { const Stretch st(a, tokens, keys); return a.KV * st.before(st.tiles); }, found)) return;
+        const Stretch st(a, found.tokens, found.keys);
+        const int of_head = st.before(st.tiles), x = g - found.before;
+        head = x / of_head;
+        tile = st.tile(x - head * of_head);
+        off0 = x - head * of_head - st.before(tile);
+        length = st.length(tile);
+        origin = g - off0;
+        off1 = min(length, off0 + stop - g);
+        g += off1 - off0;
+    }
+    const int tokens = found.tokens, keys = found.keys, first = found.start;
+    const int rows = tokens * a.G, row = tile * kTileRows + 32 * wave + li, token = a.by_group(row);
+    int end = keys;                                                          // of the keys that the tile's last row sees
+    if (a.is_causal) end = max(keys - tokens + a.by_group(min((tile + 1) * kTileRows, rows) - 1) + 1, 0);
+    auto cut = [&](int off) __attribute__((always_inline)) { return off == 0 ? 0 : off >= length ? end : min(max((off << a.unit_shift) - 96, 0) & ~(kStage - 1), end); };
+    const int k0 = cut(off0), k1 = cut(off1);
+    const bool parted = off0 > 0 || off1 < length;
+    const Split split = parted ? split_of(line, a.shares, share, origin, length) : Split{0, 1};
+    uint64_t seen = 0;
+    if (parted && threadIdx.x == 0) seen = arrive_look(a.words + split.first);
+
     u32x4 qf[NS];
     {
-        const T* qp = static_cast<const T*>(a.q) + (int64_t)(t.first + token) * a.qs[0] + (int64_t)(head * a.G + row - token * a.G) * a.qs[1];
+        const T* qp = static_cast<const T*>(a.q) + (int64_t)(first + token) * a.qs[0] + (int64_t)(head * a.G + row - token * a.G) * a.qs[1];
 #pragma unroll
         for (int s = 0; s < NS; s++) qf[s] = row < rows ? *reinterpret_cast<const u32x4*>(qp + 16 * s + 8 * lh) : u32x4{0, 0, 0, 0};
     }
-    const int limit = row < rows ? min(a.is_causal ? t.keys - t.tokens + token + 1 : t.keys, t.k1) : 0;
-    const int open = -(int)wave_max((float)-(row < rows ? limit : t.k1));            // blocks in front of it need no mask
+    const int limit = row < rows ? min(a.is_causal ? keys - tokens + token + 1 : keys, k1) : 0;
+    const int open = -(int)wave_max((float)-(row < rows ? limit : k1));              // blocks in front of it need no mask
     const int seen_keys = (int)wave_max((float)limit);                               // blocks behind it concern no row of the wave
+    const int mixed = a.is_causal ? keys - tokens + a.by_group(tile * kTileRows) + 1 : k1;       // keys from here on are seen by some rows of the tile only
 
-    const int32_t* table = a.s.table + (int64_t)t.b * a.s.width;
-    const int page = 1 << a.s.page_shift;
-    // piece i of a thread: K: key and piece of its row; V: a d's keys of a block (EIGHT), or half of them
-    constexpr int kKeyPieces = D * SIZE / 16;
-    struct Stage { u32x4 k[kMine], v[kMine]; float ks[kMine], vs[kMine]; bool ok[kMine]; };
-    struct Pages { int k[kMine], v[kMine]; bool v_ok[kMine]; };
+    const int32_t* table = a.s.table + (int64_t)found.b * a.s.width;
+    uniform_words scalar_table = (uniform_words)(uintptr_t)table;
+    // Sixteen tokens' keys are as many bytes in a row as their values are, kPer pieces of sixteen bytes: piece `idx` of a stage lies at the same place of both
+    constexpr int kPer = D * SIZE;
+    const int page_blocks = a.s.page_shift - 4;
+    // In 16 bits a thread's pieces of both do not fit the registers: values are asked for when the next keys lie in LDS
+    constexpr bool kApart = !EIGHT && D > 64;
+    struct Stage { u32x4 k[kMine], v[kApart ? 1 : kMine]; uint32_t ks[kMine], vs[kMine]; };
+    struct Pages { int at[kMine]; uint32_t absent; };       // bit i of `absent`: the table names no page for block i
     auto ask = [&](Pages& p, int key) __attribute__((always_inline)) {
+        p.absent = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int at = min(((key >> 4) + i) >> page_blocks, a.s.width - 1);
+            p.absent |= (uint32_t)scalar_table[at] < (uint32_t)a.pages ? 0u : 1u << i;
+        }
 #pragma unroll
         for (int i = 0; i < kMine; i++) {
-            const int idx = threadIdx.x + 256 * i;
-            bool ok;
-            p.k[i] = page_of(a, table, (key + idx / kKeyPieces) >> 4, ok);
-            p.v[i] = page_of(a, table, (key >> 4) + idx / (D * SIZE), p.v_ok[i]);
+            const int block = ((int)threadIdx.x + 256 * i) / kPer;
+            const int at = min(((key >> 4) + (kPer % 64 ? block : __builtin_amdgcn_readfirstlane(block))) >> page_blocks, a.s.width - 1);
+            const int page = kPer % 64 ? table[at] : scalar_table[at];
+            p.at[i] = ((uint32_t)page < (uint32_t)a.pages ? page : 0) * a.KV + head;
         }
     };
-    auto load = [&](Stage& st, const Pages& p, int key) __attribute__((always_inline)) {
+    auto load = [&](u32x4 (&w)[kMine], uint32_t (&scale)[kMine], const char* from, const uint8_t* scales, const Pages& p, int key) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kMine; i++) {
             const int idx = threadIdx.x + 256 * i;
             if (kPieces % 256 && idx >= kPieces) continue;
-            const int kk = (key + idx / kKeyPieces) & (page - 1);
-            const int64_t kh = (int64_t)p.k[i] * a.KV + head, vh = (int64_t)p.v[i] * a.KV + head;
-            st.k[i] = *reinterpret_cast<const u32x4*>(a.keys + (kh * page + kk) * (D * SIZE) + idx % kKeyPieces * 16);
-            const int vb = ((key >> 4) + idx / (D * SIZE)) & ((page >> 4) - 1);
-            st.v[i] = *reinterpret_cast<const u32x4*>(a.values + ((vh << (a.s.page_shift - 4)) + vb) * (D * 16 * SIZE) + idx % (D * SIZE) * 16);
-            st.ok[i] = p.v_ok[i];
-            if (EIGHT) {
-                st.ks[i] = scale_of(a.key_scales[kh]);
-                st.vs[i] = scale_of(a.value_scales[vh]);
+            const int block = ((key >> 4) + (kPer % 64 ? idx / kPer : __builtin_amdgcn_readfirstlane(idx / kPer))) & ((1 << page_blocks) - 1);
+            w[i] = *reinterpret_cast<const u32x4*>(from + (((int64_t)p.at[i] << page_blocks) + block) * (16 * kPer) + idx % kPer * 16);
+            if (EIGHT) scale[i] = scales[p.at[i]];
+        }
+    };
+    auto values_of = [](Stage& st) __attribute__((always_inline)) -> u32x4 (&)[kMine] {
+        if constexpr (kApart) return st.k;
+        else return st.v;
+    };
+    auto load_k = [&](Stage& st, const Pages& p, int key) __attribute__((always_inline)) { load(st.k, st.ks, a.keys, a.key_scales, p, key); };
+    auto load_v = [&](Stage& st, const Pages& p, int key) __attribute__((always_inline)) { load(values_of(st), st.vs, a.values, a.value_scales, p, key); };
+    auto put_k = [&](Stage& st, char* to) __attribute__((always_inline)) {
+        constexpr int kKeyPieces = D * SIZE / 16;
+#pragma unroll
+        for (int i = 0; i < kMine; i++) {
+            const int idx = threadIdx.x + 256 * i, k = idx / kKeyPieces, kc = idx % kKeyPieces;
+            if (kPieces % 256 && idx >= kPieces) continue;
+            if constexpr (EIGHT) {
+                const float scale = scale_of(st.ks[i]);
+                *reinterpret_cast<u32x4*>(to + tk_off<D>(k, 2 * kc)) = widen<T>(u32x2{st.k[i].x, st.k[i].y}, scale);
+                *reinterpret_cast<u32x4*>(to + tk_off<D>(k, 2 * kc + 1)) = widen<T>(u32x2{st.k[i].z, st.k[i].w}, scale);
+            } else {
+                *reinterpret_cast<u32x4*>(to + tk_off<D>(k, kc)) = st.k[i];
             }
         }
     };
-    auto put = [&](Stage& st, int key, char* to) __attribute__((always_inline)) {
+    auto put_v = [&](Stage& st, uint32_t absent, int key, char* to, bool tame) __attribute__((always_inline)) {
+        const bool leave = tame && key + kStage > mixed;
 #pragma unroll
         for (int i = 0; i < kMine; i++) {
             const int idx = threadIdx.x + 256 * i;
             if (kPieces % 256 && idx >= kPieces) continue;
-            const int k = idx / kKeyPieces, kc = idx % kKeyPieces;
-            const int block = idx / (D * SIZE), d = idx % (D * SIZE) / SIZE, half = EIGHT ? 0 : idx & 1;
+            u32x4 w = values_of(st)[i];
+            const int block = idx / kPer, d = idx % kPer / SIZE, half = EIGHT ? 0 : idx & 1;
             // values that no key of this part stands for may hold anything, a NaN among it
-            const int n = st.ok[i] ? t.k1 - key - 16 * block - 8 * half : 0;
+            const int n = absent >> block & 1 ? 0 : k1 - key - 16 * block - 8 * half;
             if (n < 16 / SIZE) {
-                constexpr int kPer = 4 / SIZE;
+                constexpr int kOf = 4 / SIZE;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int left = min(max(n - kPer * e, 0), kPer) * SIZE;
-                    st.v[i][e] &= left == 4 ? ~0u : (1u << (8 * left)) - 1;
+                    const int left = min(max(n - kOf * e, 0), kOf) * SIZE;
+                    w[e] &= left == 4 ? ~0u : (1u << (8 * left)) - 1;
                 }
             }
-            char* tk = to;
+            if (leave) {
+                bool wild = false;
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = tamed<T, EIGHT>(w[e], wild);
+            }
             char* tv = to + kKBytes;
             if constexpr (EIGHT) {
-                *reinterpret_cast<u32x4*>(tk + tk_off<D>(k, 2 * kc)) = widen<T>(u32x2{st.k[i].x, st.k[i].y}, st.ks[i]);
-                *reinterpret_cast<u32x4*>(tk + tk_off<D>(k, 2 * kc + 1)) = widen<T>(u32x2{st.k[i].z, st.k[i].w}, st.ks[i]);
-                *reinterpret_cast<u32x4*>(tv + tv_off(d, 2 * block)) = widen<T>(u32x2{st.v[i].x, st.v[i].y}, st.vs[i]);
-                *reinterpret_cast<u32x4*>(tv + tv_off(d, 2 * block + 1)) = widen<T>(u32x2{st.v[i].z, st.v[i].w}, st.vs[i]);
+                const float scale = scale_of(st.vs[i]);
+                *reinterpret_cast<u32x4*>(tv + tv_off(d, 2 * block)) = widen<T>(u32x2{w.x, w.y}, scale);
+                *reinterpret_cast<u32x4*>(tv + tv_off(d, 2 * block + 1)) = widen<T>(u32x2{w.z, w.w}, scale);
             } else {
-                *reinterpret_cast<u32x4*>(tk + tk_off<D>(k, kc)) = st.k[i];
-                *reinterpret_cast<u32x4*>(tv + tv_off(d, 2 * block + half)) = st.v[i];
+                *reinterpret_cast<u32x4*>(tv + tv_off(d, 2 * block + half)) = w;
             }
         }
     };
@@ -676,8 +837,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
     // row li of a tile of S^T is key `of` of its 32
     const int of = 16 * (li >> 4) + 8 * ((li >> 2) & 1) + 4 * ((li >> 3) & 1) + (li & 3);
 
-    auto attend = [&](const char* from, int key, uint32_t absent) __attribute__((always_inline)) {
-        f32x16 sv[2];
+    auto scores = [&](f32x16 (&sv)[2], const char* from, int key, uint32_t absent) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             sv[j] = f32x16{};
@@ -722,6 +882,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
 #pragma unroll
             for (int f = 0; f < NF; f++) oacc[f] *= alpha;
         }
+    };
+    auto product = [&](const f32x16 (&sv)[2], const char* from) __attribute__((always_inline)) {
 #pragma unroll
         for (int ks = 0; ks < 4; ks++) {
             u32x4 pb;
@@ -733,44 +895,83 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
         }
     };
 
-    if (t.k0 < t.k1) {
+    auto go = [&](bool tame) __attribute__((always_inline)) {
         Pages pg;
         Stage st;
-        ask(pg, t.k0);
-        load(st, pg, t.k0);
-        ask(pg, t.k0 + kStage);
-        put(st, t.k0, lds[0]);
+        ask(pg, k0);
+        uint32_t absent = pg.absent;
+        load_k(st, pg, k0);
+        if constexpr (kApart) put_k(st, lds[0]);
+        load_v(st, pg, k0);
+        if constexpr (!kApart) put_k(st, lds[0]);
+        put_v(st, absent, k0, lds[0], tame);
+        ask(pg, k0 + kStage);
         __syncthreads();
         int at = 0;
-        for (int key = t.k0; key < t.k1; key += kStage) {
-            const bool more = key + kStage < t.k1;
+        for (int key = k0; key < k1; key += kStage) {
+            const bool more = key + kStage < k1;
+            const uint32_t then = pg.absent;
             if (more) {
-                load(st, pg, key + kStage);
+                load_k(st, pg, key + kStage);
+                if constexpr (!kApart) {
+                    load_v(st, pg, key + kStage);
+                    ask(pg, key + 2 * kStage);
+                }
+            }
+            f32x16 sv[2];
+            if (key < seen_keys) scores(sv, lds[at], key, absent);
+            if (kApart && more) {
+                put_k(st, lds[at ^ 1]);
+                load_v(st, pg, key + kStage);
                 ask(pg, key + 2 * kStage);
             }
-            if (key < seen_keys) {
-                // blocks of sixteen keys whose page the table does not name
-                uint32_t absent = 0;
-#pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    bool ok;
-                    page_of(a, table, (key >> 4) + n, ok);
-                    absent |= (ok ? 0u : 1u) << n;
-                }
-                attend(lds[at], key, absent);
+            if (key < seen_keys) product(sv, lds[at]);
+            if (more) {
+                if constexpr (!kApart) put_k(st, lds[at ^ 1]);
+                put_v(st, then, key + kStage, lds[at ^ 1], tame);
             }
-            if (more) put(st, key + kStage, lds[at ^ 1]);
             __syncthreads();
+            absent = then;
             at ^= 1;
+        }
+    };
+    if (segment) __syncthreads();                                            // (the segment before has been read)
+    bool tame = false;
+    while (k0 < k1) {
+        go(tame);
+        if (mixed >= k1 || tame) break;
+        bool odd = false;
+#pragma unroll
+        for (int f = 0; f < NF; f++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) odd |= !(fabsf(oacc[f][r]) < INFINITY);
+        if (!__syncthreads_or(odd)) break;
+        tame = true;                                                         // (see `tamed`)
+#pragma unroll
+        for (int f = 0; f < NF; f++) oacc[f] = f32x16{};
+        m_run = -INFINITY;
+        l_run = 0.f;
+    }
+    if (tame) {
+#pragma unroll 1
+        for (int kk = max(k0, mixed) & ~(kStage - 1); kk < k1; kk++) {
+            const char* vp = kk < k0 ? nullptr : value_at<D, SIZE>(a, table, head, kk);
+            if (!vp) continue;
+#pragma unroll
+            for (int f = 0; f < NF; f++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const float x = wild_of<T, EIGHT>(vp + (32 * f + 8 * (r >> 2) + 4 * lh + (r & 3)) * (16 * SIZE));
+                    oacc[f][r] += kk < limit ? x : 0.f;
+                }
         }
     }
 
     l_run = half_sum(l_run);
-    const int64_t slots = gridDim.x;
-    if (t.parts == 1) {
+    if (!parted) {
         if (row < rows) {
             const float inv = l_run != 0.f ? 1.f / l_run : 0.f;
-            T* out = static_cast<T*>(a.o) + (int64_t)(t.first + token) * a.os[0] + (int64_t)(head * a.G + row - token * a.G) * a.os[1] + 4 * lh;
+            T* out = static_cast<T*>(a.o) + (int64_t)(first + token) * a.os[0] + (int64_t)(head * a.G + row - token * a.G) * a.os[1] + 4 * lh;
 #pragma unroll
             for (int f = 0; f < NF; f++)
 #pragma unroll
@@ -778,10 +979,10 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
                     *reinterpret_cast<u32x2*>(out + 32 * f + 8 * g) =
                         u32x2{Mfma32A<T>::pack2(oacc[f][4 * g] * inv, oacc[f][4 * g + 1] * inv), Mfma32A<T>::pack2(oacc[f][4 * g + 2] * inv, oacc[f][4 * g + 3] * inv)};
         }
-        return;
+        continue;
     }
-    if (threadIdx.x == 0) arrive_claim(a.words + slot0, seen, a.tag);
-    const Parts<kTileRows, D> own(a, slot0 + t.part * a.KV, slots);
+    if (threadIdx.x == 0) arrive_claim(a.words + split.first, seen, a.tag);
+    const Parts<kTileRows, D> own(a, 2 * share + (off0 ? 0 : 1));
     if (row < rows) {
         const __amdgpu_buffer_rsrc_t rs = parts_rsrc(own.sums);
         const int r = 32 * wave + li;
@@ -792,36 +993,36 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
                 store_part(rs, (uint32_t)((r * D + 32 * f + 8 * g + 4 * lh) * 4), f32x4{oacc[f][4 * g], oacc[f][4 * g + 1], oacc[f][4 * g + 2], oacc[f][4 * g + 3]});
         if (lh == 0) store_two(own.state + 2 * r, m_run, l_run);
     }
-    if (!arrive_last(a.words + slot0, t.parts, &last)) return;
-    join<T, kTileRows, D, 256>(a, t, head, slot0, a.KV, 0, slots);
+    if (arrive_last(a.words + split.first, split.parts, &last)) join<T, kTileRows, D, 256>(a, split, first, head, tile * kTileRows, min(kTileRows, rows - tile * kTileRows));
+    }
 }
 
-// The launch that serves these sizes: rows of a workgroup's tile, workgroups that share the work (few rows) or that parts are meant to fill, the grid, and the places for parts and counts.
-struct Plan { int rows, target; int64_t grid, slots, words; int step_shift; };
+// The launch that serves these sizes: rows of a workgroup's tile, the workgroups that share the work, and log2 of the keys that a unit of their line stands for.
+struct Plan { int rows, shares, unit_shift; bool single; int64_t tiles; };
 
 Plan plan_of(const mhip_paged_cache* c, const mhip_sequences* s, int64_t q_heads) {
     const int64_t G = q_heads / c->heads, average = (s->tokens + s->sequences - 1) / s->sequences * G;
     const int rows = average <= 16 ? 16 : average <= 32 ? 32 : kTileRows;
-    if (rows != kTileRows) {
-        const int target = rows_kernel_workgroups(rows / 16, c->head_size) * compute_units();
-        // (more keys a step where the line could have more than 2^29 steps)
-        const double tiles = (double)(s->tokens * G / rows + s->sequences) * c->heads;
-        int shift = kStepShift;
-        while (tiles * (double)((s->width * c->page_size >> shift) + 1) > (double)(1 << 29)) shift++;
-        return {rows, target, target, 2 * target, target, shift};
-    }
-    const int target = 2 * compute_units();
-    const int64_t units = s->tokens * G / rows + (s->sequences < s->tokens ? s->sequences : s->tokens) + target / c->heads + 1;
-    return {rows, target, units * c->heads, units * c->heads, units * c->heads, 0};
+    const double tiles = (double)(s->tokens * G / rows + (s->sequences < s->tokens ? s->sequences : s->tokens)) * c->heads;      // that there can be
+    const int64_t keys = s->width * c->page_size;
+    auto most = [&](int shift) { return rows == kTileRows ? tiles * (double)((2 * (keys + 2 * kTileCost) >> shift) + 1) : tiles * (double)((keys >> shift) + 1); };
+    const bool single = s->tokens <= s->sequences && G <= rows && rows != kTileRows;
+    int shift = rows == kTileRows ? 0 : kStepShift;
+    while (most(shift) > (double)(1 << 29)) shift++;
+    int shares = (rows == kTileRows ? 2 : rows_kernel_workgroups(rows / 16, c->head_size, single)) * compute_units();
+    if (rows != kTileRows && most(shift) < shares) shares = (int)most(shift);                                                     // (a step is the least share)
+    return {rows, shares, shift, single, (int64_t)tiles};
 }
 
-int64_t workspace_of(const mhip_paged_cache* c, const Plan& p) { return p.slots * p.rows * (c->head_size + 2) * 4 + p.words * 8; }
+int64_t workspace_of(const mhip_paged_cache* c, const Plan& p) { return (int64_t)p.shares * (2 * p.rows * (c->head_size + 2) * 4 + 8); }
 
 template <typename T, int D, bool EIGHT>
 int launch(hipStream_t st, const PagedArgs& a, const Plan& p) {
-    const dim3 grid((unsigned)p.grid);
-    if (p.rows == 16) hipLaunchKernelGGL((paged_rows_kernel<T, D, EIGHT, 1, 4>), grid, dim3(256), 0, st, a);
-    else if (p.rows == 32) hipLaunchKernelGGL((paged_rows_kernel<T, D, EIGHT, 2, 4>), grid, dim3(256), 0, st, a);
+    const dim3 grid((unsigned)(p.rows == kTileRows && (!a.part || p.tiles >= p.shares) ? std::max<int64_t>(p.tiles, p.shares) : p.shares));
+    if (p.rows == 16 && p.single) hipLaunchKernelGGL((paged_rows_kernel<T, D, EIGHT, 1, 4, true>), grid, dim3(256), 0, st, a);
+    else if (p.rows == 16) hipLaunchKernelGGL((paged_rows_kernel<T, D, EIGHT, 1, 4, false>), grid, dim3(256), 0, st, a);
+    else if (p.rows == 32 && p.single) hipLaunchKernelGGL((paged_rows_kernel<T, D, EIGHT, 2, 4, true>), grid, dim3(256), 0, st, a);
+    else if (p.rows == 32) hipLaunchKernelGGL((paged_rows_kernel<T, D, EIGHT, 2, 4, false>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((paged_tile_kernel<T, D, EIGHT>), grid, dim3(256), 0, st, a);
     return check_launch("paged_attention");
 }
@@ -858,15 +1059,15 @@ extern "C" int mhip_paged_attention(void* stream, const mhip_paged_cache* cache,
         if (strides[i] % 8) return fail(MHIP_ERR_UNSUPPORTED, "paged_attention: strides must be multiples of 8 elements");
     if (seqs->tokens * (q_heads / cache->heads) >= 1 << 30) return fail(MHIP_ERR_UNSUPPORTED, "paged_attention: more than 2^30 rows");
     const Plan p = plan_of(cache, seqs, q_heads);
-    if (p.grid >= 1 << 30) return fail(MHIP_ERR_UNSUPPORTED, "paged_attention: more workgroups than a launch has");
     PagedArgs a{q, o, (const char*)cache->keys, (const char*)cache->values, cache->key_scales, cache->value_scales, sequences(cache, seqs),
-                (int)cache->pages, (int)cache->heads, (int)(q_heads / cache->heads), is_causal ? 1 : 0, p.target, scale * kLog2e, {strides[0], strides[1]}, {strides[2], strides[3]},
-                nullptr, nullptr, 0, Divider((uint32_t)(q_heads / cache->heads)), Divider((uint32_t)cache->heads), Divider((uint32_t)p.target), p.step_shift};
+                (int)cache->pages, (int)cache->heads, (int)(q_heads / cache->heads), is_causal ? 1 : 0, p.shares, scale * kLog2e, {strides[0], strides[1]}, {strides[2], strides[3]},
+                nullptr, nullptr, 0, Divider((uint32_t)(q_heads / cache->heads)), Divider((uint32_t)cache->heads), Divider((uint32_t)p.shares), p.unit_shift};
     if (workspace && workspace_bytes >= workspace_of(cache, p)) {
         a.part = static_cast<float*>(workspace);
-        a.words = reinterpret_cast<uint64_t*>(a.part + p.slots * p.rows * (cache->head_size + 2));
+        a.words = reinterpret_cast<uint64_t*>(a.part + 2 * (int64_t)p.shares * p.rows * (cache->head_size + 2));
         a.tag = launch_tag();
     }
+    if (p.tiles >= 1 << 30) return fail(MHIP_ERR_UNSUPPORTED, "paged_attention: more tiles than a launch has workgroups");
     hipStream_t st = as_stream(stream);
     const bool eight = cache->key_scales != nullptr;
     const int64_t D = cache->head_size;

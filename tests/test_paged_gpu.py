@@ -413,3 +413,33 @@ def test_refusals():
     assert kernels.paged_attention(q[:0], c, table, lengths, starts).shape == (0, 4, 64)
     empty = ints(np.zeros((0, 2)))
     assert kernels.paged_append(c, k[:0], k[:0], empty, lengths[:0], starts[:1]) is None
+
+
+@EIGHT
+@HALF
+@pytest.mark.parametrize("new,H", [(3, 4), (20, 4), (90, 2)])
+def test_what_is_not_finite_stays_with_those_that_see_it(new, H, dtype, eight):
+    """A NaN (and, in 16 bits, an infinity) among the values of new tokens: the tokens in front of them have finite results."""
+    lengths, wild = [new + 70, new], {}
+
+    def change(table, cache):
+        for b, n in enumerate(lengths):
+            for at, value, d in ((n - new // 2, float("nan"), 3), (n - 1, float("nan") if eight else float("inf"), 40), (n - 2, float("-inf") if not eight else float("nan"), 17)):
+                cache.x[1][table[b, at // 16], :, at % 16, d] = value
+                wild.setdefault(b, []).append((at, value, d))
+    from metalhlo_amd import kernels
+    rng = np.random.default_rng(new)
+    table, pages = table_of(lengths, 16, rng)
+    cache = HostCache(pages, 2, 16, 64, dtype, eight).fill(table, lengths, rng)
+    starts = _starts([new, new])
+    q = _normal(rng, (2 * new, H, 64), dtype)
+    want, bound = attention(q, cache, table, lengths, starts)
+    change(table, cache)
+    got = kernels.paged_attention(q.cuda(), cache.to_device(), ints(table), ints(lengths), ints(starts)).double().cpu().numpy()
+    for b, n in enumerate(lengths):
+        for at, value, d in wild[b]:
+            want[starts[b] + at - (n - new):starts[b + 1], :, d] += value
+    assert (np.isnan(got) == np.isnan(want)).all() and (got[np.isinf(want)] == want[np.isinf(want)]).all()
+    fine = np.isfinite(want)
+    # (without the wild value the rows that see it are off in that element alone)
+    assert (np.abs(got[fine] - want[fine]) <= bound[fine]).all()
