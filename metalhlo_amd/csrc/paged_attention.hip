@@ -702,9 +702,28 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
     if (tiles) {
         const int unit = a.by_heads(blockIdx.x);
         head = blockIdx.x - unit * a.KV;
-        if (!found_at(a.s, known[wave], lane, unit, [&](int tokens, int keys) { return Stretch(a, tokens, keys).tiles; }, found)) return;
+        int level;
+        if (a.s.B <= 64) {
+            // the last tiles of all sequences, then those in front of them, ...: `level` of them lie in front of this one's
+            const int own = (known[wave].tokens[lane] * a.G + kTileRows - 1) / kTileRows;
+            auto before = [&](int n) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(wave_scan(min(own, n)), 63); };
+            int low = 0;
+            for (int step = 1 << (31 - __builtin_clz(a.s.T * a.G / kTileRows + 1)); step; step >>= 1)
+                if (before(low + step) <= unit) low += step;
+            level = low;
+            const int has = own > level ? 1 : 0, place = wave_scan(has) - has, wanted = unit - before(level);
+            const uint64_t m = __ballot(has && place == wanted);
+            if (!m) return;
+            found.b = __builtin_ctzll(m);
+            found.start = __builtin_amdgcn_readfirstlane(known[wave].start[found.b]);
+            found.tokens = __builtin_amdgcn_readfirstlane(known[wave].tokens[found.b]);
+            found.keys = __builtin_amdgcn_readfirstlane(known[wave].keys[found.b]);
+        } else {
+            if (!found_at(a.s, known[wave], lane, unit, [&](int tokens, int keys) { return Stretch(a, tokens, keys).tiles; }, found)) return;
+            level = unit - found.before;
+        }
         const Stretch st(a, found.tokens, found.keys);
-        tile = st.tiles - 1 - (unit - found.before);
+        tile = st.tiles - 1 - level;
         off1 = length = st.length(tile);
         g = stop;
     } else {

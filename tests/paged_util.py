@@ -126,3 +126,28 @@ def assert_within(got, want, bound, what=""):
     if bad.any():
         i = np.unravel_index(np.argmax(np.where(bad, off / bound, 0)), g.shape)
         raise AssertionError(f"{what}: {bad.sum()} of {rows.sum()} too far off; worst at {i}: got {g[i]!r}, expected {want[i]!r}, bound {bound[i]:.3g}")
+
+
+def attention_at_once(q, cache, table, lengths, starts, scale=None, is_causal=True):
+    """What `attention` returns, a sequence's rows of a head at a time (every key on a page)."""
+    u = half_step(q.dtype)
+    qd = q.double().cpu().numpy()
+    T, H, D = qd.shape
+    KV = cache.x[0].shape[1]
+    scale = D ** -0.5 if scale is None else scale
+    out, bound = np.full((T, H, D), np.nan), np.zeros((T, H, D))
+    for b, n in enumerate(lengths):
+        k, v = (cache.dense(w, table, b, n) for w in range(2))
+        m = starts[b + 1] - starts[b]
+        rows = slice(starts[b], starts[b + 1])
+        hidden = np.arange(n)[None] > (np.arange(n - m, n) if is_causal else np.full(m, n))[:, None]
+        for h in range(H):
+            s = np.where(hidden, -np.inf, scale * (qd[rows, h] @ k[h // (H // KV)].T))
+            p = np.exp(s - s.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            vv = v[h // (H // KV)]
+            out[rows, h] = p @ vv
+            bound[rows, h] = 1.01 * (u * np.abs(out[rows, h]) + (u + 2.0 ** -13) * (p @ np.abs(vv))) + 1e-30
+            if q.dtype == torch.float16:
+                bound[rows, h] += 2.0 ** -25 * (2 + n * np.abs(vv).max())
+    return out, bound

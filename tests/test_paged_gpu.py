@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.paged_util import E4M3, HostCache, assert_within, attention, half_step, scale_byte, table_of
+from tests.paged_util import E4M3, HostCache, assert_within, attention, attention_at_once, half_step, scale_byte, table_of
 from tests.util import NAME
 
 pytestmark = pytest.mark.gpu
@@ -443,3 +443,21 @@ def test_what_is_not_finite_stays_with_those_that_see_it(new, H, dtype, eight):
     fine = np.isfinite(want)
     # (without the wild value the rows that see it are off in that element alone)
     assert (np.abs(got[fine] - want[fine]) <= bound[fine]).all()
+
+
+@EIGHT
+@pytest.mark.parametrize("lengths,context,H,KV,D,page", [([700, 1, 300, 900, 513], 0, 32, 32, 32, 16),            # more tiles than shares, short ones among them: whole tiles
+                                                         ([300] * 40 + [5] * 60, 0, 8, 8, 32, 64),                  # the same with more than 64 sequences
+                                                         ([130, 200, 90], 1500, 32, 8, 64, 32),                     # tiles split over shares
+                                                         ([300] * 6, 900, 32, 32, 32, 256)], ids=str)               # more tiles than shares, all long
+def test_many_tiles(lengths, context, H, KV, D, page, eight):
+    from metalhlo_amd import kernels
+    rng = np.random.default_rng(len(lengths))
+    keys = [n + context for n in lengths]
+    table, pages = table_of(keys, page, rng)
+    cache = HostCache(pages, KV, page, D, torch.bfloat16, eight).fill(table, keys, rng)
+    starts = _starts(lengths)
+    q = _normal(rng, (starts[-1], H, D), torch.bfloat16)
+    got = kernels.paged_attention(q.cuda(), cache.to_device(), ints(table), ints(keys), ints(starts))
+    want, bound = attention_at_once(q, cache, table, keys, starts)
+    assert_within(got, want, bound, "many tiles")
