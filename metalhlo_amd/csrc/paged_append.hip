@@ -6,8 +6,11 @@
 //   8 bits    the page's scale is the least power of two under which its largest value is at most 448.  Where the page holds tokens already it never shrinks, and
 //             where it grows by 2^n the held values are multiplied by 2^-n and rounded, which changes none that stays above 2^-6 of the new scale.
 //
-// Bound by memory: every new value is read once and written once.  A workgroup takes one page's new tokens of one head, of keys or values (a page's scale needs all of
-// them), or of one query head, whose rotation is the keys' own; a wave takes blocks of sixteen tokens and keeps them in registers in fp32 until the page's largest value is known.
+// Bound by memory: every new value is read once and written once.  Two kernels:
+//
+//   paged_append_kernel   A wave a block of sixteen tokens, a workgroup a page (a scale needs all of its tokens), with a few heads of keys, values or queries one behind the other: the cosines and sines stay in
+//                         registers from head to head, and the next head is on its way while this one's scale is found and its values are stored.  Values pass through LDS, which turns a block's rows into its columns.
+//   append_few_kernel     No more tokens than sequences (a decode step): a row of a token is a few lanes' work, and a workgroup takes many heads of one page.
 #include "paged.h"
 
 namespace mhip {
@@ -20,7 +23,7 @@ struct AppendArgs {
     char *keys, *values;
     uint8_t *key_scales, *value_scales;
     Sequences s;
-    int pages, KV, H, R, positions;
+    int pages, KV, H, R, positions, heads_a_part;
     int64_t ks[2], vs[2], qs[2], os[2];       // token and head strides in elements
 };
 
@@ -63,191 +66,242 @@ __device__ __forceinline__ int scale_byte(float amax) {
     return max((int)(bits >> 23) - 8 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0), 1);
 }
 
-template <typename T, int D, bool EIGHT, int WAVES, int BLOCKS>
+// Rows of keys and queries are whole lines and are stored past the caches (us, plain | so: 9450 tokens of 32 and 8 heads of 128 into pages of 64 49.3 | 39.2, of 16 48.6 | 37.2, of 256 52.2 | 46.5;
+// loads so: 47.6, and 23.7 | 32.3 where two heads share a line).
+template <typename V, typename T>
+__device__ __forceinline__ void put_stream(T* p, V v) { __builtin_nontemporal_store(v, reinterpret_cast<V*>(p)); }
+
+// The page that unit u of a launch fills: `slot0` .. `slot1` of page `page_no` (which may be none of the cache's) take the tokens from row `row` on, whose positions begin at `pos`.
+struct Fill {
+    int page_no, slot0, slot1, pos;
+    int64_t row;
+    __device__ __forceinline__ bool find(const AppendArgs& a, int u) {
+        const int shift = a.s.page_shift, page = 1 << shift;
+        int first;
+        auto touched = [&](int b) __attribute__((always_inline)) {
+            const int n = a.s.tokens(b), end = a.s.keys(b), begin = max(end - n, 0);
+            return n ? ((end + page - 1) >> shift) - (begin >> shift) : 0;
+        };
+        const int b = sequence_of(a.s.B, u, touched, first);
+        if (b < 0) return false;
+        const int n = a.s.tokens(b), end = a.s.keys(b), begin = max(end - n, 0);      // (more tokens than keys: the first ones have no place)
+        const int at = (begin >> shift) + u - first;
+        if (at < begin >> shift || at << shift >= end) return false;                  // (starts that are no starts: their sums may have wrapped)
+        pos = max(begin, at << shift);
+        const int stop = min(min(end, (at + 1) << shift), a.R ? a.positions : end);
+        if (pos >= stop) return false;
+        page_no = a.s.table[(int64_t)b * a.s.width + at];
+        slot0 = pos & (page - 1);
+        slot1 = slot0 + stop - pos;
+        row = a.s.start(b) + (n - (end - pos));
+        return true;
+    }
+};
+
+// the scale's byte for a page whose new tokens reach `top`, and whether the old ones have to follow it
+struct Scale {
+    float inv, factor;
+    int byte;
+    bool moves;
+    __device__ __forceinline__ Scale(float top, int was, bool begun) {
+        was = begun ? max(was, 1) : 0;
+        byte = max(scale_byte(top), was);
+        inv = scale_of(254 - byte);
+        moves = begun && byte > was;
+        factor = scale_of(127 + was - byte > 0 ? 127 + was - byte : 1);
+    }
+};
+// the values that a page holds under a grown scale, by `lanes` lanes of which this one is `lane`
+__device__ __forceinline__ void move_keys(char* page, int slot0, int D, float factor, int lane, int lanes) {
+    u32x4* held = reinterpret_cast<u32x4*>(page);
+    for (int i = lane; i < slot0 * D / 16; i += lanes) {
+        u32x4 w = held[i];
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = moved8(w[e], factor);
+        held[i] = w;
+    }
+}
+__device__ __forceinline__ void move_values(char* page, int slot0, int D, float factor, int lane, int lanes) {
+    const int whole = slot0 / kBlock * D, rest = slot0 % kBlock;                       // sixteen bytes of a d each
+    move_keys(page, slot0 / kBlock * kBlock, D, factor, lane, lanes);
+    for (int i = lane; i < D * rest; i += lanes) {                                   // (byte by byte: the bytes behind them are being written)
+        char* p = page + (whole + i / rest) * 16 + i % rest;
+        *p = (char)(moved8((uint8_t)*p, factor) & 255);
+    }
+}
+
+// x, y: eight elements each of the two halves of a rotated pair of pieces
+__device__ __forceinline__ void turn(float* x, float* y, const f32x4 (&co)[2], const f32x4 (&si)[2]) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float u = x[e], w = y[e], c = co[e >> 2][e & 3], s = si[e >> 2][e & 3];
+        x[e] = u * c - w * s;
+        y[e] = u * s + w * c;
+    }
+}
+
+template <typename T, int D, bool EIGHT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) {
     constexpr int kLanes = D / 16;                                        // lanes of a row: each has two pieces of eight elements
-    constexpr int kRows = kLanes <= 2 ? 16 : kLanes == 4 ? 16 : 8;        // rows that a wave reads at once
+    constexpr int kRows = kLanes <= 4 ? 16 : 8;                           // rows that a wave reads at once
     constexpr int kTurns = kBlock / kRows;
-    __shared__ float tops[WAVES];
+    constexpr int kPairs = D / 2, kGroups = kPairs <= 16 ? 4 : kPairs <= 32 ? 2 : 1, kMine = kBlock / kGroups;
+    constexpr int kPieces = D / 8, kRead = kPieces <= 4 ? 16 : kPieces <= 8 ? 8 : 4, kReads = kBlock / kRead;     // of a row of values; rows a read, reads a block
+    __shared__ float tops[2][WAVES];
+    __shared__ __attribute__((aligned(16))) T turned_values[WAVES][kBlock][D];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int shift = a.s.page_shift, page = 1 << shift;
+    Fill f;
+    if (!f.find(a, blockIdx.x)) return;
+    const int page = 1 << a.s.page_shift, s0 = f.slot0, s1 = f.slot1;
+    const bool on_page = (uint32_t)f.page_no < (uint32_t)a.pages;
 
-    // ---- the page that this workgroup fills
-    int first;
-    auto touched = [&](int b) __attribute__((always_inline)) {
-        const int n = a.s.tokens(b), end = a.s.keys(b), begin = max(end - n, 0);
-        return n ? ((end + page - 1) >> shift) - (begin >> shift) : 0;
+    // heads [head0, head1) of keys, values or queries
+    const int kv_parts = (a.KV + a.heads_a_part - 1) / a.heads_a_part, part = blockIdx.y;
+    const bool is_v = part >= kv_parts && part < 2 * kv_parts, is_q = part >= 2 * kv_parts;
+    const int head0 = (part - (is_q ? 2 * kv_parts : is_v ? kv_parts : 0)) * a.heads_a_part, head1 = min(head0 + a.heads_a_part, is_q ? a.H : a.KV);
+    if (!is_q && !on_page) return;
+    const int64_t page_head0 = (int64_t)f.page_no * a.KV;
+    const uint8_t* scales = is_v ? a.value_scales : a.key_scales;
+    uint8_t* scales_out = is_v ? a.value_scales : a.key_scales;
+    // the largest value of the page's new tokens: one barrier a head, on places that alternate
+    auto of_page = [&](float top, int head) __attribute__((always_inline)) {
+        top = wave_max(top);
+        if (WAVES > 1) {
+            if (lane == 0) tops[head & 1][wave] = top;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) top = fmaxf(top, tops[head & 1][w]);
+        }
+        return top;
     };
-    const int b = sequence_of(a.s.B, (int)blockIdx.x, touched, first);
-    if (b < 0) return;
-    const int n = a.s.tokens(b), end = a.s.keys(b), begin = max(end - n, 0);          // (more tokens than keys: the first ones have no place)
-    const int at = (begin >> shift) + (int)blockIdx.x - first;
-    if (at < begin >> shift || at << shift >= end) return;                            // (starts that are no starts: their sums may have wrapped)
-    const int p0 = max(begin, at << shift), p1 = min(min(end, (at + 1) << shift), a.R ? a.positions : end);
-    const int page_no = a.s.table[(int64_t)b * a.s.width + at];
-    if (p0 >= p1) return;
-    const int s0 = p0 & (page - 1), s1 = s0 + p1 - p0;
-    const int64_t row0 = a.s.start(b) + (n - (end - p0));                               // of slot s0
-
-    const int part = blockIdx.y;                                                       // keys, values, queries
-    const bool is_v = part >= a.KV && part < 2 * a.KV, is_q = part >= 2 * a.KV;
-    const int head = is_q ? part - 2 * a.KV : is_v ? part - a.KV : part;
-    if (!is_q && (uint32_t)page_no >= (uint32_t)a.pages) return;
-    const int64_t page_head = (int64_t)page_no * a.KV + head;
 
     if (!is_v) {
-        const T* x = is_q ? static_cast<const T*>(a.q) + head * a.qs[1] : static_cast<const T*>(a.k) + head * a.ks[1];
-        const int64_t xs = is_q ? a.qs[0] : a.ks[0];
+        const T* x = is_q ? static_cast<const T*>(a.q) : static_cast<const T*>(a.k);
+        const int64_t xs = is_q ? a.qs[0] : a.ks[0], xh = is_q ? a.qs[1] : a.ks[1];
         // lane l of a row: pieces l and l + R / 16 of the rotated elements, which belong together, or two of those behind them
         const int l = lane % kLanes, r = lane / kLanes;
         const bool turned = l < a.R / 16;
         const int d1 = turned ? 8 * l : a.R + 16 * (l - a.R / 16), d2 = turned ? d1 + a.R / 2 : d1 + 8;
-        float y[BLOCKS][kTurns][16];
-        float top = 0.f;
+        bool in[kTurns];
+        f32x4 co[kTurns][2], si[kTurns][2];
+        const T* rows[kTurns];
 #pragma unroll
-        for (int c = 0; c < BLOCKS; c++) {
-            const int block = c * WAVES + wave;
-#pragma unroll
-            for (int t = 0; t < kTurns; t++) {
-                const int slot = block * kBlock + t * kRows + r;
-                const bool in = slot >= s0 && slot < s1 && r < kRows;
-                if (!in) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) y[c][t][e] = 0.f;
-                    continue;
-                }
-                const T* row = x + (row0 + slot - s0) * xs;
-                float f[16];
-                to_floats<T>(*reinterpret_cast<const u32x4*>(row + d1), f);
-                to_floats<T>(*reinterpret_cast<const u32x4*>(row + d2), f + 8);
-                if (turned) {
-                    const f32x4* cs = reinterpret_cast<const f32x4*>(a.freqs + (int64_t)(p0 + slot - s0) * a.R + 8 * l);
-                    const f32x4* sn = reinterpret_cast<const f32x4*>(a.freqs + (int64_t)(p0 + slot - s0) * a.R + 8 * l + a.R / 2);
-                    const f32x4 co[2] = {cs[0], cs[1]}, si[2] = {sn[0], sn[1]};
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float u = f[e], w = f[e + 8], cc = co[e >> 2][e & 3], ss = si[e >> 2][e & 3];
-                        f[e] = u * cc - w * ss;
-                        f[e + 8] = u * ss + w * cc;
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    y[c][t][e] = f[e];
-                    if (EIGHT) top = finite_max(top, f[e]);
-                }
+        for (int t = 0; t < kTurns; t++) {
+            const int slot = wave * kBlock + t * kRows + r;
+            in[t] = slot >= s0 && slot < s1 && r < kRows;
+            rows[t] = x + (f.row + slot - s0) * xs;
+            if (in[t] && turned) {
+                const f32x4* cs = reinterpret_cast<const f32x4*>(a.freqs + (int64_t)(f.pos + slot - s0) * a.R + 8 * l);
+                const f32x4* sn = reinterpret_cast<const f32x4*>(a.freqs + (int64_t)(f.pos + slot - s0) * a.R + 8 * l + a.R / 2);
+                co[t][0] = cs[0]; co[t][1] = cs[1];
+                si[t][0] = sn[0]; si[t][1] = sn[1];
             }
         }
-        float inv = 1.f, factor = 1.f;
-        if (EIGHT && !is_q) {
-            const int was = s0 ? max((int)a.key_scales[page_head], 1) : 0;
-            top = wave_max(top);
-            if (WAVES > 1) {
-                if (lane == 0) tops[wave] = top;
-                __syncthreads();
-#pragma unroll
-                for (int w = 0; w < WAVES; w++) top = fmaxf(top, tops[w]);
-            }
-            const int byte = max(scale_byte(top), was);
-            inv = scale_of(254 - byte);
-            if (s0 && byte > was) {
-                factor = scale_of(127 + was - byte > 0 ? 127 + was - byte : 1);
-                u32x4* held = reinterpret_cast<u32x4*>(a.keys + page_head * page * D);
-                for (int i = threadIdx.x; i < s0 * D / 16; i += 64 * WAVES) {
-                    u32x4 w = held[i];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) w[e] = moved8(w[e], factor);
-                    held[i] = w;
-                }
-            }
-            if (byte != was && threadIdx.x == 0) a.key_scales[page_head] = (uint8_t)byte;
-        }
-#pragma unroll
-        for (int c = 0; c < BLOCKS; c++) {
-            const int block = c * WAVES + wave;
+        u32x4 raw[kTurns][2];
+        auto ask = [&](int head) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < kTurns; t++) {
-                const int slot = block * kBlock + t * kRows + r;
-                if (slot < s0 || slot >= s1 || r >= kRows) continue;
+                raw[t][0] = raw[t][1] = u32x4{0, 0, 0, 0};
+                if (!in[t]) continue;
+                raw[t][0] = *reinterpret_cast<const u32x4*>(rows[t] + head * xh + d1);
+                raw[t][1] = *reinterpret_cast<const u32x4*>(rows[t] + head * xh + d2);
+            }
+        };
+        ask(head0);
+        for (int head = head0; head < head1; head++) {
+            float y[kTurns][16], top = 0.f;
+            const int64_t page_head = page_head0 + head;
+            const int was = EIGHT && !is_q && s0 ? scales[page_head] : 0;
+#pragma unroll
+            for (int t = 0; t < kTurns; t++) {
+                to_floats<T>(raw[t][0], y[t]);
+                to_floats<T>(raw[t][1], y[t] + 8);
+            }
+            if (head + 1 < head1) ask(head + 1);
+#pragma unroll
+            for (int t = 0; t < kTurns; t++) {
+                if (turned) turn(y[t], y[t] + 8, co[t], si[t]);
+                if (!in[t]) continue;
+                if (EIGHT) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) top = finite_max(top, y[t][e]);
+                }
+            }
+            float inv = 1.f;
+            if (EIGHT && !is_q) {
+                const Scale sc(of_page(top, head), was, s0 > 0);
+                inv = sc.inv;
+                if (sc.moves) move_keys(a.keys + page_head * page * D, s0, D, sc.factor, threadIdx.x, 64 * WAVES);
+                if (threadIdx.x == 0) scales_out[page_head] = (uint8_t)sc.byte;
+            }
+#pragma unroll
+            for (int t = 0; t < kTurns; t++) {
+                if (!in[t]) continue;
+                const int slot = wave * kBlock + t * kRows + r;
                 if (is_q || !EIGHT) {
-                    T* out = is_q ? static_cast<T*>(a.q_out) + (row0 + slot - s0) * a.os[0] + head * a.os[1] : reinterpret_cast<T*>(a.keys) + (page_head * page + slot) * D;
-                    *reinterpret_cast<u32x4*>(out + d1) = to_vector<T>(y[c][t]);
-                    *reinterpret_cast<u32x4*>(out + d2) = to_vector<T>(y[c][t] + 8);
+                    T* out = is_q ? static_cast<T*>(a.q_out) + (f.row + slot - s0) * a.os[0] + head * a.os[1] : reinterpret_cast<T*>(a.keys) + (page_head * page + slot) * D;
+                    put_stream<u32x4>(out + d1, to_vector<T>(y[t]));
+                    put_stream<u32x4>(out + d2, to_vector<T>(y[t] + 8));
                 } else {
                     char* out = a.keys + (page_head * page + slot) * D;
-                    *reinterpret_cast<u32x2*>(out + d1) = u32x2{pack8(y[c][t], inv), pack8(y[c][t] + 4, inv)};
-                    *reinterpret_cast<u32x2*>(out + d2) = u32x2{pack8(y[c][t] + 8, inv), pack8(y[c][t] + 12, inv)};
+                    put_stream<u32x2>(out + d1, u32x2{pack8(y[t], inv), pack8(y[t] + 4, inv)});
+                    put_stream<u32x2>(out + d2, u32x2{pack8(y[t] + 8, inv), pack8(y[t] + 12, inv)});
                 }
             }
         }
         return;
     }
 
-    // ---- values: a lane has two neighbouring d of kMine tokens, which lie side by side in the block
-    constexpr int kPairs = D / 2, kGroups = kPairs <= 16 ? 4 : kPairs <= 32 ? 2 : 1, kMine = kBlock / kGroups;
-    const int pair = lane % kPairs, group = lane / kPairs;
-    const bool mine = group < kGroups;
-    const T* x = static_cast<const T*>(a.v) + head * a.vs[1] + 2 * pair;
-    float y[BLOCKS][2][kMine];
-    float top = 0.f;
+    // ---- values: a lane reads a piece of a row, and writes two neighbouring d of kMine tokens, which lie side by side in the block
+    const int pr = lane / kPieces, pc = lane % kPieces, pair = lane % kPairs, group = lane / kPairs;
+    u32x4 raw[kReads];
+    auto ask = [&](int head) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < BLOCKS; c++)
+        for (int i = 0; i < kReads; i++) {
+            const int slot = wave * kBlock + i * kRead + pr;
+            raw[i] = u32x4{0, 0, 0, 0};
+            if (pr < kRead && slot >= s0 && slot < s1) raw[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.v) + (f.row + slot - s0) * a.vs[0] + head * a.vs[1] + 8 * pc);
+        }
+    };
+    ask(head0);
+    const int slot = wave * kBlock + group * kMine;
+    const bool mine = group < kGroups && slot + kMine > s0 && slot < s1, all = slot >= s0 && slot + kMine <= s1;
+    for (int head = head0; head < head1; head++) {
+        const int64_t page_head = page_head0 + head;
+        const int was = EIGHT && s0 ? scales[page_head] : 0;
+#pragma unroll
+        for (int i = 0; i < kReads; i++)
+            if (pr < kRead) *reinterpret_cast<u32x4*>(&turned_values[wave][i * kRead + pr][8 * pc]) = raw[i];
+        if (head + 1 < head1) ask(head + 1);
+        float y[2][kMine], top = 0.f;
 #pragma unroll
         for (int t = 0; t < kMine; t++) {
-            const int slot = (c * WAVES + wave) * kBlock + group * kMine + t;
-            uint32_t w = 0;
-            if (mine && slot >= s0 && slot < s1) w = *reinterpret_cast<const uint32_t*>(x + (row0 + slot - s0) * a.vs[0]);
-            y[c][0][t] = Elem<T>::to_f32(__builtin_bit_cast(T, (uint16_t)w));
-            y[c][1][t] = Elem<T>::to_f32(__builtin_bit_cast(T, (uint16_t)(w >> 16)));
-            if (EIGHT) top = finite_max(finite_max(top, y[c][0][t]), y[c][1][t]);
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(&turned_values[wave][(group % kGroups) * kMine + t][2 * pair]);
+            y[0][t] = Elem<T>::to_f32(__builtin_bit_cast(T, (uint16_t)w));
+            y[1][t] = Elem<T>::to_f32(__builtin_bit_cast(T, (uint16_t)(w >> 16)));
+            if (EIGHT) top = finite_max(finite_max(top, y[0][t]), y[1][t]);
         }
-    float inv = 1.f;
-    if (EIGHT) {
-        const int was = s0 ? max((int)a.value_scales[page_head], 1) : 0;
-        top = wave_max(top);
-        if (WAVES > 1) {
-            if (lane == 0) tops[wave] = top;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < WAVES; w++) top = fmaxf(top, tops[w]);
+        float inv = 1.f;
+        if (EIGHT) {
+            const Scale sc(of_page(top, head), was, s0 > 0);
+            inv = sc.inv;
+            if (sc.moves) move_values(a.values + page_head * page * D, s0, D, sc.factor, threadIdx.x, 64 * WAVES);
+            if (threadIdx.x == 0) scales_out[page_head] = (uint8_t)sc.byte;
         }
-        const int byte = max(scale_byte(top), was);
-        inv = scale_of(254 - byte);
-        if (s0 && byte > was) {
-            const float factor = scale_of(127 + was - byte > 0 ? 127 + was - byte : 1);
-            char* held = a.values + page_head * page * D;
-            const int whole = s0 / kBlock * D, rest = s0 % kBlock;               // sixteen bytes of a d each
-            for (int i = threadIdx.x; i < whole; i += 64 * WAVES) {
-                u32x4 w = reinterpret_cast<u32x4*>(held)[i];
-#pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = moved8(w[e], factor);
-                reinterpret_cast<u32x4*>(held)[i] = w;
-            }
-            for (int i = threadIdx.x; i < D * rest; i += 64 * WAVES) {           // (byte by byte: the bytes behind them are being written)
-                char* p = held + (whole + i / rest) * 16 + i % rest;
-                *p = (char)(moved8((uint8_t)*p, factor) & 255);
-            }
-        }
-        if (byte != was && threadIdx.x == 0) a.value_scales[page_head] = (uint8_t)byte;
-    }
-    if (!mine) return;
-#pragma unroll
-    for (int c = 0; c < BLOCKS; c++) {
-        const int block = c * WAVES + wave, slot = block * kBlock + group * kMine;
-        if (slot + kMine <= s0 || slot >= s1) continue;
+        if (!mine) continue;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const int64_t at16 = ((page_head * (page / kBlock) + block) * D + 2 * pair + j) * kBlock + group * kMine;
-            if (slot >= s0 && slot + kMine <= s1) {
+            const int64_t at16 = ((page_head * (page / kBlock) + wave) * D + 2 * pair + j) * kBlock + group * kMine;
+            if (all) {
                 if constexpr (EIGHT) {
                     uint32_t w[kMine / 4];
 #pragma unroll
-                    for (int e = 0; e < kMine / 4; e++) w[e] = pack8(y[c][j] + 4 * e, inv);
+                    for (int e = 0; e < kMine / 4; e++) w[e] = pack8(y[j] + 4 * e, inv);
                     __builtin_memcpy(__builtin_assume_aligned(a.values + at16, kMine), w, kMine);
                 } else {
                     T w[kMine];
 #pragma unroll
-                    for (int e = 0; e < kMine; e++) w[e] = Elem<T>::from_f32(y[c][j][e]);
+                    for (int e = 0; e < kMine; e++) w[e] = Elem<T>::from_f32(y[j][e]);
                     __builtin_memcpy(__builtin_assume_aligned(reinterpret_cast<T*>(a.values) + at16, kMine >= 8 ? 16 : 8), w, 2 * kMine);
                 }
             } else {
@@ -255,10 +309,10 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
                 for (int t = 0; t < kMine; t++) {
                     if (slot + t < s0 || slot + t >= s1) continue;
                     if constexpr (EIGHT) {
-                        const float four[4] = {y[c][j][t], 0.f, 0.f, 0.f};
+                        const float four[4] = {y[j][t], 0.f, 0.f, 0.f};
                         a.values[at16 + t] = (char)(pack8(four, inv) & 255);
                     } else {
-                        reinterpret_cast<T*>(a.values)[at16 + t] = Elem<T>::from_f32(y[c][j][t]);
+                        reinterpret_cast<T*>(a.values)[at16 + t] = Elem<T>::from_f32(y[j][t]);
                     }
                 }
             }
@@ -266,15 +320,125 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
     }
 }
 
+// A row of a token for D / 16 lanes: all new tokens of one page and one head of keys, values or queries, one after the other.  The first token's row stays in registers between the
+// search for the page's largest value and the store; further ones are read again.
 template <typename T, int D, bool EIGHT>
-int launch(hipStream_t st, const AppendArgs& a, int64_t units) {
-    const dim3 grid((unsigned)units, (unsigned)(2 * a.KV + (a.q ? a.H : 0)));
+__global__ __launch_bounds__(256) void append_few_kernel(AppendArgs a) {
+    constexpr int kLanes = D / 16, kItems = 64 / kLanes;                  // lanes of an item, items of a wave
+    const int lane = threadIdx.x & 63, l = lane % kLanes;
+    Fill f;
+    if (!f.find(a, blockIdx.x)) return;
+    const int item = ((int)blockIdx.y * 4 + (threadIdx.x >> 6)) * kItems + lane / kLanes;
+    const bool is_q = item >= 2 * a.KV, is_v = !is_q && item >= a.KV;
+    const int head = is_q ? item - 2 * a.KV : is_v ? item - a.KV : item;
+    if (lane >= kItems * kLanes || (is_q ? head >= a.H : (uint32_t)f.page_no >= (uint32_t)a.pages)) return;
+    const int page = 1 << a.s.page_shift;
+    const int64_t page_head = (int64_t)f.page_no * a.KV + head;
+    uint8_t* scales = is_v ? a.value_scales : a.key_scales;
+    const int was = EIGHT && !is_q && f.slot0 ? scales[page_head] : 0;
+
+    const bool turned = !is_v && l < a.R / 16;
+    const int d1 = is_v ? 16 * l : turned ? 8 * l : a.R + 16 * (l - a.R / 16), d2 = turned ? d1 + a.R / 2 : d1 + 8;
+    const T* x = is_q ? static_cast<const T*>(a.q) + head * a.qs[1] : is_v ? static_cast<const T*>(a.v) + head * a.vs[1] : static_cast<const T*>(a.k) + head * a.ks[1];
+    const int64_t xs = is_q ? a.qs[0] : is_v ? a.vs[0] : a.ks[0];
+    auto row_of = [&](int i, float (&y)[16]) __attribute__((always_inline)) {
+        const T* row = x + (f.row + i) * xs;
+        const u32x4 w1 = *reinterpret_cast<const u32x4*>(row + d1), w2 = *reinterpret_cast<const u32x4*>(row + d2);
+        f32x4 co[2], si[2];
+        if (turned) {
+            const f32x4* cs = reinterpret_cast<const f32x4*>(a.freqs + (int64_t)(f.pos + i) * a.R + 8 * l);
+            const f32x4* sn = reinterpret_cast<const f32x4*>(a.freqs + (int64_t)(f.pos + i) * a.R + 8 * l + a.R / 2);
+            co[0] = cs[0]; co[1] = cs[1];
+            si[0] = sn[0]; si[1] = sn[1];
+        }
+        to_floats<T>(w1, y);
+        to_floats<T>(w2, y + 8);
+        if (turned) turn(y, y + 8, co, si);
+    };
+    const int n = f.slot1 - f.slot0;
+    float y0[16], inv = 1.f;
+    row_of(0, y0);
+    if (EIGHT && !is_q) {
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; e++) top = finite_max(top, y0[e]);
+        for (int i = 1; i < n; i++) {
+            float y[16];
+            row_of(i, y);
+#pragma unroll
+            for (int e = 0; e < 16; e++) top = finite_max(top, y[e]);
+        }
+        if constexpr (kLanes == 6) {
+            const int base = lane - l;
+            float most = 0.f;
+#pragma unroll
+            for (int j = 0; j < kLanes; j++) most = fmaxf(most, __shfl(top, base + j, 64));
+            top = most;
+        } else {
+#pragma unroll
+            for (int j = 1; j < kLanes; j *= 2) top = fmaxf(top, __shfl_xor(top, j, 64));
+        }
+        const Scale sc(top, was, f.slot0 > 0);
+        inv = sc.inv;
+        if (sc.moves) {
+            if (is_v) move_values(a.values + page_head * page * D, f.slot0, D, sc.factor, l, kLanes);
+            else move_keys(a.keys + page_head * page * D, f.slot0, D, sc.factor, l, kLanes);
+        }
+        if (l == 0) scales[page_head] = (uint8_t)sc.byte;
+    }
+    for (int i = 0; i < n; i++) {
+        float y[16];
+        if (i == 0) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) y[e] = y0[e];
+        } else {
+            row_of(i, y);
+        }
+        const int slot = f.slot0 + i;
+        if (is_v) {
+            const int64_t at16 = ((page_head * (page / kBlock) + slot / kBlock) * D + d1) * kBlock + slot % kBlock;
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                if constexpr (EIGHT) {
+                    const uint32_t w = pack8(y + e, inv);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) a.values[at16 + (e + j) * kBlock] = (char)(w >> 8 * j);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) reinterpret_cast<T*>(a.values)[at16 + (e + j) * kBlock] = Elem<T>::from_f32(y[e + j]);
+                }
+            }
+        } else if (is_q || !EIGHT) {
+            T* out = is_q ? static_cast<T*>(a.q_out) + (f.row + i) * a.os[0] + head * a.os[1] : reinterpret_cast<T*>(a.keys) + (page_head * page + slot) * D;
+            *reinterpret_cast<u32x4*>(out + d1) = to_vector<T>(y);
+            *reinterpret_cast<u32x4*>(out + d2) = to_vector<T>(y + 8);
+        } else {
+            char* out = a.keys + (page_head * page + slot) * D;
+            *reinterpret_cast<u32x2*>(out + d1) = u32x2{pack8(y, inv), pack8(y + 4, inv)};
+            *reinterpret_cast<u32x2*>(out + d2) = u32x2{pack8(y + 8, inv), pack8(y + 12, inv)};
+        }
+    }
+}
+
+template <typename T, int D, bool EIGHT>
+int launch(hipStream_t st, AppendArgs a, int64_t units) {
+    if (a.s.T <= a.s.B) {
+        const int items = 4 * (64 / (D / 16));
+        hipLaunchKernelGGL((append_few_kernel<T, D, EIGHT>), dim3((unsigned)units, (unsigned)((2 * a.KV + a.H + items - 1) / items)), dim3(256), 0, st, a);
+        return check_launch("paged_append");
+    }
+    auto parts = [&](int heads) { return 2 * ((a.KV + heads - 1) / heads) + (a.H + heads - 1) / heads; };
+    // Heads of a workgroup: what they share (the page's place, cosines and sines) against waves to fill the device with.  us, one | two | four | eight heads: 9450 tokens as above 57.9 | 48.1 | 49.4 | 53.7 (15200,
+    // 7600 waves with two, four), 300 tokens 5.8 | 6.2 | 9.1 | 15.2, 32000 tokens 212 | 191 | 185 | 172
+    a.heads_a_part = 8;
+    while (a.heads_a_part > 1 && units * (1 << (a.s.page_shift - 4)) * parts(a.heads_a_part) < 7000) a.heads_a_part /= 2;
+    const dim3 grid((unsigned)units, (unsigned)parts(a.heads_a_part));
     switch (a.s.page_shift) {
-        case 4: hipLaunchKernelGGL((paged_append_kernel<T, D, EIGHT, 1, 1>), grid, dim3(64), 0, st, a); break;
-        case 5: hipLaunchKernelGGL((paged_append_kernel<T, D, EIGHT, 2, 1>), grid, dim3(128), 0, st, a); break;
-        case 6: hipLaunchKernelGGL((paged_append_kernel<T, D, EIGHT, 4, 1>), grid, dim3(256), 0, st, a); break;
-        case 7: hipLaunchKernelGGL((paged_append_kernel<T, D, EIGHT, 4, 2>), grid, dim3(256), 0, st, a); break;
-        default: hipLaunchKernelGGL((paged_append_kernel<T, D, EIGHT, 4, 4>), grid, dim3(256), 0, st, a); break;
+        case 4: hipLaunchKernelGGL((paged_append_kernel<T, D, EIGHT, 1>), grid, dim3(64), 0, st, a); break;
+        case 5: hipLaunchKernelGGL((paged_append_kernel<T, D, EIGHT, 2>), grid, dim3(128), 0, st, a); break;
+        case 6: hipLaunchKernelGGL((paged_append_kernel<T, D, EIGHT, 4>), grid, dim3(256), 0, st, a); break;
+        case 7: hipLaunchKernelGGL((paged_append_kernel<T, D, EIGHT, 8>), grid, dim3(512), 0, st, a); break;
+        default: hipLaunchKernelGGL((paged_append_kernel<T, D, EIGHT, 16>), grid, dim3(1024), 0, st, a); break;
     }
     return check_launch("paged_append");
 }
@@ -330,7 +494,7 @@ extern "C" int mhip_paged_append(void* stream, const mhip_paged_cache* cache, co
     for (int i = 0; i < (q ? 8 : 4); i++)
         if (strides[i] % 8) return fail(MHIP_ERR_UNSUPPORTED, "paged_append: strides must be multiples of 8 elements");
     AppendArgs a{k, v, q, q_out, freqs, (char*)cache->keys, (char*)cache->values, cache->key_scales, cache->value_scales, sequences(cache, seqs),
-                 (int)cache->pages, (int)cache->heads, (int)(q ? q_heads : 0), (int)rotated, (int)positions, {}, {}, {}, {}};
+                 (int)cache->pages, (int)cache->heads, (int)(q ? q_heads : 0), (int)rotated, (int)positions, 1, {}, {}, {}, {}};
     for (int i = 0; i < 2; i++) {
         a.ks[i] = strides[i];
         a.vs[i] = strides[2 + i];
