@@ -13,6 +13,7 @@
 // whose error of half a step each (2^-9 for bf16) is below the result's own rounding once it is averaged over keys.  Values in 8 bits become the queries' type exactly,
 // scale and all, except that f16 ends at 65504 and at 2^-24.
 #include <algorithm>
+#include <cmath>
 
 #include "arrive.h"
 #include "attention_common.h"
@@ -40,7 +41,8 @@ struct PagedArgs {
     const uint8_t *key_scales, *value_scales;
     Sequences s;
     int pages, KV, G, is_causal, shares;
-    float c;                                  // scale * log2(e)
+    float c;                                  // |scale| * log2(e), a tiny number instead of 0 (which times -inf is none)
+    uint32_t sign;                            // 0x80008000 where the scale is negative: of the queries
     int64_t qs[2], os[2];                     // token and head strides in elements
     float* part;                              // workspace, NULL: keys are not dealt
     uint64_t* words;
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
             const bool mine = row < rows && (!SINGLE || 16 * x + li < a.G);
             const T* qp = static_cast<const T*>(a.q) + (int64_t)(first + token) * a.qs[0] + (int64_t)(head * a.G + row - token * a.G) * a.qs[1];
 #pragma unroll
-            for (int s = 0; s < NS; s++) qf[x][s] = mine ? *reinterpret_cast<const u32x4*>(qp + d_of(s)) : u32x4{0, 0, 0, 0};
+            for (int s = 0; s < NS; s++) qf[x][s] = (mine ? *reinterpret_cast<const u32x4*>(qp + d_of(s)) : u32x4{0, 0, 0, 0}) ^ a.sign;
             limit[x] = SINGLE ? k1 : min(a.is_causal ? keys - tokens + token + 1 : keys, k1);
             open = min(open, mine ? limit[x] : k1);
         }
@@ -620,6 +622,15 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
 }
 
 // ---------------------------------------------------------------- many rows
+// x and the two numbers of w
+template <typename T>
+__device__ __forceinline__ float plus_two(uint32_t w, float x) {
+    typedef T two __attribute__((ext_vector_type(2)));
+    const two one = {(T)1.f, (T)1.f};
+    if constexpr (std::is_same<T, bf16_t>::value) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(two, w), one, x, false);
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(two, w), one, x, false);
+}
+
 // 128 rows, 32 a wave, over stages of 64 keys that lie in LDS in the queries' type, two of them: the next one is on its way in registers and is converted and put down
 // behind this one's products.
 //   S^T = K Q^T     v_mfma_f32_32x32x16: operand row i of tile j is key 32 j + 16 (r / 8) + 8 h + r % 8 where register r of half h of the result is row i, so that
@@ -753,7 +764,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
     {
         const T* qp = static_cast<const T*>(a.q) + (int64_t)(first + token) * a.qs[0] + (int64_t)(head * a.G + row - token * a.G) * a.qs[1];
 #pragma unroll
-        for (int s = 0; s < NS; s++) qf[s] = row < rows ? *reinterpret_cast<const u32x4*>(qp + 16 * s + 8 * lh) : u32x4{0, 0, 0, 0};
+        for (int s = 0; s < NS; s++) qf[s] = (row < rows ? *reinterpret_cast<const u32x4*>(qp + 16 * s + 8 * lh) : u32x4{0, 0, 0, 0}) ^ a.sign;
     }
     const int limit = row < rows ? min(a.is_causal ? keys - tokens + token + 1 : keys, k1) : 0;
     const int open = -(int)wave_max((float)-(row < rows ? limit : k1));              // blocks in front of it need no mask
@@ -816,7 +827,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
         }
     };
     auto put_v = [&](Stage& st, uint32_t absent, int key, char* to, bool tame) __attribute__((always_inline)) {
-        const bool leave = tame && key + kStage > mixed;
+        const bool leave = tame && key + kStage > mixed, last_ones = key + kStage > k1 || absent;
 #pragma unroll
         for (int i = 0; i < kMine; i++) {
             const int idx = threadIdx.x + 256 * i;
@@ -824,8 +835,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
             u32x4 w = values_of(st)[i];
             const int block = idx / kPer, d = idx % kPer / SIZE, half = EIGHT ? 0 : idx & 1;
             // values that no key of this part stands for may hold anything, a NaN among it
-            const int n = absent >> block & 1 ? 0 : k1 - key - 16 * block - 8 * half;
-            if (n < 16 / SIZE) {
+            if (last_ones) {
+                const int n = absent >> block & 1 ? 0 : k1 - key - 16 * block - 8 * half;
                 constexpr int kOf = 4 / SIZE;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -856,7 +867,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
     // row li of a tile of S^T is key `of` of its 32
     const int of = 16 * (li >> 4) + 8 * ((li >> 2) & 1) + 4 * ((li >> 3) & 1) + (li & 3);
 
-    auto scores = [&](f32x16 (&sv)[2], const char* from, int key, uint32_t absent) __attribute__((always_inline)) {
+    auto scores = [&](u32x4 (&pb)[4], const char* from, int key, uint32_t absent) __attribute__((always_inline)) {
+        f32x16 sv[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             sv[j] = f32x16{};
@@ -872,46 +884,40 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
                 for (int r = 0; r < 16; r++) {
                     const int at = 32 * j + 16 * (r >> 3) + 8 * lh + (r & 7);
                     const bool in = key + at < limit && !(absent >> (2 * j + (r >> 3)) & 1);
-                    sv[j][r] = in ? sv[j][r] * a.c : -INFINITY;
-                    top = fmaxf(top, sv[j][r]);
-                }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    sv[j][r] *= a.c;
-                    top = fmaxf(top, sv[j][r]);
+                    sv[j][r] = in ? sv[j][r] : -INFINITY;
                 }
         }
-        top = half_max(top);
-        const float m_new = moved_reference(m_run, top), use = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = weight(m_run, use);
-        m_run = m_new;
-        float lsum = 0.f;
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                sv[j][r] = weight(sv[j][r], use);
-                lsum += sv[j][r];
+            for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(top, sv[j][r]), sv[j][r + 1]);
+        // (the products are scaled in one step with the subtraction; a.c > 0)
+        top = half_max(top) * a.c;
+        const float m_new = moved_reference(m_run, top), use = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = weight(m_run, use);
+        m_run = m_new;
+        // the sum is that of the rounded weights, which are the ones that the values are multiplied with
+        float lsum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                const uint32_t two = Mfma32A<T>::pack2(__builtin_amdgcn_exp2f(fmaf(sv[j][r], a.c, -use)), __builtin_amdgcn_exp2f(fmaf(sv[j][r + 1], a.c, -use)));
+                pb[2 * j + (r >> 3)][(r >> 1) & 3] = two;
+                lsum[j] = plus_two<T>(two, lsum[j]);
             }
-        l_run = l_run * alpha + lsum;
+        l_run = l_run * alpha + (lsum[0] + lsum[1]);
         if (__any(alpha != 1.f)) {
 #pragma unroll
             for (int f = 0; f < NF; f++) oacc[f] *= alpha;
         }
     };
-    auto product = [&](const f32x16 (&sv)[2], const char* from) __attribute__((always_inline)) {
+    auto product = [&](const u32x4 (&pb)[4], const char* from) __attribute__((always_inline)) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ks++) {
-            u32x4 pb;
-#pragma unroll
-            for (int e = 0; e < 4; e++) pb[e] = Mfma32A<T>::pack2(sv[ks >> 1][8 * (ks & 1) + 2 * e], sv[ks >> 1][8 * (ks & 1) + 2 * e + 1]);
+        for (int ks = 0; ks < 4; ks++)
 #pragma unroll
             for (int f = 0; f < NF; f++)
-                oacc[f] = Mfma32A<T>::run(*reinterpret_cast<const u32x4*>(from + kKBytes + tv_off(32 * f + li, 2 * ks + lh)), pb, oacc[f]);
-        }
+                oacc[f] = Mfma32A<T>::run(*reinterpret_cast<const u32x4*>(from + kKBytes + tv_off(32 * f + li, 2 * ks + lh)), pb[ks], oacc[f]);
     };
 
     auto go = [&](bool tame) __attribute__((always_inline)) {
@@ -937,14 +943,14 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
                     ask(pg, key + 2 * kStage);
                 }
             }
-            f32x16 sv[2];
-            if (key < seen_keys) scores(sv, lds[at], key, absent);
+            u32x4 pb[4];
+            if (key < seen_keys) scores(pb, lds[at], key, absent);
             if (kApart && more) {
                 put_k(st, lds[at ^ 1]);
                 load_v(st, pg, key + kStage);
                 ask(pg, key + 2 * kStage);
             }
-            if (key < seen_keys) product(sv, lds[at]);
+            if (key < seen_keys) product(pb, lds[at]);
             if (more) {
                 if constexpr (!kApart) put_k(st, lds[at ^ 1]);
                 put_v(st, then, key + kStage, lds[at ^ 1], tame);
@@ -1079,7 +1085,7 @@ extern "C" int mhip_paged_attention(void* stream, const mhip_paged_cache* cache,
     if (seqs->tokens * (q_heads / cache->heads) >= 1 << 30) return fail(MHIP_ERR_UNSUPPORTED, "paged_attention: more than 2^30 rows");
     const Plan p = plan_of(cache, seqs, q_heads);
     PagedArgs a{q, o, (const char*)cache->keys, (const char*)cache->values, cache->key_scales, cache->value_scales, sequences(cache, seqs),
-                (int)cache->pages, (int)cache->heads, (int)(q_heads / cache->heads), is_causal ? 1 : 0, p.shares, scale * kLog2e, {strides[0], strides[1]}, {strides[2], strides[3]},
+                (int)cache->pages, (int)cache->heads, (int)(q_heads / cache->heads), is_causal ? 1 : 0, p.shares, scale == 0.f ? 1e-30f : std::fabs(scale) * kLog2e, std::signbit(scale) ? 0x80008000u : 0u, {strides[0], strides[1]}, {strides[2], strides[3]},
                 nullptr, nullptr, 0, Divider((uint32_t)(q_heads / cache->heads)), Divider((uint32_t)cache->heads), Divider((uint32_t)p.shares), p.unit_shift};
     if (workspace && workspace_bytes >= workspace_of(cache, p)) {
         a.part = static_cast<float*>(workspace);
