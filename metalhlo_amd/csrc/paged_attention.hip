@@ -195,50 +195,74 @@ __device__ __forceinline__ u32x2 load_two(const float* p) {
 }
 
 // By the last workgroup of a tile: its parts put together in order.  `rows`: of the tile, from row `row0` of the sequence that starts at token `start`.
+// The sums of a tile of few rows lie row by row, those of many as the lanes of their waves hold them (the stores pass the L2: sixteen bytes of each of 64 rows at a time went to memory as such).
 template <typename T, int ROWS, int D, int THREADS>
 __device__ __forceinline__ void join(const PagedArgs& a, const Split& split, int start, int head, int row0, int rows) {
-    constexpr int kFours = D / 4;
-    // AHEAD parts are asked for at once: up to 16 of them arrive after one latency
-    auto put = [&](auto ahead) __attribute__((always_inline)) {
-        constexpr int AHEAD = decltype(ahead)::value;
-        for (int idx = threadIdx.x; idx < rows * kFours; idx += THREADS) {
-            const int row = idx / kFours, four = idx % kFours;
-            float m = -INFINITY, l = 0.f;
-            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    constexpr int kFours = D / 4, kAll = (ROWS * kFours + THREADS - 1) / THREADS;             // fours of numbers of a row; a thread's of a full tile
+    constexpr bool kByLanes = ROWS > 32;
+    const int all = kByLanes ? (rows + 31) / 32 * 32 * kFours : rows * kFours;
+    auto row_of = [](int idx) { return kByLanes ? idx / (64 * (D / 8)) * 32 + (idx & 31) : idx / kFours; };
+    auto four_of = [](int idx) { return kByLanes ? (idx >> 6) % (D / 8) * 2 + (idx >> 5 & 1) : idx % kFours; };
+    // AHEAD parts of ITEMS fours are asked for at once, sixteen loads that arrive after one latency: with one four at a time the sixteen of a tile of 128 rows took 40 us
+    auto put = [&](auto ahead, auto items) __attribute__((always_inline)) {
+        constexpr int AHEAD = decltype(ahead)::value, ITEMS = decltype(items)::value < kAll ? decltype(items)::value : kAll;
+        for (int idx0 = threadIdx.x; idx0 < all; idx0 += ITEMS * THREADS) {
+            float m[ITEMS], l[ITEMS];
+            f32x4 o[ITEMS];
+#pragma unroll
+            for (int i = 0; i < ITEMS; i++) {
+                m[i] = -INFINITY;
+                l[i] = 0.f;
+                o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
             for (int p0 = 0; p0 < split.parts; p0 += AHEAD) {
-                u32x2 st[AHEAD];
-                f32x4 v[AHEAD];
+                u32x2 st[ITEMS][AHEAD];
+                f32x4 v[ITEMS][AHEAD];
 #pragma unroll
                 for (int p = 0; p < AHEAD; p++) {
                     const int q = min(p0 + p, split.parts - 1);
                     const Parts<ROWS, D> at(a, 2 * (split.first + q) + (q ? 0 : 1));
-                    st[p] = load_two(at.state + 2 * row);
-                    v[p] = load_part(parts_rsrc(at.sums), (uint32_t)((row * kFours + four) * 16));
+#pragma unroll
+                    for (int i = 0; i < ITEMS; i++) {
+                        const int idx = min(idx0 + i * THREADS, all - 1);
+                        st[i][p] = load_two(at.state + 2 * row_of(idx));
+                        v[i][p] = load_part(parts_rsrc(at.sums), (uint32_t)(idx * 16));
+                    }
                 }
-                float top = m;
 #pragma unroll
-                for (int p = 0; p < AHEAD; p++) top = fmaxf(top, p0 + p < split.parts ? __builtin_bit_cast(float, (uint32_t)st[p].x) : -INFINITY);
-                const float use = top == -INFINITY ? 0.f : top, old = weight(m, use);
-                m = top;
-                l *= old;
-                o *= old;
+                for (int i = 0; i < ITEMS; i++) {
+                    float top = m[i];
 #pragma unroll
-                for (int p = 0; p < AHEAD; p++) {
-                    const float al = p0 + p < split.parts ? weight(__builtin_bit_cast(float, (uint32_t)st[p].x), use) : 0.f;
-                    l = fmaf(__builtin_bit_cast(float, (uint32_t)st[p].y), al, l);
+                    for (int p = 0; p < AHEAD; p++) top = fmaxf(top, p0 + p < split.parts ? __builtin_bit_cast(float, (uint32_t)st[i][p].x) : -INFINITY);
+                    const float use = top == -INFINITY ? 0.f : top, old = weight(m[i], use);
+                    m[i] = top;
+                    l[i] *= old;
+                    o[i] *= old;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[e] = fmaf(v[p][e], al, o[e]);
+                    for (int p = 0; p < AHEAD; p++) {
+                        const float al = p0 + p < split.parts ? weight(__builtin_bit_cast(float, (uint32_t)st[i][p].x), use) : 0.f;
+                        l[i] = fmaf(__builtin_bit_cast(float, (uint32_t)st[i][p].y), al, l[i]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[i][e] = fmaf(v[i][p][e], al, o[i][e]);
+                    }
                 }
             }
-            const float inv = l != 0.f ? 1.f / l : 0.f;
-            const int r = row0 + row, token = a.by_group(r);
-            T* out = static_cast<T*>(a.o) + (int64_t)(start + token) * a.os[0] + (int64_t)(head * a.G + r - token * a.G) * a.os[1] + 4 * four;
-            *reinterpret_cast<u32x2*>(out) = u32x2{Mfma32A<T>::pack2(o[0] * inv, o[1] * inv), Mfma32A<T>::pack2(o[2] * inv, o[3] * inv)};
+#pragma unroll
+            for (int i = 0; i < ITEMS; i++) {
+                const int idx = idx0 + i * THREADS;
+                if (idx >= all || row_of(idx) >= rows) continue;
+                const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;
+                const int r = row0 + row_of(idx), token = a.by_group(r);
+                T* out = static_cast<T*>(a.o) + (int64_t)(start + token) * a.os[0] + (int64_t)(head * a.G + r - token * a.G) * a.os[1] + 4 * four_of(idx);
+                *reinterpret_cast<u32x2*>(out) = u32x2{Mfma32A<T>::pack2(o[i][0] * inv, o[i][1] * inv), Mfma32A<T>::pack2(o[i][2] * inv, o[i][3] * inv)};
+            }
         }
     };
-    if (split.parts <= 4) put(std::integral_constant<int, 4>{});
-    else if (split.parts <= 8 || ROWS > 32) put(std::integral_constant<int, 8>{});
-    else put(std::integral_constant<int, 16>{});
+    using std::integral_constant;
+    if (ROWS > 32 && split.parts <= 2) put(integral_constant<int, 2>{}, integral_constant<int, 8>{});
+    else if (split.parts <= 4) put(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    else if (split.parts <= 8 || ROWS > 32) put(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+    else put(integral_constant<int, 16>{}, integral_constant<int, 1>{});
 }
 
 // ---------------------------------------------------------------- few rows
@@ -631,11 +655,13 @@ __device__ __forceinline__ float plus_two(uint32_t w, float x) {
     else return __builtin_amdgcn_fdot2(__builtin_bit_cast(two, w), one, x, false);
 }
 
-// 128 rows, 32 a wave, over stages of 64 keys that lie in LDS in the queries' type, two of them: the next one is on its way in registers and is converted and put down
+// 128 rows, 32 a wave (256 in eight waves where keys of 128 numbers lie in 16 bits and sequences have as many rows: a thread has half the pieces to stage, so keys and values are asked for together.
+// us, 128 rows | 256: four pieces of 1024 tokens behind 7168 702 | 641, one of 512 behind 32000 361 | 345, prompts of 2048 tokens 212 | 207, 512 rows over 2000 keys 76 | 69; but heads of 96 566 | 615 and
+// 8-bit pages 297 | 299, 195 | 198: there two workgroups, one at its products while the other is at its weights, are worth more), over stages of 64 keys that lie in LDS in the queries' type, two of them: the next one is on its way in registers and is converted and put down
 // behind this one's products.
 //   S^T = K Q^T     v_mfma_f32_32x32x16: operand row i of tile j is key 32 j + 16 (r / 8) + 8 h + r % 8 where register r of half h of the result is row i, so that
 //   O^T += V^T P^T  a half's eight registers of a step are the probabilities of eight neighbouring keys: sixteen bytes of a row of V^T.
-constexpr int kTileRows = 128, kStage = 64;
+constexpr int kStage = 64;
 
 template <int D>
 __device__ __forceinline__ uint32_t tk_off(int key, int chunk) {          // K [64][D]: chunks of eight elements, rotated by the key
@@ -647,13 +673,14 @@ __device__ __forceinline__ uint32_t tv_off(int d, int chunk) {            // V^T
     return (uint32_t)(d * 128 + ((chunk ^ ((d >> 1) & 7)) << 4));
 }
 
-// The line's stretches: a tile's is its keys and what a tile costs besides (kTileCost keys' worth), which grows from tile to tile by the tokens of one where the causal rule holds; head by head.
-constexpr int kTileCost = 128;
+// The line's stretches: a tile's is its keys and what a tile costs besides (kTileCost keys' worth: 16 times 64 tokens behind 2000 take 84 us where it is 128, 74 with 400, 76 with 600), which grows from tile to tile by the tokens of one where the causal rule holds; head by head.
+constexpr int kTileCost = 384;
+template <int ROWS>
 struct Stretch {
     int tiles, first, grows;
     __device__ __forceinline__ Stretch(const PagedArgs& a, int tokens, int keys) {
-        const int wide = (kTileRows + a.G - 1) / a.G;
-        tiles = (tokens * a.G + kTileRows - 1) / kTileRows;
+        const int wide = a.by_group(ROWS + a.G - 1);
+        tiles = (tokens * a.G + ROWS - 1) / ROWS;
         first = (((a.is_causal ? max(keys - tokens, 0) + wide : keys) + kTileCost) >> a.unit_shift) + 1;
         grows = a.is_causal ? wide >> a.unit_shift : 0;
     }
@@ -670,13 +697,14 @@ struct Stretch {
     }
 };
 
-template <typename T, int D, bool EIGHT>
-__global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
+template <typename T, int D, bool EIGHT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_tile_kernel(PagedArgs a) {
+    constexpr int ROWS = 32 * WAVES, kThreads = 64 * WAVES;
     constexpr int NS = D / 16, NF = D / 32, SIZE = EIGHT ? 1 : 2;
     constexpr int kKBytes = D == 96 ? 64 * 208 : 64 * D * 2, kVBytes = D * 128;
-    constexpr int kPieces = 64 * D * SIZE / 16, kMine = (kPieces + 255) / 256;      // pieces of sixteen bytes of K, and of V, of a stage; a thread's
+    constexpr int kPieces = 64 * D * SIZE / 16, kMine = (kPieces + kThreads - 1) / kThreads;      // pieces of sixteen bytes of K, and of V, of a stage; a thread's
     __shared__ __attribute__((aligned(16))) char lds[2][kKBytes + kVBytes];
-    __shared__ Known known[4];
+    __shared__ Known known[WAVES];
     __shared__ int last;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 31, lh = lane >> 5;
@@ -685,7 +713,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
     known_of(a.s, known[wave], lane);
     int longest = 1, shortest = 1 << 30, all = 0, count = 0;
     auto add = [&](int tokens, int keys) __attribute__((always_inline)) {
-        const Stretch st(a, tokens, keys);
+        const Stretch<ROWS> st(a, tokens, keys);
         if (!st.tiles) return;
         longest = max(longest, st.length(st.tiles - 1));
         shortest = min(shortest, st.first);
@@ -698,9 +726,10 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
     shortest = -(int)wave_max((float)-shortest);
     all = __builtin_amdgcn_readlane(wave_scan(all), 63) * a.KV;
     count = __builtin_amdgcn_readlane(wave_scan(count), 63) * a.KV;
-    // Where there is a tile for every share, and short ones that come last and fill the gaps (a prompt from its beginning), a workgroup takes one whole tile instead, and none is joined; so it does
-    // without a workspace.  us, shares | tiles: four prompts of 2048 tokens 270 | 196, one of 4000 199 | 180; three pieces of 550 to 930 tokens behind 5000 to 7000 304 | 480
-    const bool tiles = !a.part || (count >= a.shares && shortest <= 5 * kTileCost >> a.unit_shift);
+    // Where no tile has many keys, or there is a tile for every share and short ones that come last and fill the gaps (a prompt from its beginning), a workgroup takes one whole tile instead, and
+    // none is joined; so it does without a workspace.  us, shares | tiles: 16 times 64 tokens behind 500 45 | 29, two of 512 50 | 42, one of 300 behind 2000 46 | 81; four prompts of 2048 tokens
+    // 270 | 196, one of 4000 199 | 180; three pieces of 550 to 930 tokens behind 5000 to 7000 304 | 480
+    const bool tiles = !a.part || longest <= (1024 + kTileCost) >> a.unit_shift || (count >= a.shares && shortest <= (512 + kTileCost) >> a.unit_shift);
     const Line line(a.by_shares, a.shares, all, longest);
     if ((int)blockIdx.x >= (tiles ? count : a.shares)) return;
     const int share = a.shares & 7 ? blockIdx.x : (blockIdx.x & 7) * (a.shares >> 3) + (blockIdx.x >> 3);
@@ -716,10 +745,10 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
         int level;
         if (a.s.B <= 64) {
             // the last tiles of all sequences, then those in front of them, ...: `level` of them lie in front of this one's
-            const int own = (known[wave].tokens[lane] * a.G + kTileRows - 1) / kTileRows;
+            const int own = (known[wave].tokens[lane] * a.G + ROWS - 1) / ROWS;
             auto before = [&](int n) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(wave_scan(min(own, n)), 63); };
             int low = 0;
-            for (int step = 1 << (31 - __builtin_clz(a.s.T * a.G / kTileRows + 1)); step; step >>= 1)
+            for (int step = 1 << (31 - __builtin_clz(a.s.T * a.G / ROWS + 1)); step; step >>= 1)
                 if (before(low + step) <= unit) low += step;
             level = low;
             const int has = own > level ? 1 : 0, place = wave_scan(has) - has, wanted = unit - before(level);
@@ -730,16 +759,16 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
             found.tokens = __builtin_amdgcn_readfirstlane(known[wave].tokens[found.b]);
             found.keys = __builtin_amdgcn_readfirstlane(known[wave].keys[found.b]);
         } else {
-            if (!found_at(a.s, known[wave], lane, unit, [&](int tokens, int keys) { return Stretch(a, tokens, keys).tiles; }, found)) return;
+            if (!found_at(a.s, known[wave], lane, unit, [&](int tokens, int keys) { return Stretch<ROWS>(a, tokens, keys).tiles; }, found)) return;
             level = unit - found.before;
         }
-        const Stretch st(a, found.tokens, found.keys);
+        const Stretch<ROWS> st(a, found.tokens, found.keys);
         tile = st.tiles - 1 - level;
         off1 = length = st.length(tile);
         g = stop;
     } else {
-        if (!found_at(a.s, known[wave], lane, g, [&](int tokens, int keys) { const Stretch st(a, tokens, keys); return a.KV * st.before(st.tiles); }, found)) return;
-        const Stretch st(a, found.tokens, found.keys);
+        if (!found_at(a.s, known[wave], lane, g, [&](int tokens, int keys) { const Stretch<ROWS> st(a, tokens, keys); return a.KV * st.before(st.tiles); }, found)) return;
+        const Stretch<ROWS> st(a, found.tokens, found.keys);
         const int of_head = st.before(st.tiles), x = g - found.before;
         head = x / of_head;
         tile = st.tile(x - head * of_head);
@@ -750,9 +779,9 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
         g += off1 - off0;
     }
     const int tokens = found.tokens, keys = found.keys, first = found.start;
-    const int rows = tokens * a.G, row = tile * kTileRows + 32 * wave + li, token = a.by_group(row);
+    const int rows = tokens * a.G, row = tile * ROWS + 32 * wave + li, token = a.by_group(row);
     int end = keys;                                                          // of the keys that the tile's last row sees
-    if (a.is_causal) end = max(keys - tokens + a.by_group(min((tile + 1) * kTileRows, rows) - 1) + 1, 0);
+    if (a.is_causal) end = max(keys - tokens + a.by_group(min((tile + 1) * ROWS, rows) - 1) + 1, 0);
     auto cut = [&](int off) __attribute__((always_inline)) { return off == 0 ? 0 : off >= length ? end : min(max((off << a.unit_shift) - 96, 0) & ~(kStage - 1), end); };
     const int k0 = cut(off0), k1 = cut(off1);
     const bool parted = off0 > 0 || off1 < length;
@@ -769,7 +798,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
     const int limit = row < rows ? min(a.is_causal ? keys - tokens + token + 1 : keys, k1) : 0;
     const int open = -(int)wave_max((float)-(row < rows ? limit : k1));              // blocks in front of it need no mask
     const int seen_keys = (int)wave_max((float)limit);                               // blocks behind it concern no row of the wave
-    const int mixed = a.is_causal ? keys - tokens + a.by_group(tile * kTileRows) + 1 : k1;       // keys from here on are seen by some rows of the tile only
+    const int mixed = a.is_causal ? keys - tokens + a.by_group(tile * ROWS) + 1 : k1;       // keys from here on are seen by some rows of the tile only
 
     const int32_t* table = a.s.table + (int64_t)found.b * a.s.width;
     uniform_words scalar_table = (uniform_words)(uintptr_t)table;
@@ -777,7 +806,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
     constexpr int kPer = D * SIZE;
     const int page_blocks = a.s.page_shift - 4;
     // In 16 bits a thread's pieces of both do not fit the registers: values are asked for when the next keys lie in LDS
-    constexpr bool kApart = !EIGHT && D > 64;
+    constexpr bool kApart = !EIGHT && D > 64 && WAVES == 4;
     struct Stage { u32x4 k[kMine], v[kApart ? 1 : kMine]; uint32_t ks[kMine], vs[kMine]; };
     struct Pages { int at[kMine]; uint32_t absent; };       // bit i of `absent`: the table names no page for block i
     auto ask = [&](Pages& p, int key) __attribute__((always_inline)) {
@@ -789,7 +818,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < kMine; i++) {
-            const int block = ((int)threadIdx.x + 256 * i) / kPer;
+            const int block = ((int)threadIdx.x + kThreads * i) / kPer;
             const int at = min(((key >> 4) + (kPer % 64 ? block : __builtin_amdgcn_readfirstlane(block))) >> page_blocks, a.s.width - 1);
             const int page = kPer % 64 ? table[at] : scalar_table[at];
             p.at[i] = ((uint32_t)page < (uint32_t)a.pages ? page : 0) * a.KV + head;
@@ -798,8 +827,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
     auto load = [&](u32x4 (&w)[kMine], uint32_t (&scale)[kMine], const char* from, const uint8_t* scales, const Pages& p, int key) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kMine; i++) {
-            const int idx = threadIdx.x + 256 * i;
-            if (kPieces % 256 && idx >= kPieces) continue;
+            const int idx = threadIdx.x + kThreads * i;
+            if (kPieces % kThreads && idx >= kPieces) continue;
             const int block = ((key >> 4) + (kPer % 64 ? idx / kPer : __builtin_amdgcn_readfirstlane(idx / kPer))) & ((1 << page_blocks) - 1);
             w[i] = *reinterpret_cast<const u32x4*>(from + (((int64_t)p.at[i] << page_blocks) + block) * (16 * kPer) + idx % kPer * 16);
             if (EIGHT) scale[i] = scales[p.at[i]];
@@ -815,8 +844,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
         constexpr int kKeyPieces = D * SIZE / 16;
 #pragma unroll
         for (int i = 0; i < kMine; i++) {
-            const int idx = threadIdx.x + 256 * i, k = idx / kKeyPieces, kc = idx % kKeyPieces;
-            if (kPieces % 256 && idx >= kPieces) continue;
+            const int idx = threadIdx.x + kThreads * i, k = idx / kKeyPieces, kc = idx % kKeyPieces;
+            if (kPieces % kThreads && idx >= kPieces) continue;
             if constexpr (EIGHT) {
                 const float scale = scale_of(st.ks[i]);
                 *reinterpret_cast<u32x4*>(to + tk_off<D>(k, 2 * kc)) = widen<T>(u32x2{st.k[i].x, st.k[i].y}, scale);
@@ -830,8 +859,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
         const bool leave = tame && key + kStage > mixed, last_ones = key + kStage > k1 || absent;
 #pragma unroll
         for (int i = 0; i < kMine; i++) {
-            const int idx = threadIdx.x + 256 * i;
-            if (kPieces % 256 && idx >= kPieces) continue;
+            const int idx = threadIdx.x + kThreads * i;
+            if (kPieces % kThreads && idx >= kPieces) continue;
             u32x4 w = values_of(st)[i];
             const int block = idx / kPer, d = idx % kPer / SIZE, half = EIGHT ? 0 : idx & 1;
             // values that no key of this part stands for may hold anything, a NaN among it
@@ -869,6 +898,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
 
     auto scores = [&](u32x4 (&pb)[4], const char* from, int key, uint32_t absent) __attribute__((always_inline)) {
         f32x16 sv[2];
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             sv[j] = f32x16{};
@@ -876,6 +906,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
             for (int s = 0; s < NS; s++)
                 sv[j] = Mfma32A<T>::run(*reinterpret_cast<const u32x4*>(from + tk_off<D>(32 * j + of, 2 * s + lh)), qf[s], sv[j]);
         }
+        __builtin_amdgcn_s_setprio(0);
         float top = -INFINITY;
         if (key + kStage > open || absent) {
 #pragma unroll
@@ -913,11 +944,13 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
         }
     };
     auto product = [&](const u32x4 (&pb)[4], const char* from) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int ks = 0; ks < 4; ks++)
 #pragma unroll
             for (int f = 0; f < NF; f++)
                 oacc[f] = Mfma32A<T>::run(*reinterpret_cast<const u32x4*>(from + kKBytes + tv_off(32 * f + li, 2 * ks + lh)), pb[ks], oacc[f]);
+        __builtin_amdgcn_s_setprio(0);
     };
 
     auto go = [&](bool tame) __attribute__((always_inline)) {
@@ -1007,7 +1040,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
         continue;
     }
     if (threadIdx.x == 0) arrive_claim(a.words + split.first, seen, a.tag);
-    const Parts<kTileRows, D> own(a, 2 * share + (off0 ? 0 : 1));
+    const Parts<ROWS, D> own(a, 2 * share + (off0 ? 0 : 1));
     if (row < rows) {
         const __amdgpu_buffer_rsrc_t rs = parts_rsrc(own.sums);
         const int r = 32 * wave + li;
@@ -1015,10 +1048,10 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedArgs a) {
         for (int f = 0; f < NF; f++)
 #pragma unroll
             for (int g = 0; g < 4; g++)
-                store_part(rs, (uint32_t)((r * D + 32 * f + 8 * g + 4 * lh) * 4), f32x4{oacc[f][4 * g], oacc[f][4 * g + 1], oacc[f][4 * g + 2], oacc[f][4 * g + 3]});
+                store_part(rs, (uint32_t)((((wave * NF + f) * 4 + g) * 64 + lane) * 16), f32x4{oacc[f][4 * g], oacc[f][4 * g + 1], oacc[f][4 * g + 2], oacc[f][4 * g + 3]});
         if (lh == 0) store_two(own.state + 2 * r, m_run, l_run);
     }
-    if (arrive_last(a.words + split.first, split.parts, &last)) join<T, kTileRows, D, 256>(a, split, first, head, tile * kTileRows, min(kTileRows, rows - tile * kTileRows));
+    if (arrive_last(a.words + split.first, split.parts, &last)) join<T, ROWS, D, kThreads>(a, split, first, head, tile * ROWS, min(ROWS, rows - tile * ROWS));
     }
 }
 
@@ -1027,15 +1060,15 @@ struct Plan { int rows, shares, unit_shift; bool single; int64_t tiles; };
 
 Plan plan_of(const mhip_paged_cache* c, const mhip_sequences* s, int64_t q_heads) {
     const int64_t G = q_heads / c->heads, average = (s->tokens + s->sequences - 1) / s->sequences * G;
-    const int rows = average <= 16 ? 16 : average <= 32 ? 32 : kTileRows;
+    const int rows = average <= 16 ? 16 : average <= 32 ? 32 : average >= 256 && c->head_size == 128 && !c->key_scales ? 256 : 128;
     const double tiles = (double)(s->tokens * G / rows + (s->sequences < s->tokens ? s->sequences : s->tokens)) * c->heads;      // that there can be
     const int64_t keys = s->width * c->page_size;
-    auto most = [&](int shift) { return rows == kTileRows ? tiles * (double)((2 * (keys + 2 * kTileCost) >> shift) + 1) : tiles * (double)((keys >> shift) + 1); };
-    const bool single = s->tokens <= s->sequences && G <= rows && rows != kTileRows;
-    int shift = rows == kTileRows ? 0 : kStepShift;
+    auto most = [&](int shift) { return rows >= 128 ? tiles * (double)((2 * (keys + 2 * kTileCost) >> shift) + 1) : tiles * (double)((keys >> shift) + 1); };
+    const bool single = s->tokens <= s->sequences && G <= rows && rows < 128;
+    int shift = rows >= 128 ? 0 : kStepShift;
     while (most(shift) > (double)(1 << 29)) shift++;
-    int shares = (rows == kTileRows ? 2 : rows_kernel_workgroups(rows / 16, c->head_size, single)) * compute_units();
-    if (rows != kTileRows && most(shift) < shares) shares = (int)most(shift);                                                     // (a step is the least share)
+    int shares = (rows >= 128 ? 256 / rows : rows_kernel_workgroups(rows / 16, c->head_size, single)) * compute_units();
+    if (rows < 128 && most(shift) < shares) shares = (int)most(shift);                                                     // (a step is the least share)
     return {rows, shares, shift, single, (int64_t)tiles};
 }
 
@@ -1043,12 +1076,13 @@ int64_t workspace_of(const mhip_paged_cache* c, const Plan& p) { return (int64_t
 
 template <typename T, int D, bool EIGHT>
 int launch(hipStream_t st, const PagedArgs& a, const Plan& p) {
-    const dim3 grid((unsigned)(p.rows == kTileRows && (!a.part || p.tiles >= p.shares) ? std::max<int64_t>(p.tiles, p.shares) : p.shares));
+    const dim3 grid((unsigned)(p.rows >= 128 && (!a.part || p.tiles >= p.shares) ? std::max<int64_t>(p.tiles, p.shares) : p.shares));
     if (p.rows == 16 && p.single) hipLaunchKernelGGL((paged_rows_kernel<T, D, EIGHT, 1, 4, true>), grid, dim3(256), 0, st, a);
     else if (p.rows == 16) hipLaunchKernelGGL((paged_rows_kernel<T, D, EIGHT, 1, 4, false>), grid, dim3(256), 0, st, a);
     else if (p.rows == 32 && p.single) hipLaunchKernelGGL((paged_rows_kernel<T, D, EIGHT, 2, 4, true>), grid, dim3(256), 0, st, a);
     else if (p.rows == 32) hipLaunchKernelGGL((paged_rows_kernel<T, D, EIGHT, 2, 4, false>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((paged_tile_kernel<T, D, EIGHT>), grid, dim3(256), 0, st, a);
+    else if (p.rows == 128) hipLaunchKernelGGL((paged_tile_kernel<T, D, EIGHT, 4>), grid, dim3(256), 0, st, a);
+    else if constexpr (D == 128 && !EIGHT) hipLaunchKernelGGL((paged_tile_kernel<T, D, EIGHT, 8>), grid, dim3(512), 0, st, a);
     return check_launch("paged_attention");
 }
 
