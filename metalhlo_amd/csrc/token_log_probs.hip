@@ -3,10 +3,11 @@
 //   m = max x, l = sum exp(x - m):  log p = (x - m) - log l,  entropy = log l - sum exp(x - m) (x - m) / l
 //
 // One pass over the logits.  A lane keeps a reference instead of the maximum, which moves when a piece of sixteen bytes exceeds it by more than 8 (powers of two up to 2^8 are as exact
-// as those below one), its sum, the sum of the products, and its own greatest value with the piece that holds it.  Bound by memory and, in 16 bits, as much by the exponentials: six instructions and
-// a quarter-rate one a value.
+// as those below one), its sum, the sum of the products, and its own greatest value with the piece that holds it.  Bound by memory in 32 bits; in 16 bits as much by the instructions, seven and a
+// quarter-rate exponential a value: 4096 rows of 50257 bf16 (412 MB) take 75 us, 5.5 TB/s, without alternatives and 100 us with 20.  Few rows are bound by latency: three take 11 us, 300 of 32003
+// f32 (38 MB) 10 us without and 13 us with five alternatives.
 //
-// The alternatives need no second pass over the row: the `top`-th greatest of the maxima of 64 groups of eight lanes is a bound that `top` values reach, so only lanes whose own maximum reaches it look
+// The alternatives need no second pass over the row: the `top`-th greatest of the maxima of 64 groups of four lanes (eight of a larger workgroup) is a bound that `top` values reach, so only lanes whose own maximum reaches it look
 // at their pieces again; of 50257 random values some thirty to fifty are found for 20 and sorted in one wave.  Values are ordered by (value, lower index first) all
 // the way, a piece's index standing for its values', so that the bound is one among equals too.  Where a row is built so that more than kMost values reach the bound, the row is read once for each alternative.
 //
@@ -19,7 +20,7 @@
 namespace mhip {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / 64, kGroup = kThreads / 64, kMost = 2048, kMaxTop = 64, kMaxParts = 64;
+constexpr int kMost = 2048, kMaxTop = 64, kMaxParts = 64;
 constexpr float kLn2 = 0.69314718055994531f, kLog2eT = 1.4426950408889634f;
 
 struct LogProbArgs {
@@ -109,9 +110,9 @@ __device__ __forceinline__ Sums joined(Sums s) {
     return {m, wave_sum(s.l * f), wave_sum(f * (s.t + s.l * d))};
 }
 
-template <typename T>
+template <typename T, int kThreads>
 __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a) {
-    constexpr int EPV = 16 / sizeof(T);
+    constexpr int EPV = 16 / sizeof(T), kWaves = kThreads / 64, kGroup = kThreads / 64;
     __shared__ uint64_t found[kMost];
     __shared__ Sums wave_sums[kWaves];
     __shared__ uint64_t groups[64], bound, best[kWaves];
@@ -388,7 +389,8 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
     }
 }
 
-// How a row is dealt: parts of at least 4096 values (a piece for every thread), as many as fill the device twice.
+// How a row is dealt: parts of at least 4096 values (two to four pieces a thread), as many as fill the device twice.  (us, twice | four | eight times: 64 rows of 128000 with 20 alternatives 13 | 16 | 30,
+// 300 of 32003 f32 with five 15.1 | 15.3 | 18.8, 1000 of 50257 27 | 27 | 35.)
 int parts_of(int64_t rows, int64_t vocab) {
     const int64_t want = 2 * (int64_t)compute_units() / (rows ? rows : 1), most = vocab / 4096;
     const int64_t n = want < most ? want : most;
@@ -429,10 +431,13 @@ extern "C" int mhip_token_log_probs(void* stream, const void* logits, const void
     const int64_t per = 16 / size_of(dtype), pieces = (vocab + per - 1) / per + 1;
     a.pieces = (pieces + a.parts - 1) / a.parts;
     if (rows * a.parts > INT32_MAX) return fail(MHIP_ERR_UNSUPPORTED, "token_log_probs: more rows than a launch has workgroups");
-    const dim3 grid((unsigned)(rows * a.parts));
     hipStream_t st = as_stream(stream);
-    if (dtype == MHIP_BF16) hipLaunchKernelGGL(token_log_probs_kernel<bf16_t>, grid, dim3(kThreads), 0, st, a);
-    else if (dtype == MHIP_F16) hipLaunchKernelGGL(token_log_probs_kernel<f16_t>, grid, dim3(kThreads), 0, st, a);
-    else hipLaunchKernelGGL(token_log_probs_kernel<float>, grid, dim3(kThreads), 0, st, a);
+    // rows that neither are dealt nor fill the device have workgroups of eight waves.  us, four waves | eight: 300 rows of 32003 f32 with five alternatives 15.1 | 13.1, 400 of 50257 bf16 with 20 17.9 | 15.5;
+    // but 64 of 128000 13.1 | 14.2, 1000 of 32000 with 20 18.3 | 19.7, 1500 of 32003 18.6 | 20.1
+    const bool wide = a.parts == 1 && rows <= 2 * (int64_t)compute_units() && vocab >= 4096;
+    auto go = [&](auto kernel, auto wider) { hipLaunchKernelGGL(wide ? wider : kernel, dim3((unsigned)(rows * a.parts)), dim3(wide ? 512 : 256), 0, st, a); };
+    if (dtype == MHIP_BF16) go(token_log_probs_kernel<bf16_t, 256>, token_log_probs_kernel<bf16_t, 512>);
+    else if (dtype == MHIP_F16) go(token_log_probs_kernel<f16_t, 256>, token_log_probs_kernel<f16_t, 512>);
+    else go(token_log_probs_kernel<float, 256>, token_log_probs_kernel<float, 512>);
     return check_launch("token_log_probs");
 }

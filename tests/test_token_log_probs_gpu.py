@@ -12,7 +12,7 @@ STEP = 2.0 ** -24
 
 
 def _check(x, tokens, top, what=""):
-    """x [rows, vocab] on the device.  A lane adds n / 512 weights one after the other and the tree another few dozen, at 2 ** -24 each; a weight of exponent d is off by
+    """x [rows, vocab] on the device.  A lane of a workgroup of 256 adds n / 256 weights one after the other and the tree another few dozen, at 2 ** -24 each; a weight of exponent d is off by
     (4 + 2 |d|) 2 ** -24; the reference lies up to 8 below the maximum."""
     from metalhlo_amd import kernels
     got = kernels.token_log_probs(x, tokens, top=top)
@@ -31,7 +31,7 @@ def _check(x, tokens, top, what=""):
         entropy[np.isnan(total[:, 0])] = np.nan
         far = np.where(e > 0, np.abs(d), 0.0) + 8
         mean = (p * far).sum(1)
-        count = n / 512 + 64
+        count = n / 256 + 64
         entropy_off = STEP * (count * (1 + mean) + (p * (4 + 2 * far) * (far + mean[:, None])).sum(1)) + 1e-7
         off = STEP * (count + 8 * np.abs(m) + 8 * np.abs(np.where(np.isfinite(log_p), log_p, 0.0)) + 8 * np.where(np.isfinite(d64), np.abs(d64), 0.0))
     inside = (t >= 0) & (t < n)
