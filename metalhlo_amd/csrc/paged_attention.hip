@@ -2,12 +2,15 @@
 //
 //   rows   of a sequence and a key/value head: its tokens times the G = H / KV query heads that share the head, row = token * G + query head, so that K and V are read
 //          once for all of them.  A token's position is keys(b) - tokens(b) + i; with the causal rule it sees the keys up to its own.
-//   parts  The keys of a tile of rows are dealt over parts of one length for the whole launch, chosen on the device from all sequences' lengths such that the
-//          parts fill it: the lengths are not known on the host, and a batch may hold one long sequence among short ones.  A part leaves its
-//          reference maximum, its sum and its unnormalised rows in the workspace, and the last one to arrive puts them together (arrive.h).
+//   line   All the work of a launch in one line, sequence by sequence, head by head and tile by tile, each as long as its keys: workgroup w takes the w-th of equal shares.  The lengths are not known
+//          on the host, and a batch may hold one long sequence among short ones: the line is measured on the device, by every workgroup for itself.  (Parts of one length for the whole launch
+//          instead: 64 sequences of 100 to 8000 keys 117 us | 96.)  A part of a tile leaves its reference maximum, its sum and its unnormalised rows in the workspace, and the last one
+//          to arrive puts them together in order (arrive.h): results do not depend on who that is.  Without a workspace a workgroup takes whole tiles.
 //
 // Two kernels.  Up to 32 rows a sequence on average (decode steps): paged_rows_kernel, whose waves have keys of their own and load them straight into matrix operands;
-// its time is that of reading K and V.  More rows: paged_tile_kernel, 128 rows whose four waves share K and V in LDS, in the queries' type; its time is the matrix products'.
+// its time is that of reading K and V: 64 sequences of 4096 keys, 8 heads of 128 in 8 bits (537 MB), 88 us, 6.1 TB/s; of 100 to 8000 keys (477 MB) 88 us; one token over 200 keys 8 us, which is latency.
+// More rows: paged_tile_kernel, 128 rows whose four waves share K and V in LDS, in the queries' type; its time is the matrix products' and the exponentials' between them:
+// 32 over 8 heads of 128, four pieces of 1024 tokens behind 7168 600 us, 860 TFLOP/s (16-bit pages 613).
 //
 // fp32 sums, softmax state and scores (a key's scale is applied to its score in the first kernel, while it is converted in the second); probabilities are rounded to the queries' type in front of the second product,
 // whose error of half a step each (2^-9 for bf16) is below the result's own rounding once it is averaged over keys.  Values in 8 bits become the queries' type exactly,
@@ -272,7 +275,9 @@ __device__ __forceinline__ void join(const PagedArgs& a, const Split& split, int
 //                  lane loads sixteen bytes of a key at a time, two steps' worth in 8 bits.
 //   O^T += V^T P^T operand row = d; the eight keys that a lane holds of it in a step are neighbours in the cache's block, so that one load of sixteen bytes feeds two steps (one of a 16-bit cache), and
 //                  they are those whose probabilities the lane has just computed.
-// Two blocks are in registers or on their way; K of the next but one is asked for behind this one's scores, V behind its second product.
+// Two blocks are in registers or on their way; K of the next but one is asked for behind this one's scores, V behind its second product.  The loads of K and V pass the caches, which no one else
+// would find them in (us, plain | so: 64 sequences of 4096 keys 97.8 | 88.2), and the page numbers and scales come by scalar loads, which the vector loads do not queue behind.  The kernel holds what the registers
+// do: a spill of a few words costs a launch 10 us whatever its size, since scratch memory is set up for it.
 //
 // SINGLE: no sequence has more tokens than its place among as many others suggests, one, and a tile is one token's G rows, which see the same keys; else the rows of a tile may see
 // different numbers of them.
@@ -655,10 +660,14 @@ __device__ __forceinline__ float plus_two(uint32_t w, float x) {
     else return __builtin_amdgcn_fdot2(__builtin_bit_cast(two, w), one, x, false);
 }
 
-// 128 rows, 32 a wave (256 in eight waves where keys of 128 numbers lie in 16 bits and sequences have as many rows: a thread has half the pieces to stage, so keys and values are asked for together.
-// us, 128 rows | 256: four pieces of 1024 tokens behind 7168 702 | 641, one of 512 behind 32000 361 | 345, prompts of 2048 tokens 212 | 207, 512 rows over 2000 keys 76 | 69; but heads of 96 566 | 615 and
-// 8-bit pages 297 | 299, 195 | 198: there two workgroups, one at its products while the other is at its weights, are worth more), over stages of 64 keys that lie in LDS in the queries' type, two of them: the next one is on its way in registers and is converted and put down
-// behind this one's products.
+// 128 rows, 32 a wave, over stages of 64 keys that lie in LDS in the queries' type, two of them: the next one is on its way in registers and is converted and put down behind this one's products.
+// Two workgroups a unit, so that one is at its products while the other is at its weights; a wave at its products goes first (s_setprio: 647 us | 639).  A stage of a wave takes 3080 cycles, two waves
+// at a time, with 1024 of matrix products and some 1440 of vector instructions each (the 32 exponentials 512 of them): the latter bound it.
+//
+// WAVES = 8, where keys of 128 numbers lie in 16 bits and sequences have 256 rows: a thread has half the pieces to stage, so that keys and values are asked for together.  us, 128 rows | 256: four
+// pieces of 1024 tokens behind 7168 702 | 641, one of 512 behind 32000 361 | 345, prompts of 2048 tokens 212 | 207, 512 rows over 2000 keys 76 | 69; but heads of 96 566 | 615, and 8-bit pages
+// 297 | 299 and 195 | 198.  (64 rows a wave, so that a row of K from LDS feeds two products: 609 | 848, for one workgroup a unit has nothing to do meanwhile.)
+//
 //   S^T = K Q^T     v_mfma_f32_32x32x16: operand row i of tile j is key 32 j + 16 (r / 8) + 8 h + r % 8 where register r of half h of the result is row i, so that
 //   O^T += V^T P^T  a half's eight registers of a step are the probabilities of eight neighbouring keys: sixteen bytes of a row of V^T.
 constexpr int kStage = 64;
