@@ -6,7 +6,8 @@
 //   8 bits    the page's scale is the least power of two under which its largest value is at most 448.  Where the page holds tokens already it never shrinks, and
 //             where it grows by 2^n the held values are multiplied by 2^-n and rounded, which changes none that stays above 2^-6 of the new scale.
 //
-// Bound by memory: every new value is read once and written once.  Two kernels:
+// Bound by memory: every new value is read once and written once.  9450 tokens of 32 query and 8 key heads of 128 in 8 bits (218 MB) 39 us, 5.6 TB/s; 6300 of 16 heads of 96 in 16 bits (92 MB) 19 us,
+// 4.8 TB/s; a decode step of 48 sequences 5.5 us and of one 4.8, which is latency.  Two kernels:
 //
 //   paged_append_kernel   A wave a block of sixteen tokens, a workgroup a page (a scale needs all of its tokens), with a few heads of keys, values or queries one behind the other: the cosines and sines stay in
 //                         registers from head to head, and the next head is on its way while this one's scale is found and its values are stored.  Values pass through LDS, which turns a block's rows into its columns.
@@ -67,6 +68,7 @@ __device__ __forceinline__ int scale_byte(float amax) {
 }
 
 // Rows of keys and queries are whole lines and are stored past the caches (us, plain | so: 9450 tokens of 32 and 8 heads of 128 into pages of 64 49.3 | 39.2, of 16 48.6 | 37.2, of 256 52.2 | 46.5;
+// where only a part of a row is turned, so that a store has parts of lines, 64 of 128 elements 48.6 | 43.0, 48 of 96 in 12600 tokens of 16 heads 44.8 | 36.7, in 6300 17.9 | 19.0;
 // loads so: 47.6, and 23.7 | 32.3 where two heads share a line).
 template <typename V, typename T>
 __device__ __forceinline__ void put_stream(T* p, V v) { __builtin_nontemporal_store(v, reinterpret_cast<V*>(p)); }
@@ -178,10 +180,10 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
     if (!is_v) {
         const T* x = is_q ? static_cast<const T*>(a.q) : static_cast<const T*>(a.k);
         const int64_t xs = is_q ? a.qs[0] : a.ks[0], xh = is_q ? a.qs[1] : a.ks[1];
-        // lane l of a row: pieces l and l + R / 16 of the rotated elements, which belong together, or two of those behind them
+        // lane l of a row: pieces l and l + R / 16 of the rotated elements, which belong together, or one of each half of those behind them, so that neighbours' pieces are neighbours
         const int l = lane % kLanes, r = lane / kLanes;
         const bool turned = l < a.R / 16;
-        const int d1 = turned ? 8 * l : a.R + 16 * (l - a.R / 16), d2 = turned ? d1 + a.R / 2 : d1 + 8;
+        const int d1 = turned ? 8 * l : a.R / 2 + 8 * l, d2 = d1 + (turned ? a.R : D - a.R) / 2;
         bool in[kTurns];
         f32x4 co[kTurns][2], si[kTurns][2];
         const T* rows[kTurns];
@@ -252,7 +254,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
         return;
     }
 
-    // ---- values: a lane reads a piece of a row, and writes two neighbouring d of kMine tokens, which lie side by side in the block
+    // ---- values: a lane reads a piece of a row, and writes (in 8 bits) two neighbouring d of kMine tokens, which lie side by side in the block
     const int pr = lane / kPieces, pc = lane % kPieces, pair = lane % kPairs, group = lane / kPairs;
     u32x4 raw[kReads];
     auto ask = [&](int head) __attribute__((always_inline)) {
@@ -273,47 +275,55 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
         for (int i = 0; i < kReads; i++)
             if (pr < kRead) *reinterpret_cast<u32x4*>(&turned_values[wave][i * kRead + pr][8 * pc]) = raw[i];
         if (head + 1 < head1) ask(head + 1);
+        if constexpr (!EIGHT) {
+            // in 16 bits a lane writes eight tokens of one d, its neighbour the other eight: a store of the wave is a kilobyte in one piece
+            // (us, two d of sixteen tokens a lane | so: 6300 tokens of 16 heads of 96 24.2 | 19.0, of 128 27.4 | 21.2, 8192 of 12 heads of 64 15.9 | 11.2, past the caches level)
+            typedef T eight __attribute__((ext_vector_type(8)));
+#pragma unroll
+            for (int i = 0; i < (D + 31) / 32; i++) {
+                const int d = 32 * i + lane / 2, t0 = 8 * (lane & 1), at = wave * kBlock + t0;
+                eight w;
+#pragma unroll
+                for (int t = 0; t < 8; t++) w[t] = turned_values[wave][t0 + t][d];
+                if (at + 8 <= s0 || at >= s1) continue;
+                T* out = reinterpret_cast<T*>(a.values) + ((page_head * (page / kBlock) + wave) * D + d) * kBlock + t0;
+                if (at >= s0 && at + 8 <= s1) {
+                    *reinterpret_cast<eight*>(out) = w;
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 8; t++)
+                        if (at + t >= s0 && at + t < s1) out[t] = w[t];
+                }
+            }
+            continue;
+        }
         float y[2][kMine], top = 0.f;
 #pragma unroll
         for (int t = 0; t < kMine; t++) {
             const uint32_t w = *reinterpret_cast<const uint32_t*>(&turned_values[wave][(group % kGroups) * kMine + t][2 * pair]);
             y[0][t] = Elem<T>::to_f32(__builtin_bit_cast(T, (uint16_t)w));
             y[1][t] = Elem<T>::to_f32(__builtin_bit_cast(T, (uint16_t)(w >> 16)));
-            if (EIGHT) top = finite_max(finite_max(top, y[0][t]), y[1][t]);
+            top = finite_max(finite_max(top, y[0][t]), y[1][t]);
         }
-        float inv = 1.f;
-        if (EIGHT) {
-            const Scale sc(of_page(top, head), was, s0 > 0);
-            inv = sc.inv;
-            if (sc.moves) move_values(a.values + page_head * page * D, s0, D, sc.factor, threadIdx.x, 64 * WAVES);
-            if (threadIdx.x == 0) scales_out[page_head] = (uint8_t)sc.byte;
-        }
+        const Scale sc(of_page(top, head), was, s0 > 0);
+        const float inv = sc.inv;
+        if (sc.moves) move_values(a.values + page_head * page * D, s0, D, sc.factor, threadIdx.x, 64 * WAVES);
+        if (threadIdx.x == 0) scales_out[page_head] = (uint8_t)sc.byte;
         if (!mine) continue;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const int64_t at16 = ((page_head * (page / kBlock) + wave) * D + 2 * pair + j) * kBlock + group * kMine;
             if (all) {
-                if constexpr (EIGHT) {
-                    uint32_t w[kMine / 4];
+                uint32_t w[kMine / 4];
 #pragma unroll
-                    for (int e = 0; e < kMine / 4; e++) w[e] = pack8(y[j] + 4 * e, inv);
-                    __builtin_memcpy(__builtin_assume_aligned(a.values + at16, kMine), w, kMine);
-                } else {
-                    T w[kMine];
-#pragma unroll
-                    for (int e = 0; e < kMine; e++) w[e] = Elem<T>::from_f32(y[j][e]);
-                    __builtin_memcpy(__builtin_assume_aligned(reinterpret_cast<T*>(a.values) + at16, kMine >= 8 ? 16 : 8), w, 2 * kMine);
-                }
+                for (int e = 0; e < kMine / 4; e++) w[e] = pack8(y[j] + 4 * e, inv);
+                __builtin_memcpy(__builtin_assume_aligned(a.values + at16, kMine), w, kMine);
             } else {
 #pragma unroll
                 for (int t = 0; t < kMine; t++) {
                     if (slot + t < s0 || slot + t >= s1) continue;
-                    if constexpr (EIGHT) {
-                        const float four[4] = {y[j][t], 0.f, 0.f, 0.f};
-                        a.values[at16 + t] = (char)(pack8(four, inv) & 255);
-                    } else {
-                        reinterpret_cast<T*>(a.values)[at16 + t] = Elem<T>::from_f32(y[j][t]);
-                    }
+                    const float four[4] = {y[j][t], 0.f, 0.f, 0.f};
+                    a.values[at16 + t] = (char)(pack8(four, inv) & 255);
                 }
             }
         }
@@ -338,7 +348,7 @@ __global__ __launch_bounds__(256) void append_few_kernel(AppendArgs a) {
     const int was = EIGHT && !is_q && f.slot0 ? scales[page_head] : 0;
 
     const bool turned = !is_v && l < a.R / 16;
-    const int d1 = is_v ? 16 * l : turned ? 8 * l : a.R + 16 * (l - a.R / 16), d2 = turned ? d1 + a.R / 2 : d1 + 8;
+    const int d1 = is_v ? 16 * l : turned ? 8 * l : a.R / 2 + 8 * l, d2 = d1 + (is_v ? 8 : (turned ? a.R : D - a.R) / 2);
     const T* x = is_q ? static_cast<const T*>(a.q) + head * a.qs[1] : is_v ? static_cast<const T*>(a.v) + head * a.vs[1] : static_cast<const T*>(a.k) + head * a.ks[1];
     const int64_t xs = is_q ? a.qs[0] : is_v ? a.vs[0] : a.ks[0];
     auto row_of = [&](int i, float (&y)[16]) __attribute__((always_inline)) {
