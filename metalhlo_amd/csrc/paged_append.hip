@@ -6,8 +6,8 @@
 //   8 bits    the page's scale is the least power of two under which its largest value is at most 448.  Where the page holds tokens already it never shrinks, and
 //             where it grows by 2^n the held values are multiplied by 2^-n and rounded, which changes none that stays above 2^-6 of the new scale.
 //
-// Bound by memory: every new value is read once and written once.  9450 tokens of 32 query and 8 key heads of 128 in 8 bits (218 MB) 39 us, 5.6 TB/s; 6300 of 16 heads of 96 in 16 bits (92 MB) 19 us,
-// 4.8 TB/s; a decode step of 48 sequences 5.5 us and of one 4.8, which is latency.  Two kernels:
+// Bound by memory: every new value is read once and written once.  9450 tokens of 32 query and 8 key heads of 128 in 8 bits (218 MB) 46 us, 4.7 TB/s, 32000 (737 MB)
+// 140 us, 5.3 TB/s; 6300 of 16 heads of 96 in 16 bits (92 MB) 20 us, 4.5 TB/s; a decode step of 48 sequences 5.5 us and of one 4.8, which is latency.  Two kernels:
 //
 //   paged_append_kernel   A wave a block of sixteen tokens, a workgroup a page (a scale needs all of its tokens), with a few heads of keys, values or queries one behind the other: the cosines and sines stay in
 //                         registers from head to head, and the next head is on its way while this one's scale is found and its values are stored.  Values pass through LDS, which turns a block's rows into its columns.
@@ -24,7 +24,7 @@ struct AppendArgs {
     char *keys, *values;
     uint8_t *key_scales, *value_scales;
     Sequences s;
-    int pages, KV, H, R, positions, heads_a_part;
+    int pages, KV, H, R, positions, heads_a_part, parts;
     int64_t ks[2], vs[2], qs[2], os[2];       // token and head strides in elements
 };
 
@@ -153,12 +153,13 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
     __shared__ __attribute__((aligned(16))) T turned_values[WAVES][kBlock][D];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Fill f;
-    if (!f.find(a, blockIdx.x)) return;
+    const int unit = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - unit * a.parts;
+    if (!f.find(a, unit)) return;
     const int page = 1 << a.s.page_shift, s0 = f.slot0, s1 = f.slot1;
     const bool on_page = (uint32_t)f.page_no < (uint32_t)a.pages;
 
     // heads [head0, head1) of keys, values or queries
-    const int kv_parts = (a.KV + a.heads_a_part - 1) / a.heads_a_part, part = blockIdx.y;
+    const int kv_parts = (a.KV + a.heads_a_part - 1) / a.heads_a_part;
     const bool is_v = part >= kv_parts && part < 2 * kv_parts, is_q = part >= 2 * kv_parts;
     const int head0 = (part - (is_q ? 2 * kv_parts : is_v ? kv_parts : 0)) * a.heads_a_part, head1 = min(head0 + a.heads_a_part, is_q ? a.H : a.KV);
     if (!is_q && !on_page) return;
@@ -438,11 +439,15 @@ int launch(hipStream_t st, AppendArgs a, int64_t units) {
         return check_launch("paged_append");
     }
     auto parts = [&](int heads) { return 2 * ((a.KV + heads - 1) / heads) + (a.H + heads - 1) / heads; };
-    // Heads of a workgroup: what they share (the page's place, cosines and sines) against waves to fill the device with.  us, one | two | four | eight heads: 9450 tokens as above 57.9 | 48.1 | 49.4 | 53.7 (15200,
-    // 7600 waves with two, four), 300 tokens 5.8 | 6.2 | 9.1 | 15.2, 32000 tokens 212 | 191 | 185 | 172
-    a.heads_a_part = 8;
-    while (a.heads_a_part > 1 && units * (1 << (a.s.page_shift - 4)) * parts(a.heads_a_part) < 7000) a.heads_a_part /= 2;
-    const dim3 grid((unsigned)units, (unsigned)parts(a.heads_a_part));
+    // Heads of a workgroup: what they share (the page's place, cosines and sines) against waves to fill the device with.  us, one | two | four | eight heads, buffers larger than the caches: 9450 tokens of
+    // 32 and 8 heads of 128 51.7 | 46.6 | 48.7 | 55.7 (14700, 7300 waves with two, four), 32000 162 | 140 | 140 | 142, of 32 and 32 heads 320 | 257 | 248 | 255, 6300 of 16 and 16 of 96
+    // 21.2 | 20.5 | 21.6 | 22.4 (9800, 4900 waves), 300 tokens 6.0 | 6.2 | 9.1 | 15.0
+    a.heads_a_part = 4;
+    while (a.heads_a_part > 1 && units * (1 << (a.s.page_shift - 4)) * parts(a.heads_a_part) < 8000) a.heads_a_part /= 2;
+    // All heads of a page run side by side, and a token's row is read and written in one go: page after page of one part of the heads first was 52.4 and 159 us where 9450 and 32000 take 48.7 and 142
+    a.parts = parts(a.heads_a_part);
+    if (units * a.parts >= (int64_t)1 << (26 - (a.s.page_shift - 4))) return fail(MHIP_ERR_UNSUPPORTED, "paged_append: more threads than a launch has");       // (2^32 of them)
+    const dim3 grid((unsigned)(units * a.parts));
     switch (a.s.page_shift) {
         case 4: hipLaunchKernelGGL((paged_append_kernel<T, D, EIGHT, 1>), grid, dim3(64), 0, st, a); break;
         case 5: hipLaunchKernelGGL((paged_append_kernel<T, D, EIGHT, 2>), grid, dim3(128), 0, st, a); break;
