@@ -4,11 +4,11 @@
 //          once for all of them.  A token's position is keys(b) - tokens(b) + i; with the causal rule it sees the keys up to its own.
 //   line   All the work of a launch in one line, sequence by sequence, head by head and tile by tile, each as long as its keys: workgroup w takes the w-th of equal shares.  The lengths are not known
 //          on the host, and a batch may hold one long sequence among short ones: the line is measured on the device, by every workgroup for itself.  (Parts of one length for the whole launch
-//          instead: 64 sequences of 100 to 8000 keys 117 us | 96.)  A part of a tile leaves its reference maximum, its sum and its unnormalised rows in the workspace, and the last one
+//          instead: 48 sequences of 1600 to 8000 keys 117 us | 96.)  A part of a tile leaves its reference maximum, its sum and its unnormalised rows in the workspace, and the last one
 //          to arrive puts them together in order (arrive.h): results do not depend on who that is.  Without a workspace a workgroup takes whole tiles.
 //
 // Two kernels.  Up to 32 rows a sequence on average (decode steps): paged_rows_kernel, whose waves have keys of their own and load them straight into matrix operands;
-// its time is that of reading K and V: 64 sequences of 4096 keys, 8 heads of 128 in 8 bits (537 MB), 88 us, 6.1 TB/s; of 100 to 8000 keys (477 MB) 88 us; one token over 200 keys 8 us, which is latency.
+// its time is that of reading K and V: 64 sequences of 4096 keys, 8 heads of 128 in 8 bits (537 MB), 88 us, 6.1 TB/s; 48 of 1600 to 8000 keys (477 MB) 90 us; one token over some hundred keys 8 us, which is latency.
 // More rows: paged_tile_kernel, 128 rows whose four waves share K and V in LDS, in the queries' type; its time is the matrix products' and the exponentials' between them:
 // 32 over 8 heads of 128, four pieces of 1024 tokens behind 7168 600 us, 860 TFLOP/s (16-bit pages 613).
 //
