@@ -74,18 +74,18 @@ struct Line {
     __device__ __forceinline__ int owner(int g) const { return g < more * (per + 1) ? g / (per + 1) : more + (g - more * (per + 1)) / per; }
 };
 
-// The first 64 sequences, in a wave's own LDS.
-struct Known { int start[64], tokens[64], keys[64]; };
-struct Found { int b, before, start, tokens, keys; };
+// The first 64 sequences, in a wave's own LDS.  `line`: the keys that its tiles' stretches of the line are made for.
+struct Known { int start[64], tokens[64], keys[64], line[64]; };
+struct Found { int b, before, start, tokens, keys, line; };
 __device__ __forceinline__ void known_of(const Sequences& s, Known& known, int lane) {
     known.start[lane] = lane < s.B ? s.start(lane) : 0;
     known.tokens[lane] = lane < s.B ? s.tokens(lane) : 0;
-    known.keys[lane] = lane < s.B ? s.keys(lane) : 0;
+    known.keys[lane] = known.line[lane] = lane < s.B ? s.keys(lane) : 0;
 }
 // The sequence that place g of the line lies in, when one has stretch(tokens, keys) of it; `before`: where it begins.  False behind the last.
 template <typename F>
 __device__ __forceinline__ bool found_at(const Sequences& s, const Known& known, int lane, int g, F stretch, Found& at) {
-    const int mine = stretch(known.tokens[lane], known.keys[lane]), sum = wave_scan(mine);
+    const int mine = stretch(known.tokens[lane], known.line[lane]), sum = wave_scan(mine);
     int length;
     if (const uint64_t m = __ballot(sum > g)) {
         at.b = __builtin_ctzll(m);
@@ -94,6 +94,7 @@ __device__ __forceinline__ bool found_at(const Sequences& s, const Known& known,
         at.start = __builtin_amdgcn_readfirstlane(known.start[at.b]);
         at.tokens = __builtin_amdgcn_readfirstlane(known.tokens[at.b]);
         at.keys = __builtin_amdgcn_readfirstlane(known.keys[at.b]);
+        at.line = __builtin_amdgcn_readfirstlane(known.line[at.b]);
     } else {
         at.before = __builtin_amdgcn_readlane(sum, 63);
         int further;
@@ -102,7 +103,7 @@ __device__ __forceinline__ bool found_at(const Sequences& s, const Known& known,
         at.before += further;
         at.start = __builtin_amdgcn_readfirstlane(s.start(at.b));
         at.tokens = __builtin_amdgcn_readfirstlane(s.tokens(at.b));
-        at.keys = __builtin_amdgcn_readfirstlane(s.keys(at.b));
+        at.keys = at.line = __builtin_amdgcn_readfirstlane(s.keys(at.b));
         length = stretch(at.tokens, at.keys);
     }
     return g >= at.before && g - at.before < length;                       // (starts that are no starts: their sums may have wrapped)
@@ -317,9 +318,25 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
     };
     count(known[wave].tokens[lane], known[wave].keys[lane]);
     for (int b = 64 + lane; b < a.s.B; b += 64) count(a.s.tokens(b), a.s.keys(b));
-    longest = (int)wave_max((float)longest);                                  // of one sequence (exact: at most 2^16)
+    longest = __builtin_amdgcn_readfirstlane((int)wave_max((float)longest));      // of one sequence (exact: at most 2^16)
     steps = __builtin_amdgcn_readlane(wave_scan(steps), 63) * a.KV;           // of all heads
-    const Line line(a.by_shares, a.shares, steps, longest);
+    Line line(a.by_shares, a.shares, steps, longest);
+    // Shares of a few steps: a share that is the end of one tile and the beginning of another costs two rounds of first loads and of joining.  Where stretches that are rounded up to l steps fit as many
+    // shares of l, every workgroup has one part of one tile.  us, plain | rounded: 16 sequences of 2800 to 4000 keys (8 heads of 128, 8 bits) 32.4 | 27.9, 64 of them 85.4 | 79.0, with four tokens each 97 | 81,
+    // 24 of 600 to 6000 42.3 | 37.0, 64 of 300 to 600 25.6 | 19.2, one of 30000 22.0 | 19.8; but 30 of 450 to 900, 12 heads of 64, 18.5 | 19.4.  More than 16 steps a share: level
+    if (line.per <= 16 && (line.per > 1 || line.more) && a.s.B <= 64) {
+        const int n = steps_of(known[wave].keys[lane]), tiles = tiles_of(known[wave].tokens[lane]);
+        for (int l = line.per + (line.more ? 1 : 0), l1 = line.per + line.per / 4 + 1; l <= l1; l++) {
+            const int of = (int)(((float)n + (float)l - 0.5f) / (float)l);       // n / l, rounded up (n and l below 2^16, l of a few)
+            const int shares = __builtin_amdgcn_readlane(wave_scan(tiles * of), 63) * a.KV;
+            if (shares > a.shares) continue;
+            known[wave].line[lane] = of * l << a.unit_shift;
+            line.per = l;
+            line.more = 0;
+            steps = shares * l;
+            break;
+        }
+    }
     int g = line.begin(blockIdx.x);
     const int stop = min(line.begin(blockIdx.x + 1), steps);
     const int page_bytes = (D * SIZE) << a.s.page_shift;
@@ -329,7 +346,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
         Found at;
         if (!found_at(a.s, known[wave], lane, g, [&](int tokens, int keys) { return tiles_of(tokens) * a.KV * steps_of(keys); }, at)) return;
         const int b = at.b, tokens = at.tokens, keys = at.keys, first = at.start;
-        const int mine = steps_of(keys), pair = (g - at.before) / mine, s0 = g - at.before - pair * mine;
+        const int mine = steps_of(at.line), pair = (g - at.before) / mine, s0 = g - at.before - pair * mine;
         if (!a.part && s0) {                                                  // without a workspace a head is its beginning's, whole
             g += mine - s0;
             continue;
