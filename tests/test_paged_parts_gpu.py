@@ -199,6 +199,63 @@ def test_log_probs_without_a_workspace(rows, vocab, dtype):
         assert ((a - b).abs() <= 2.0 ** -24 * (vocab / 128 + 64) * (2 + b.abs())).all()
 
 
+@gpu
+@EIGHT
+@pytest.mark.parametrize("new", [[1, 1, 1], [9, 2, 4], [200, 1, 150]], ids=str)
+def test_pages_far_into_a_cache(new, eight):
+    """Bytes beyond 2^32 of a cache, and rows of queries as far apart: the same bits as in a small cache."""
+    from metalhlo_amd import kernels
+    KV, page, D, pages = 8, 64, 128, 70000
+    keys = [n + c for n, c in zip(new, (100, 3, 1500))]
+    T, starts = sum(new), ints([0] + list(np.cumsum(new)))
+    g = torch.Generator("cuda").manual_seed(3)
+    k, v = (torch.randn(T, KV, D, device="cuda", generator=g).bfloat16() for _ in range(2))
+    far_q = torch.empty_strided((T, 2 * KV, D), (2 ** 31 // T // 64 * 64 + 64, D, 1), dtype=torch.bfloat16, device="cuda")
+    q = torch.randn(T, 2 * KV, D, device="cuda", generator=g).bfloat16()
+    far_q.copy_(q)
+    freqs = torch.randn(2000, D, device="cuda", generator=g)
+    count = [-(-n // page) for n in keys]
+    table = -np.ones((3, max(count)), dtype=np.int32)
+    for b, c in enumerate(count):
+        table[b, :c] = sum(count[:b]) + np.arange(c)
+    results = []
+    for size, first in ((sum(count), 0), (pages, pages - sum(count))):
+        cache = kernels.paged_cache(size, KV, page, D, torch.float8_e4m3fn if eight else torch.bfloat16)
+        held = [t[first:] for t in cache if t is not None]
+        for t in held:
+            t.view(torch.uint8).fill_(40)
+        t = ints(np.where(table < 0, table, table + first))
+        turned = kernels.paged_append(cache, k, v, t, ints(keys), starts, q=far_q if first else q, freqs=freqs, out=far_q if first else None)
+        o = kernels.paged_attention(turned, cache, t, ints(keys), starts)
+        results.append([turned.contiguous(), o] + [h.view(torch.uint8).clone() for h in held])
+        del cache, held
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and bool(results[0][1].isfinite().all())
+
+
+@gpu
+@pytest.mark.parametrize("T", [3, 40, 300])
+def test_a_table_without_columns(T):
+    """No sequence can have keys: zeros, and nothing is stored."""
+    from metalhlo_amd import kernels
+    cache = kernels.paged_cache(4, 2, 16, 64, torch.bfloat16)
+    cache.keys.fill_(3)
+    q, k = torch.ones(T, 4, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(T, 2, 64, dtype=torch.bfloat16, device="cuda")
+    table = torch.empty(3, 0, dtype=torch.int32, device="cuda")
+    args = (table, ints([5, 0, T]), ints([0, 1, 1, T]))
+    kernels.paged_append(cache, k, k, *args)
+    assert (cache.keys == 3).all()
+    for causal in (True, False):
+        assert (kernels.paged_attention(q, cache, *args, is_causal=causal) == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("rows,vocab,dtype,top", [(300, 32003, torch.float32, 5), (400, 9001, torch.bfloat16, 64), (512, 4096, torch.float16, 1), (7, 300001, torch.float32, 20)],
+                         ids=lambda v: str(NAME.get(v, v)))
+def test_log_probs_of_some_hundred_rows(rows, vocab, dtype, top):
+    from tests.test_token_log_probs_gpu import _check, _logits
+    _check(*_logits(rows, vocab, dtype, rows), top, str((rows, vocab, top)))
+
+
 @pytest.mark.parametrize("name", ["paged_rows_kernel", "paged_tile_kernel", "paged_append_kernel", "append_few_kernel", "token_log_probs_kernel"])
 def test_nothing_is_kept_in_scratch(name):
     """Scratch memory costs a launch of these 10 us, whatever its size."""
