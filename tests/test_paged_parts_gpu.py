@@ -204,6 +204,13 @@ def test_log_probs_without_a_workspace(rows, vocab, dtype):
 @pytest.mark.parametrize("new", [[1, 1, 1], [9, 2, 4], [200, 1, 150]], ids=str)
 def test_pages_far_into_a_cache(new, eight):
     """Bytes beyond 2^32 of a cache, and rows of queries as far apart: the same bits as in a small cache."""
+    try:
+        _far(new, eight)
+    finally:
+        torch.cuda.empty_cache()                # (gigabytes, which a later test's small tensor would keep from going back)
+
+
+def _far(new, eight):
     from metalhlo_amd import kernels
     KV, page, D, pages = 8, 64, 128, 70000
     keys = [n + c for n, c in zip(new, (100, 3, 1500))]
