@@ -678,8 +678,9 @@ __device__ __forceinline__ float plus_two(uint32_t w, float x) {
 }
 
 // 128 rows, 32 a wave, over stages of 64 keys that lie in LDS in the queries' type, two of them: the next one is on its way in registers and is converted and put down behind this one's products.
-// Two workgroups a unit, so that one is at its products while the other is at its weights; a wave at its products goes first (s_setprio: 647 us | 639).  A stage of a wave takes 3080 cycles, two waves
-// at a time, with 1024 of matrix products and some 1440 of vector instructions each (the 32 exponentials 512 of them): the latter bound it.
+// Two workgroups a unit, so that one is at its products while the other is at its weights; a wave at its products goes first (s_setprio: 647 us | 639).  A stage of all eight waves of a unit takes
+// some 3000 cycles, of which the matrix units are busy 2048 (1024 a wave, two waves each), LDS 2560 (32 KB of operands a wave, and two stages that are put down) and the vector units some 2600 (the
+// exponentials 1024 of them): three pipes that are full to 70 and 85 in a hundred, none of which leaves room for much.
 //
 // WAVES = 8, where keys of 128 numbers lie in 16 bits and sequences have 256 rows: a thread has half the pieces to stage, so that keys and values are asked for together.  us, 128 rows | 256: four
 // pieces of 1024 tokens behind 7168 702 | 641, one of 512 behind 32000 361 | 345, prompts of 2048 tokens 212 | 207, 512 rows over 2000 keys 76 | 69; but heads of 96 566 | 615, and 8-bit pages
