@@ -4,11 +4,11 @@
 //
 // One pass over the logits.  A lane keeps a reference instead of the maximum, which moves when a piece of sixteen bytes exceeds it by more than 8 (powers of two up to 2^8 are as exact
 // as those below one), its sum, the sum of the products, and its own greatest value with the piece that holds it.  Bound by memory in 32 bits; in 16 bits as much by the instructions, seven and a
-// quarter-rate exponential a value: 4096 rows of 50257 bf16 (412 MB) take 75 us, 5.5 TB/s, without alternatives and 100 us with 20.  Few rows are bound by latency: three take 11 us, 300 of 32003
+// quarter-rate exponential a value: 4096 rows of 50257 bf16 (412 MB) take 75 us, 5.5 TB/s, without alternatives and 90 us with 20.  Few rows are bound by latency: three take 11 us, 300 of 32003
 // f32 (38 MB) 10 us without and 13 us with five alternatives.
 //
-// The alternatives need no second pass over the row: the `top`-th greatest of the maxima of 64 groups of four lanes (eight of a larger workgroup) is a bound that `top` values reach, so only lanes whose own maximum reaches it look
-// at their pieces again; of 50257 random values some thirty to fifty are found for 20 and sorted in one wave.  Values are ordered by (value, lower index first) all
+// The alternatives need no second pass over the row: the `top`-th greatest of the maxima of 64 groups of four lanes (eight of a larger workgroup) is a bound that `top` values reach, so only the pieces of lanes (or classes of
+// a lane's pieces) whose own maximum reaches it are looked at again; of 50257 random values some thirty to fifty are found for 20 and sorted in one wave.  Values are ordered by (value, lower index first) all
 // the way, a piece's index standing for its values', so that the bound is one among equals too.  Where a row is built so that more than kMost values reach the bound, the row is read once for each alternative.
 //
 // Few rows are dealt over several workgroups each, and the last one to arrive puts the parts together (arrive.h).
@@ -20,7 +20,7 @@
 namespace mhip {
 namespace {
 
-constexpr int kMost = 2048, kMaxTop = 64, kMaxParts = 64;
+constexpr int kMost = 1536, kMaxTop = 64, kMaxParts = 64;
 constexpr float kLn2 = 0.69314718055994531f, kLog2eT = 1.4426950408889634f;
 
 struct LogProbArgs {
@@ -110,13 +110,16 @@ __device__ __forceinline__ Sums joined(Sums s) {
     return {m, wave_sum(s.l * f), wave_sum(f * (s.t + s.l * d))};
 }
 
-template <typename T, int kThreads>
+// kClasses: a lane's pieces fall into so many classes, in turn, each with a greatest value of its own.
+template <typename T, int kThreads, int kClasses>
 __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a) {
     constexpr int EPV = 16 / sizeof(T), kWaves = kThreads / 64, kGroup = kThreads / 64;
+    constexpr int kAhead = 4;                                             // pieces that are asked for together
+    static_assert(kAhead % kClasses == 0, "a piece's class is its place among those");
     __shared__ uint64_t found[kMost];
     __shared__ Sums wave_sums[kWaves];
     __shared__ uint64_t groups[64], bound, best[kWaves];
-    __shared__ uint16_t holders[kThreads];
+    __shared__ uint16_t holders[kClasses * kThreads];
     __shared__ int count, holding, last;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int part = blockIdx.x % a.parts;
@@ -148,10 +151,15 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
     // ---- the sums, and each lane's greatest value.  Weights are 2^(x log2(e) - c) with c = ref log2(e) rounded: 2^slip times what they are to be, `slip` being what the
     // rounding took (2^-8 at most).  Where a lane of the wave has a reference beyond 2^16 it is subtracted before the multiplication
     Sums s{-INFINITY, 0.f, 0.f};
-    float c = 0.f, slip = 0.f, most = -INFINITY;
-    int where = -1;
+    float c = 0.f, slip = 0.f, most[kClasses];
+    int where[kClasses];
+#pragma unroll
+    for (int i = 0; i < kClasses; i++) {
+        most[i] = -INFINITY;
+        where[i] = -1;
+    }
     bool far = false;
-    auto take = [&](const float (&v)[EPV], int p) __attribute__((always_inline)) {
+    auto take = [&](const float (&v)[EPV], int p, float& most, int& where) __attribute__((always_inline)) {
         float m = fmaxf(v[0], v[1]);
 #pragma unroll
         for (int e = 2; e < EPV; e += 2) m = fmaxf(fmaxf(m, v[e]), v[e + 1]);
@@ -190,16 +198,16 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
     if (head && threadIdx.x == kThreads - 1) {
         float v[EPV];
         broken(0, v);
-        where = 0;
-        take(v, 0);
+        where[0] = 0;
+        take(v, 0, most[0], where[0]);
     }
-    constexpr int kAhead = 4;                                             // pieces that are asked for together
     auto widened = [&](const u32x4& w, float (&v)[EPV]) __attribute__((always_inline)) {
         const Vec16<T> t = __builtin_bit_cast(Vec16<T>, w);
 #pragma unroll
         for (int e = 0; e < EPV; e++) v[e] = Elem<T>::to_f32(t.v[e]);
     };
-    where = whole0 + (int)threadIdx.x < whole1 && where < 0 ? whole0 + threadIdx.x : where;
+#pragma unroll
+    for (int i = 0; i < kClasses; i++) where[i] = whole0 + i * kThreads + (int)threadIdx.x < whole1 && where[i] < 0 ? whole0 + i * kThreads + threadIdx.x : where[i];
     int p = whole0;                                                       // (the same in all lanes: an address is a scalar and a lane's own offset)
     u32x4 w[kAhead];
     for (; p <= whole1 - kAhead * kThreads; p += kAhead * kThreads) {
@@ -209,7 +217,7 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
         for (int i = 0; i < kAhead; i++) {
             float v[EPV];
             widened(w[i], v);
-            take(v, p + i * kThreads + threadIdx.x);
+            take(v, p + i * kThreads + threadIdx.x, most[i % kClasses], where[i % kClasses]);
         }
     }
     if (p < whole1) {
@@ -220,7 +228,7 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
             if (p + i * kThreads + (int)threadIdx.x < whole1) {
                 float v[EPV];
                 widened(w[i], v);
-                take(v, p + i * kThreads + threadIdx.x);
+                take(v, p + i * kThreads + threadIdx.x, most[i % kClasses], where[i % kClasses]);
             }
         };
         static_assert(kAhead == 4, "a call each");
@@ -232,8 +240,8 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
     if (tail && threadIdx.x == 0) {
         float v[EPV];
         broken(p1 - 1, v);
-        if (where < 0) where = p1 - 1;
-        take(v, p1 - 1);
+        if (where[0] < 0) where[0] = p1 - 1;
+        take(v, p1 - 1, most[0], where[0]);
     }
     const float unslipped = __builtin_amdgcn_exp2f(-slip);
     s.t = unslipped * (s.t - slip * s.l);
@@ -257,16 +265,24 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
             }
         };
         if (not_a_number) {                                               // (or an infinity: its sums are no numbers either)
-            auto look = [&](int q) __attribute__((always_inline)) {
+            auto look = [&](int q, float& most, int& where) __attribute__((always_inline)) {
                 each_of(q, [&](float v, uint32_t) __attribute__((always_inline)) {
                     if (v != v && most == most) { most = v; where = q; }
                 });
             };
-            if (head && threadIdx.x == kThreads - 1) look(0);
-            for (int q = whole0 + threadIdx.x; q < whole1; q += kThreads) look(q);
-            if (tail && threadIdx.x == 0) look(p1 - 1);
+            if (head && threadIdx.x == kThreads - 1) look(0, most[0], where[0]);
+            for (int q = whole0 + threadIdx.x; q < whole1; q += kClasses * kThreads)
+#pragma unroll
+                for (int i = 0; i < kClasses; i++)
+                    if (q + i * kThreads < whole1) look(q + i * kThreads, most[i], where[i]);
+            if (tail && threadIdx.x == 0) look(p1 - 1, most[0], where[0]);
         }
-        const uint64_t key = where >= 0 ? key_of(most, (uint32_t)where) : 0;
+        uint64_t keys[kClasses], key = 0;
+#pragma unroll
+        for (int i = 0; i < kClasses; i++) {
+            keys[i] = where[i] >= 0 ? key_of(most[i], (uint32_t)where[i]) : 0;
+            key = keys[i] > key ? keys[i] : key;
+        }
         uint64_t group = greater<2>(greater<1>(key));
         if (kGroup == 8) group = greater<4>(group);
         if (lane % kGroup == 0) groups[threadIdx.x / kGroup] = group;
@@ -278,10 +294,14 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
         }
         __syncthreads();
         const uint64_t limit = bound;
-        if (key >= limit && where >= 0) holders[atomicAdd(&holding, 1)] = (uint16_t)threadIdx.x;
+        if (key >= limit) {
+#pragma unroll
+            for (int i = 0; i < kClasses; i++)
+                if (keys[i] >= limit && where[i] >= 0) holders[atomicAdd(&holding, 1)] = (uint16_t)(i * kThreads + threadIdx.x);
+        }
         __syncthreads();
-        // every piece of the lanes whose own maximum reaches the bound, dealt over the workgroup (2^shift items a lane), and the two that are broken
-        const int turns = (whole1 - whole0 + kThreads - 1) / kThreads, shift = turns > 1 ? 32 - __builtin_clz(turns - 1) : 0, items = turns > 0 ? holding << shift : 0;
+        // every piece of those classes of lanes whose own maximum reaches the bound, dealt over the workgroup (2^shift items a class), and the two that are broken
+        const int turns = (whole1 - whole0 + kClasses * kThreads - 1) / (kClasses * kThreads), shift = turns > 1 ? 32 - __builtin_clz(turns - 1) : 0, items = turns > 0 ? holding << shift : 0;
         const float least = value_of((uint32_t)(limit >> 32));
         auto keep = [&](float v, int q, uint32_t i) __attribute__((always_inline)) {
             if (v < least || key_of(v, (uint32_t)q) < limit) return;
@@ -294,7 +314,7 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int i = min(i0 + j * kThreads + (int)threadIdx.x, items - 1);
-                q[j] = whole0 + holders[i >> shift] + (i & ((1 << shift) - 1)) * kThreads;
+                q[j] = whole0 + holders[i >> shift] + (i & ((1 << shift) - 1)) * (kClasses * kThreads);
                 w[j] = base[min(q[j], whole1 - 1)];
             }
 #pragma unroll
@@ -434,10 +454,12 @@ extern "C" int mhip_token_log_probs(void* stream, const void* logits, const void
     hipStream_t st = as_stream(stream);
     // rows that neither are dealt nor fill the device have workgroups of eight waves.  us, four waves | eight: 300 rows of 32003 f32 with five alternatives 15.1 | 13.1, 400 of 50257 bf16 with 20 17.9 | 15.5;
     // but 64 of 128000 13.1 | 14.2, 1000 of 32000 with 20 18.3 | 19.7, 1500 of 32003 18.6 | 20.1
-    const bool wide = a.parts == 1 && rows <= 2 * (int64_t)compute_units() && vocab >= 4096;
-    auto go = [&](auto kernel, auto wider) { hipLaunchKernelGGL(wide ? wider : kernel, dim3((unsigned)(rows * a.parts)), dim3(wide ? 512 : 256), 0, st, a); };
-    if (dtype == MHIP_BF16) go(token_log_probs_kernel<bf16_t, 256>, token_log_probs_kernel<bf16_t, 512>);
-    else if (dtype == MHIP_F16) go(token_log_probs_kernel<f16_t, 256>, token_log_probs_kernel<f16_t, 512>);
-    else go(token_log_probs_kernel<float, 256>, token_log_probs_kernel<float, 512>);
+    // Of the others, 16-bit rows that fill the device several times have four classes: a class that reaches the bound is a quarter of the pieces to look at again, each a line from memory, and the others'
+    // launch is shorter by what four maxima take: 4096 rows of 50257 with 20 alternatives 100.2 | 89.6, 700 21.7 | 20.2; but 3 10.8 | 11.1, 2000 of 32003 f32 with five 55.4 | 56.5
+    const bool wide = a.parts == 1 && rows <= 2 * (int64_t)compute_units() && vocab >= 4096, many = a.parts == 1 && !wide;
+    auto go = [&](auto few, auto wider, auto more) { hipLaunchKernelGGL(wide ? wider : many ? more : few, dim3((unsigned)(rows * a.parts)), dim3(wide ? 512 : 256), 0, st, a); };
+    if (dtype == MHIP_BF16) go(token_log_probs_kernel<bf16_t, 256, 1>, token_log_probs_kernel<bf16_t, 512, 1>, token_log_probs_kernel<bf16_t, 256, 4>);
+    else if (dtype == MHIP_F16) go(token_log_probs_kernel<f16_t, 256, 1>, token_log_probs_kernel<f16_t, 512, 1>, token_log_probs_kernel<f16_t, 256, 4>);
+    else go(token_log_probs_kernel<float, 256, 1>, token_log_probs_kernel<float, 512, 1>, token_log_probs_kernel<float, 256, 1>);
     return check_launch("token_log_probs");
 }
