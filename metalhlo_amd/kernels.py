@@ -206,7 +206,7 @@ def paged_cache(pages: int, heads: int, page_size: int, head_size: int, dtype, d
 def paged_append(cache: PagedCache, k, v, table, lengths, starts, q=None, freqs=None, out=None):
     """Stores k and v [tokens, heads, D] (views with a contiguous last axis) of each sequence's new tokens in the cache.  With `freqs` [positions, R] in fp32 (R / 2
     cosines, then sines; R a multiple of 16) the first R elements of k, and of q [tokens, query heads, D], are turned on the way as `rope` turns them; returns the
-    turned q (`out`, which may be q, or a new tensor).  A token whose position lies outside of freqs is passed over.  8 bits: a page's scale is the least
+    turned q (`out`, which may be q and overlaps nothing else of the call, or a new tensor).  A token whose position lies outside of freqs is passed over.  8 bits: a page's scale is the least
     that its largest value needs and only grows while the page holds older tokens, whose values are then rounded anew; what is not finite becomes NaN."""
     return (_native or _host()).paged_append(cache, k, v, table, lengths, starts, q, freqs, out)
 
@@ -215,7 +215,8 @@ def paged_attention(q, cache: PagedCache, table, lengths, starts, scale: Optiona
                     out: Optional[torch.Tensor] = None):
     """softmax(scale * q k^T, causal) v over each sequence's keys in the cache: q [tokens, query heads, D], query heads a multiple of the cache's heads.  Causal: a
     token sees the keys up to its own position.  A token without keys yields zeros.  Default scale 1/sqrt(D).  Values of an
-    8-bit cache become q's type on the way, so that float16 holds them up to 65504.  The last bits of a row may depend on the
+    8-bit cache become q's type on the way, so that float16 holds them up to 65504.
+    `out` may be q, and overlaps nothing else of the call.  The last bits of a row may depend on the
     lengths of the other sequences, as mhip.h says."""
     return (_native or _host()).paged_attention(q, cache, table, lengths, starts, scale, is_causal, out)
 
