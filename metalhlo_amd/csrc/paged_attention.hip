@@ -324,9 +324,12 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
     // Shares of a few steps: a share that is the end of one tile and the beginning of another costs two rounds of first loads and of joining.  Where stretches that are rounded up to l steps fit as many
     // shares of l, every workgroup has one part of one tile.  us, plain | rounded: 16 sequences of 2800 to 4000 keys (8 heads of 128, 8 bits) 32.4 | 27.9, 64 of them 85.4 | 79.0, with four tokens each 97 | 81,
     // 24 of 600 to 6000 42.3 | 37.0, 64 of 300 to 600 25.6 | 19.2, one of 30000 22.0 | 19.8; but 30 of 450 to 900, 12 heads of 64, 18.5 | 19.4.  More than 16 steps a share: level
-    if (line.per <= 16 && (line.per > 1 || line.more) && a.s.B <= 64) {
+    // Where there is a share for every step, shares of two make half as many parts to join; four to eight steps are quicker in as many parts.  us, one | two: 4 sequences of 4000 keys 16.0 | 12.4, with
+    // four tokens each 20.0 | 14.4, one of 8000 11.8 | 11.6, 8 of 250 to 500, 2 heads of 96, 8.0 | 7.1; but one of 1000, 12 heads of 64, 7.8 | 8.3
+    const bool ample = line.per == 1 && !line.more;
+    if (line.per <= 16 && !(ample && longest > 2 && longest <= 8) && a.s.B <= 64) {
         const int n = steps_of(known[wave].keys[lane]), tiles = tiles_of(known[wave].tokens[lane]);
-        for (int l = line.per + (line.more ? 1 : 0), l1 = line.per + line.per / 4 + 1; l <= l1; l++) {
+        for (int l = line.per + (ample || line.more ? 1 : 0), l1 = line.per + line.per / 4 + 1; l <= l1; l++) {
             const int of = (int)(((float)n + (float)l - 0.5f) / (float)l);       // n / l, rounded up (n and l below 2^16, l of a few)
             const int shares = __builtin_amdgcn_readlane(wave_scan(tiles * of), 63) * a.KV;
             if (shares > a.shares) continue;
