@@ -201,6 +201,7 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(LogProbArgs a
         where[0] = 0;
         take(v, 0, most[0], where[0]);
     }
+    far = __any(far);                                                     // (one lane took the broken piece: the others' pieces go the way that its reference needs)
     auto widened = [&](const u32x4& w, float (&v)[EPV]) __attribute__((always_inline)) {
         const Vec16<T> t = __builtin_bit_cast(Vec16<T>, w);
 #pragma unroll
