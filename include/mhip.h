@@ -305,7 +305,7 @@ int mhip_paged_append(void* stream, const mhip_paged_cache* cache, const mhip_se
  * head h / (q_heads / heads)).  Causal: a token sees the keys up to its own position.  A token without keys yields zeros.
  * fp32 softmax state and accumulation; the last bits of a row may depend on the other sequences of the call, whose lengths decide over how many
  * parts its keys are dealt.  strides: {token, head} of q and o in elements, multiples of 8; 16-byte aligned tensors; o may be q, and overlaps nothing else.  BF16, F16.
- * Values in 8 bits become the queries' type in front of the second product, which for F16 ends at 65504.
+ * Values in 8 bits become the queries' type in front of the second product; one beyond F16's greatest number, 65504, counts as that.
  * The workspace (mhip_paged_attention_workspace bytes, 16-byte aligned, overwritten) lets keys be dealt over the whole device; with less, or none, they are not. */
 int64_t mhip_paged_attention_workspace(const mhip_paged_cache* cache, const mhip_sequences* seqs, int64_t q_heads);
 int mhip_paged_attention(void* stream, const mhip_paged_cache* cache, const mhip_sequences* seqs, const void* q, void* o, int64_t q_heads, float scale,

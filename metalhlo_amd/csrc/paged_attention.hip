@@ -145,6 +145,17 @@ __device__ __forceinline__ u32x4 widen(u32x2 w, float scale) {
     return r;
 }
 
+// A finite value under its scale may be more than f16 holds, which ends at 65504 then: an infinity times the weight zero of a key that a row does not see were a NaN of that row's.  (A NaN stays one.)
+// The greatest e4m3 is 448, so that no scale up to 2^7 needs it: the tile kernel, which is short of vector instructions, asks (us, four f16 pieces of 1024 tokens behind 7168 over 8-bit pages, not at all |
+// always 600 | 614, not at all | asked 615 | 622); the rows kernel, whose registers have no room for another way through its loop, does it always (64 sequences of 4096 keys 88.1 | 88.8).
+__device__ __forceinline__ u32x4 ended(u32x4 w) {
+    typedef _Float16 two __attribute__((ext_vector_type(2)));
+    const two most = {(_Float16)65504.f, (_Float16)65504.f};
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_maximum(__builtin_elementwise_minimum(__builtin_bit_cast(two, (uint32_t)w[e]), most), -most));
+    return w;
+}
+
 // A key's value that is not finite makes the results of the rows that see it so, and of no others, but zero times it is no zero: where a result is not finite, the keys are
 // gone through once more with such values left out of the second product where some rows see them and others do not, and they are added to the rows behind it, one by one.
 template <typename T, bool EIGHT>
@@ -556,7 +567,8 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
                 for (int h = 0; h < NT / 2; h++) {
                     u32x4 vf;
                     if constexpr (EIGHT) vf = widen<T>(u32x2{blk.v[f][2 * h], blk.v[f][2 * h + 1]}, vs);
-                    else vf = u32x4{blk.v[f][0], blk.v[f][1], blk.v[f][2], blk.v[f][3]};
+                    if constexpr (EIGHT && std::is_same<T, f16_t>::value) vf = ended(vf);
+                    if constexpr (!EIGHT) vf = u32x4{blk.v[f][0], blk.v[f][1], blk.v[f][2], blk.v[f][3]};
 #pragma unroll
                     for (int x = 0; x < TILES; x++) oacc[x][f] = Mfma16P<T>::run(vf, pb[x][h], oacc[x][f]);
                 }
@@ -911,8 +923,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_tile_kernel(PagedArgs a) 
             char* tv = to + kKBytes;
             if constexpr (EIGHT) {
                 const float scale = scale_of(st.vs[i]);
-                *reinterpret_cast<u32x4*>(tv + tv_off(d, 2 * block)) = widen<T>(u32x2{w.x, w.y}, scale);
-                *reinterpret_cast<u32x4*>(tv + tv_off(d, 2 * block + 1)) = widen<T>(u32x2{w.z, w.w}, scale);
+                u32x4 low = widen<T>(u32x2{w.x, w.y}, scale), high = widen<T>(u32x2{w.z, w.w}, scale);
+                if (std::is_same<T, f16_t>::value && __any(scale > 128.f)) {
+                    low = ended(low);
+                    high = ended(high);
+                }
+                *reinterpret_cast<u32x4*>(tv + tv_off(d, 2 * block)) = low;
+                *reinterpret_cast<u32x4*>(tv + tv_off(d, 2 * block + 1)) = high;
             } else {
                 *reinterpret_cast<u32x4*>(tv + tv_off(d, 2 * block + half)) = w;
             }

@@ -215,7 +215,7 @@ def paged_attention(q, cache: PagedCache, table, lengths, starts, scale: Optiona
                     out: Optional[torch.Tensor] = None):
     """softmax(scale * q k^T, causal) v over each sequence's keys in the cache: q [tokens, query heads, D], query heads a multiple of the cache's heads.  Causal: a
     token sees the keys up to its own position.  A token without keys yields zeros.  Default scale 1/sqrt(D).  Values of an
-    8-bit cache become q's type on the way, so that float16 holds them up to 65504.
+    8-bit cache become q's type on the way, in float16 those beyond 65504 that number.
     `out` may be q, and overlaps nothing else of the call.  The last bits of a row may depend on the
     lengths of the other sequences, as mhip.h says."""
     return (_native or _host()).paged_attention(q, cache, table, lengths, starts, scale, is_causal, out)

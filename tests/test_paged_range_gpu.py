@@ -1,0 +1,74 @@
+"""The operators on a paged cache at the ends of their types' ranges and of their tables: values and keys that float16 does not hold, scales far from one, sequences that are longer than their table, weights far
+apart, many query heads to a key head; and attention over what an append has left in 8 bits, against what is held."""
+import numpy as np
+import pytest
+import torch
+
+from tests.paged_util import E4M3, HostCache, assert_within, attention, table_of
+
+pytestmark = pytest.mark.gpu
+# tokens a sequence that put two query heads a key head into every form: 16 rows, 32 rows, tiles of 128, tiles of 256 (heads of 128 numbers in 16 bits)
+NEW = pytest.mark.parametrize("new", [1, 3, 14, 90, 300])
+ints = lambda v: torch.tensor(np.asarray(v), dtype=torch.int32, device="cuda")  # noqa: E731
+
+
+def _batch(new, context, H, KV, D, page, dtype, eight, seed=0, width=None):
+    rng = np.random.default_rng(seed)
+    keys = [n + c for n, c in zip(new, context)]
+    table, pages = table_of(keys, page, rng, width)
+    cache = HostCache(pages, KV, page, D, dtype, eight).fill(table, keys, rng)
+    starts = [0] + list(np.cumsum(new))
+    q = torch.from_numpy(rng.standard_normal((starts[-1], H, D)).astype(np.float32)).to(dtype)
+    return q, cache, table, keys, starts
+
+
+def _attend(q, cache, table, keys, starts, **kw):
+    from metalhlo_amd import kernels
+    return kernels.paged_attention(q.cuda(), cache.to_device(), ints(table), ints(keys), ints(starts), **kw)
+
+
+class Saturated(HostCache):
+    """Values end at 65504, as float16 holds them."""
+
+    def dense(self, which, table, b, n):
+        x = super().dense(which, table, b, n)
+        return np.clip(x, -65504.0, 65504.0) if which == 1 else x
+
+
+def _rescale(cache, which, page, byte):
+    """A page under another scale, its values rounded to it."""
+    was = cache.scales[which][page].float()
+    cache.x[which][page] = torch.nan_to_num(cache.x[which][page] * (2.0 ** (was - byte))[:, None, None]).to(E4M3).float()
+    cache.scales[which][page] = byte
+
+
+@NEW
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_beyond_float16_end_there(new, D):
+    """An 8-bit page whose largest value is float16's own holds 65536 = 256 * 2 ** 8 for it: the tokens that see it take 65504, those in front of it nothing of it."""
+    q, cache, table, keys, starts = _batch([new, new], [40, 3], 4, 2, D, 16, torch.float16, True, seed=new)
+    cache.__class__ = Saturated
+    for b, n in enumerate(keys):
+        p = table[b, (n - 1) // 16]
+        _rescale(cache, 1, p, 135)
+        cache.x[1][p, :, (n - 1) % 16, 5] = 256.0
+        cache.x[1][p, :, (n - 1) % 16, 9] = -448.0              # (bfloat16 wrote it: 114688)
+    got = _attend(q, cache, table, keys, starts)
+    want, bound = attention(q, cache, table, keys, starts)
+    assert_within(got, want, bound, f"{new}")
+
+
+@NEW
+def test_what_is_no_number_stays_one_beside_values_that_saturate(new):
+    q, cache, table, keys, starts = _batch([new], [40], 4, 2, 64, 16, torch.float16, True, seed=new)
+    cache.__class__ = Saturated
+    n = keys[0]
+    p = table[0, (n - 1) // 16]
+    _rescale(cache, 1, p, 136)
+    cache.x[1][p, :, (n - 1) % 16, 5] = 448.0
+    want, bound = attention(q, cache, table, keys, starts)
+    cache.x[1][p, :, (n - 1) % 16, 7] = float("nan")
+    got = _attend(q, cache, table, keys, starts)
+    assert torch.isnan(got[-1, :, 7]).all()
+    got[-1, :, 7] = torch.from_numpy(want[-1, :, 7]).to(got)
+    assert_within(got, want, bound, f"{new}")
