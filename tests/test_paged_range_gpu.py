@@ -5,8 +5,10 @@ import pytest
 import torch
 
 from tests.paged_util import E4M3, HostCache, assert_within, attention, table_of
+from tests.util import NAME
 
 pytestmark = pytest.mark.gpu
+HALF = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=lambda d: NAME[d])
 # tokens a sequence that put two query heads a key head into every form: 16 rows, 32 rows, tiles of 128, tiles of 256 (heads of 128 numbers in 16 bits)
 NEW = pytest.mark.parametrize("new", [1, 3, 14, 90, 300])
 ints = lambda v: torch.tensor(np.asarray(v), dtype=torch.int32, device="cuda")  # noqa: E731
@@ -72,3 +74,42 @@ def test_what_is_no_number_stays_one_beside_values_that_saturate(new):
     assert torch.isnan(got[-1, :, 7]).all()
     got[-1, :, 7] = torch.from_numpy(want[-1, :, 7]).to(got)
     assert_within(got, want, bound, f"{new}")
+
+
+@NEW
+def test_keys_beyond_float16(new):
+    """A key of 320 * 2 ** 8, which a rotation of float16's greatest numbers comes to: a row's score is what its product in fp32 is, whichever kernel serves it."""
+    q, cache, table, keys, starts = _batch([new, new], [40, 3], 4, 2, 64, 16, torch.float16, True, seed=new)
+    q = torch.where(q.abs() < 0.25, 0.25, q.float()).half()
+    for b, n in enumerate(keys):
+        p = table[b, (n - 1) // 16]
+        _rescale(cache, 0, p, 135)
+        cache.x[0][p, :, (n - 1) % 16] = 0.0
+        cache.x[0][p, :, (n - 1) % 16, 11] = 320.0
+    got = _attend(q, cache, table, keys, starts)
+    want, bound = attention(q, cache, table, keys, starts)          # (scores of 81920 * |q| / 8, 2560 at least: the key has the whole weight, or none)
+    assert_within(got, want, bound, f"{new}")
+
+
+@HALF
+@NEW
+@pytest.mark.parametrize("by", [-40, 30])
+def test_keys_whose_scales_are_far_from_one(by, new, dtype):
+    """Keys of 2 ** by times the usual size under an attention scale that makes up for it."""
+    q, cache, table, keys, starts = _batch([new, new], [40, 3], 4, 2, 64, 16, dtype, True, seed=new)
+    cache.scales[0] = (cache.scales[0].int() + by).clamp(min=0).to(torch.uint8)
+    scale = 2.0 ** (-by - 3)
+    got = _attend(q, cache, table, keys, starts, scale=scale)
+    want, bound = attention(q, cache, table, keys, starts, scale=scale)
+    assert_within(got, want, bound, f"{by} {new}")
+
+
+@NEW
+@pytest.mark.parametrize("scale", [1e-35, 0.0, -1e-35])
+def test_products_of_scales_that_are_no_float(scale, new):
+    """A page's scale times the attention's is below every float: all keys alike, and masked ones none."""
+    q, cache, table, keys, starts = _batch([new, new], [40, 3], 4, 2, 64, 16, torch.bfloat16, True, seed=new)
+    cache.scales[0].fill_(3)
+    got = _attend(q, cache, table, keys, starts, scale=scale)
+    want, bound = attention(q, cache, table, keys, starts, scale=0.0)
+    assert_within(got, want, bound, f"{scale} {new}")
