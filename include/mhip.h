@@ -282,7 +282,7 @@ typedef struct {
  *   starts  [sequences + 1]      sequence b's new tokens are rows starts[b] .. starts[b + 1] of the call's tensors, in order; rows behind the last one
  *                                (a padded batch) are neither read nor written
  *   lengths [sequences]          its keys in all, the new tokens' among them (they are the last ones)
- *   table   [sequences, width]   the pages of its keys; an entry outside [0, pages) holds no keys and takes none
+ *   table   [sequences, width]   the pages of its keys; an entry outside [0, pages) holds no keys and takes none, and so does a position behind the last entry
  * `tokens` is the number of rows of the tensors.  A sequence may have no new tokens.  Pages may be shared for reading; a page that takes tokens
  * belongs to one sequence, once.  Up to 65536 sequences, 2^24 tokens and 2^24 keys a sequence. */
 typedef struct {

@@ -7,8 +7,8 @@
 // in 16 bits, or in 8 as e4m3 with a scale 2^(byte - 127) for each page and head ([pages, KV]).  A power of two moves the exponent alone: a value keeps
 // its four significant bits under any scale, and only what falls below the format's range (2^-9 of the scale; the page's largest value is 2^7.8 of it or more) is lost.
 //
-// Every index that comes from device memory is bounded before it is used: a sequence's rows to the tokens of the call, its length to what the table reaches, a page's
-// number to the cache (one outside of it holds no keys and takes none).
+// Every index that comes from device memory is bounded before it is used: a sequence's rows to the tokens of the call, its keys to what the table reaches, a page's
+// number to the cache (one outside of it holds no keys and takes none, and so does what lies behind the table).
 #pragma once
 #include <type_traits>
 
@@ -26,7 +26,9 @@ struct Sequences {
 
     __device__ __forceinline__ int start(int b) const { return min(max(starts[b], 0), T); }
     __device__ __forceinline__ int tokens(int b) const { return max(min(starts[b + 1], T) - start(b), 0); }
+    // the keys that have a place; the position behind the last token, which may lie behind the table
     __device__ __forceinline__ int keys(int b) const { return min(max(lengths[b], 0), width << page_shift); }
+    __device__ __forceinline__ int end(int b) const { return min(max(lengths[b], 0), 1 << 30); }
 };
 
 // sum over the lanes up to this one

@@ -1,6 +1,6 @@
 // Keys and values of new tokens into a paged cache (paged.h), the position rotation applied on the way; in 8 bits with the page's scale.
 //
-//   position  p = keys(b) - tokens(b) + i of token i of sequence b, its page table[b, p / page], its slot p % page
+//   position  p = lengths[b] - tokens(b) + i of token i of sequence b, its page table[b, p / page], its slot p % page
 //   rotation  of the first R elements of a head, as mhip_rope turns them: with x = [x1 | x2] (halves) y = [x1 cos - x2 sin | x1 sin + x2 cos], row p of `freqs`
 //             holding the cosines and then the sines.  fp32, and one rounding, to the type that is stored.
 //   8 bits    the page's scale is the least power of two under which its largest value is at most 448.  Where the page holds tokens already it never shrinks, and
@@ -81,18 +81,18 @@ struct Fill {
         const int shift = a.s.page_shift, page = 1 << shift;
         int first;
         auto touched = [&](int b) __attribute__((always_inline)) {
-            const int n = a.s.tokens(b), end = a.s.keys(b), begin = max(end - n, 0);
+            const int n = a.s.tokens(b), end = a.s.end(b), begin = max(end - n, 0);
             return n ? ((end + page - 1) >> shift) - (begin >> shift) : 0;
         };
         const int b = sequence_of(a.s.B, u, touched, first);
         if (b < 0) return false;
-        const int n = a.s.tokens(b), end = a.s.keys(b), begin = max(end - n, 0);      // (more tokens than keys: the first ones have no place)
+        const int n = a.s.tokens(b), end = a.s.end(b), begin = max(end - n, 0);       // (more tokens than keys: the first ones have no place)
         const int at = (begin >> shift) + u - first;
         if (at < begin >> shift || at << shift >= end) return false;                  // (starts that are no starts: their sums may have wrapped)
         pos = max(begin, at << shift);
         const int stop = min(min(end, (at + 1) << shift), a.R ? a.positions : end);
         if (pos >= stop) return false;
-        page_no = a.s.table[(int64_t)b * a.s.width + at];
+        page_no = at < a.s.width ? a.s.table[(int64_t)b * a.s.width + at] : -1;
         slot0 = pos & (page - 1);
         slot1 = slot0 + stop - pos;
         row = a.s.start(b) + (n - (end - pos));

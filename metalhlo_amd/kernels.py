@@ -184,7 +184,7 @@ class PagedCache(NamedTuple):
     float8_e4m3fn with a scale 2 ** (byte - 127) a page and head (`key_scales`, `value_scales`, uint8 [pages, heads]).
 
     The calls on it take what describes the sequences from device memory (all int32): `table` [sequences, width], the pages of each (an entry outside the
-    cache holds no keys and takes none); `lengths` [sequences], its keys, those of the call's tokens among them, which are the last; `starts` [sequences + 1], where its
+    cache holds no keys and takes none, and so does a position behind the last entry); `lengths` [sequences], its keys, those of the call's tokens among them, which are the last; `starts` [sequences + 1], where its
     tokens begin among the rows of q, k and v.  Rows behind the last sequence stay as they are.  A page that takes tokens belongs to one sequence, once."""
     keys: torch.Tensor
     values: torch.Tensor

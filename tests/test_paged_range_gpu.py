@@ -9,6 +9,7 @@ from tests.util import NAME
 
 pytestmark = pytest.mark.gpu
 HALF = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=lambda d: NAME[d])
+EIGHT = pytest.mark.parametrize("eight", [False, True], ids=["16bit", "8bit"])
 # tokens a sequence that put two query heads a key head into every form: 16 rows, 32 rows, tiles of 128, tiles of 256 (heads of 128 numbers in 16 bits)
 NEW = pytest.mark.parametrize("new", [1, 3, 14, 90, 300])
 ints = lambda v: torch.tensor(np.asarray(v), dtype=torch.int32, device="cuda")  # noqa: E731
@@ -113,3 +114,30 @@ def test_products_of_scales_that_are_no_float(scale, new):
     got = _attend(q, cache, table, keys, starts, scale=scale)
     want, bound = attention(q, cache, table, keys, starts, scale=0.0)
     assert_within(got, want, bound, f"{scale} {new}")
+
+
+@EIGHT
+@HALF
+@pytest.mark.parametrize("lengths,new,width", [([35], [5], 2), ([33, 40, 7], [3, 9, 2], 2), ([17, 40, 16], [1, 1, 1], 1), ([33, 1000, 31], [1, 1, 1], 2), ([300, 16, 65], [200, 16, 65], 3),
+                                               ([2000, 16, 48], [20, 16, 48], 3), ([9], [9], 0)], ids=str)
+def test_append_to_sequences_longer_than_their_table(lengths, new, width, eight, dtype):
+    """A token behind the table's last column takes no place, and no other's: the same as with columns that name no page."""
+    from metalhlo_amd import kernels
+    rng = np.random.default_rng(len(lengths))
+    page, KV, H, D = 16, 2, 4, 64
+    starts = [0] + list(np.cumsum(new))
+    table = rng.permutation(3 * width + 1)[:len(lengths) * width].reshape(len(lengths), width)
+    wide = -np.ones((len(lengths), 130), dtype=np.int32)
+    wide[:, :width] = table
+    k, v, q = (torch.from_numpy(rng.standard_normal((starts[-1], n, D)).astype(np.float32)).to(dtype).cuda() for n in (KV, KV, H))
+    freqs = torch.from_numpy(rng.standard_normal((1990, 32)).astype(np.float32)).cuda()
+    results = []
+    for t in (table, wide):
+        c = kernels.paged_cache(3 * width + 1, KV, page, D, E4M3 if eight else dtype)
+        for held in c:
+            if held is not None:
+                held.view(torch.uint8).fill_(40)
+        out = torch.full_like(q, 7)
+        kernels.paged_append(c, k, v, ints(t), ints(lengths), ints(starts), q=q, freqs=freqs, out=out)
+        results.append([out] + [held.view(torch.uint8) for held in c if held is not None])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
