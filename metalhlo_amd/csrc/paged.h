@@ -27,8 +27,11 @@ struct Sequences {
     __device__ __forceinline__ int start(int b) const { return min(max(starts[b], 0), T); }
     __device__ __forceinline__ int tokens(int b) const { return max(min(starts[b + 1], T) - start(b), 0); }
     // the keys that have a place; the position behind the last token, which may lie behind the table
-    __device__ __forceinline__ int keys(int b) const { return min(max(lengths[b], 0), width << page_shift); }
+    __device__ __forceinline__ int reach() const { return width << page_shift; }
+    __device__ __forceinline__ int keys(int b) const { return min(max(lengths[b], 0), reach()); }
     __device__ __forceinline__ int end(int b) const { return min(max(lengths[b], 0), 1 << 30); }
+    // the same where it only matters which keys a token sees: no further behind the table than its tokens are many (below 2^25)
+    __device__ __forceinline__ int bounded_end(int b) const { return min(max(lengths[b], 0), reach() + tokens(b)); }
 };
 
 // sum over the lanes up to this one

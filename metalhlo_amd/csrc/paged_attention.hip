@@ -1,7 +1,7 @@
 // Attention over a paged cache (paged.h): O = softmax(scale Q K^T) V, rows of queries from one token of a sequence to a whole prompt behind a long context.
 //
 //   rows   of a sequence and a key/value head: its tokens times the G = H / KV query heads that share the head, row = token * G + query head, so that K and V are read
-//          once for all of them.  A token's position is keys(b) - tokens(b) + i; with the causal rule it sees the keys up to its own.
+//          once for all of them.  A token's position is lengths[b] - tokens(b) + i; with the causal rule it sees the keys up to its own.
 //   line   All the work of a launch in one line, sequence by sequence, head by head and tile by tile, each as long as its keys: workgroup w takes the w-th of equal shares.  The lengths are not known
 //          on the host, and a batch may hold one long sequence among short ones: the line is measured on the device, by every workgroup for itself.  (Parts of one length for the whole launch
 //          instead: 48 sequences of 1600 to 8000 keys 117 us | 96.)  A part of a tile leaves its reference maximum, its sum and its unnormalised rows in the workspace, and the last one
@@ -74,13 +74,15 @@ struct Line {
     __device__ __forceinline__ int owner(int g) const { return g < more * (per + 1) ? g / (per + 1) : more + (g - more * (per + 1)) / per; }
 };
 
-// The first 64 sequences, in a wave's own LDS.  `line`: the keys that its tiles' stretches of the line are made for.
+// The first 64 sequences, in a wave's own LDS.  `keys`: the position behind its last token, which is more than it has keys where it has outgrown its table; `line`: the keys that its tiles' stretches of the
+// line are made for.
 struct Known { int start[64], tokens[64], keys[64], line[64]; };
 struct Found { int b, before, start, tokens, keys, line; };
 __device__ __forceinline__ void known_of(const Sequences& s, Known& known, int lane) {
     known.start[lane] = lane < s.B ? s.start(lane) : 0;
     known.tokens[lane] = lane < s.B ? s.tokens(lane) : 0;
-    known.keys[lane] = known.line[lane] = lane < s.B ? s.keys(lane) : 0;
+    known.keys[lane] = lane < s.B ? s.bounded_end(lane) : 0;
+    known.line[lane] = lane < s.B ? s.keys(lane) : 0;
 }
 // The sequence that place g of the line lies in, when one has stretch(tokens, keys) of it; `before`: where it begins.  False behind the last.
 template <typename F>
@@ -103,8 +105,9 @@ __device__ __forceinline__ bool found_at(const Sequences& s, const Known& known,
         at.before += further;
         at.start = __builtin_amdgcn_readfirstlane(s.start(at.b));
         at.tokens = __builtin_amdgcn_readfirstlane(s.tokens(at.b));
-        at.keys = at.line = __builtin_amdgcn_readfirstlane(s.keys(at.b));
-        length = stretch(at.tokens, at.keys);
+        at.keys = __builtin_amdgcn_readfirstlane(s.bounded_end(at.b));
+        at.line = __builtin_amdgcn_readfirstlane(s.keys(at.b));
+        length = stretch(at.tokens, at.line);
     }
     return g >= at.before && g - at.before < length;                       // (starts that are no starts: their sums may have wrapped)
 }
@@ -327,7 +330,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
         if (tokens) longest = max(longest, n);
         steps += tiles_of(tokens) * n;
     };
-    count(known[wave].tokens[lane], known[wave].keys[lane]);
+    count(known[wave].tokens[lane], known[wave].line[lane]);
     for (int b = 64 + lane; b < a.s.B; b += 64) count(a.s.tokens(b), a.s.keys(b));
     longest = __builtin_amdgcn_readfirstlane((int)wave_max((float)longest));      // of one sequence (exact: at most 2^16)
     steps = __builtin_amdgcn_readlane(wave_scan(steps), 63) * a.KV;           // of all heads
@@ -339,7 +342,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
     // four tokens each 20.0 | 14.4, one of 8000 11.8 | 11.6, 8 of 250 to 500, 2 heads of 96, 8.0 | 7.1; but one of 1000, 12 heads of 64, 7.8 | 8.3
     const bool ample = line.per == 1 && !line.more;
     if (line.per <= 16 && !(ample && longest > 2 && longest <= 8) && a.s.B <= 64) {
-        const int n = steps_of(known[wave].keys[lane]), tiles = tiles_of(known[wave].tokens[lane]);
+        const int n = steps_of(known[wave].line[lane]), tiles = tiles_of(known[wave].tokens[lane]);
         for (int l = line.per + (ample || line.more ? 1 : 0), l1 = line.per + line.per / 4 + 1; l <= l1; l++) {
             const int of = (int)(((float)n + (float)l - 0.5f) / (float)l);       // n / l, rounded up (n and l below 2^16, l of a few)
             const int shares = __builtin_amdgcn_readlane(wave_scan(tiles * of), 63) * a.KV;
@@ -371,6 +374,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
         const int rows = tokens * a.G;
         int end = keys;                                                       // of the keys that the tile's last row sees
         if (a.is_causal) end = max(keys - tokens + a.by_group(min((tile + 1) * tile_rows, rows) - 1) + 1, 0);
+        end = min(end, a.s.reach());
         const int k0 = s0 << a.unit_shift, k1 = min(end, s1 << a.unit_shift);
         const bool parted = s1 - s0 < mine;
         const Split split = parted ? split_of(line, a.shares, blockIdx.x, origin, mine) : Split{0, 1};
@@ -766,7 +770,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_tile_kernel(PagedArgs a) 
         all += st.before(st.tiles);
         count += st.tiles;
     };
-    add(known[wave].tokens[lane], known[wave].keys[lane]);
+    add(known[wave].tokens[lane], known[wave].line[lane]);
     for (int b = 64 + lane; b < a.s.B; b += 64) add(a.s.tokens(b), a.s.keys(b));
     longest = (int)(wave_max((float)longest) * 1.00001f) + 1;
     shortest = -(int)wave_max((float)-shortest);
@@ -804,17 +808,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_tile_kernel(PagedArgs a) 
             found.start = __builtin_amdgcn_readfirstlane(known[wave].start[found.b]);
             found.tokens = __builtin_amdgcn_readfirstlane(known[wave].tokens[found.b]);
             found.keys = __builtin_amdgcn_readfirstlane(known[wave].keys[found.b]);
+            found.line = __builtin_amdgcn_readfirstlane(known[wave].line[found.b]);
         } else {
             if (!found_at(a.s, known[wave], lane, unit, [&](int tokens, int keys) { return Stretch<ROWS>(a, tokens, keys).tiles; }, found)) return;
             level = unit - found.before;
         }
-        const Stretch<ROWS> st(a, found.tokens, found.keys);
+        const Stretch<ROWS> st(a, found.tokens, found.line);
         tile = st.tiles - 1 - level;
         off1 = length = st.length(tile);
         g = stop;
     } else {
         if (!found_at(a.s, known[wave], lane, g, [&](int tokens, int keys) { const Stretch<ROWS> st(a, tokens, keys); return a.KV * st.before(st.tiles); }, found)) return;
-        const Stretch<ROWS> st(a, found.tokens, found.keys);
+        const Stretch<ROWS> st(a, found.tokens, found.line);
         const int of_head = st.before(st.tiles), x = g - found.before;
         head = x / of_head;
         tile = st.tile(x - head * of_head);
@@ -828,6 +833,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_tile_kernel(PagedArgs a) 
     const int rows = tokens * a.G, row = tile * ROWS + 32 * wave + li, token = a.by_group(row);
     int end = keys;                                                          // of the keys that the tile's last row sees
     if (a.is_causal) end = max(keys - tokens + a.by_group(min((tile + 1) * ROWS, rows) - 1) + 1, 0);
+    end = min(end, a.s.reach());
     auto cut = [&](int off) __attribute__((always_inline)) { return off == 0 ? 0 : off >= length ? end : min(max((off << a.unit_shift) - 96, 0) & ~(kStage - 1), end); };
     const int k0 = cut(off0), k1 = cut(off1);
     const bool parted = off0 > 0 || off1 < length;

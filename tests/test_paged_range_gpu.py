@@ -116,6 +116,21 @@ def test_products_of_scales_that_are_no_float(scale, new):
     assert_within(got, want, bound, f"{scale} {new}")
 
 
+# ---------------------------------------------------------------- more keys than the table reaches
+@EIGHT
+@NEW
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_of_sequences_longer_than_their_table(causal, new, eight):
+    """Keys behind a table's last column are keys that it does not name; the positions of the tokens are what the lengths say."""
+    q, cache, table, keys, starts = _batch([new] * 3, [64 - new % 64 + 32, 300, 7], 4, 2, 64, 32, torch.bfloat16, eight, seed=new)
+    for width in (1, 2, (new + 32) // 32, 5):
+        short = table[:, :width].copy() if width < table.shape[1] else table
+        padded = np.where(np.arange(table.shape[1])[None] < width, table, -1)
+        got = _attend(q, cache, short, keys, starts, is_causal=causal)
+        want, bound = attention(q, cache, padded, keys, starts, is_causal=causal)
+        assert_within(got, want, bound, f"{width} {new} {causal}")
+
+
 @EIGHT
 @HALF
 @pytest.mark.parametrize("lengths,new,width", [([35], [5], 2), ([33, 40, 7], [3, 9, 2], 2), ([17, 40, 16], [1, 1, 1], 1), ([33, 1000, 31], [1, 1, 1], 2), ([300, 16, 65], [200, 16, 65], 3),
