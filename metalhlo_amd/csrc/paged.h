@@ -70,7 +70,8 @@ __device__ __forceinline__ int sequence_of(int B, int u, F units, int& first) {
 // 2^(byte - 127); the byte 0, which no append writes, as 1
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __builtin_bit_cast(float, max(byte, 1u) << 23); }
 
-// What the two entry points ask of a cache and of sequences before anything is launched.
+// What the two entry points ask of a cache and of sequences before anything is planned or launched: their sizes, and then what they point to.
+int check_sizes(const char* what, const mhip_paged_cache* c, const mhip_sequences* s);
 int check_paged(const char* what, const mhip_paged_cache* c, const mhip_sequences* s, int dtype, bool* empty);
 
 inline Sequences sequences(const mhip_paged_cache* c, const mhip_sequences* s) {

@@ -470,16 +470,22 @@ int launch_d(hipStream_t st, const AppendArgs& a, int64_t D, int64_t units) {
 
 }  // namespace
 
-int check_paged(const char* what, const mhip_paged_cache* c, const mhip_sequences* s, int dtype, bool* empty) {
-    *empty = false;
+int check_sizes(const char* what, const mhip_paged_cache* c, const mhip_sequences* s) {
     if (!c || !s) return fail(MHIP_ERR_INVALID_ARGUMENT, "%s: NULL cache or sequences", what);
-    if (dtype != MHIP_BF16 && dtype != MHIP_F16) return fail(MHIP_ERR_UNSUPPORTED, "%s: dtype %d (need bf16 or f16)", what, dtype);
     if (c->pages <= 0 || c->heads <= 0 || s->sequences < 0 || s->width < 0 || s->tokens < 0) return fail(MHIP_ERR_INVALID_ARGUMENT, "%s: a size is negative, or the cache has no pages or heads", what);
     if (c->head_size < 32 || c->head_size > 128 || c->head_size % 32) return fail(MHIP_ERR_UNSUPPORTED, "%s: head size %lld (need 32, 64, 96 or 128)", what, (long long)c->head_size);
     if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
         return fail(MHIP_ERR_UNSUPPORTED, "%s: page size %lld (need a power of two from 16 to 256)", what, (long long)c->page_size);
-    if (c->pages * c->heads > INT32_MAX || c->pages > INT32_MAX || c->heads > 1024 || s->sequences > 65536 || s->tokens > (1 << 24) || s->width > (1 << 20) || s->width * c->page_size > (1 << 24))
-        return fail(MHIP_ERR_UNSUPPORTED, "%s: more than 65536 sequences, 2^24 tokens, 2^24 keys a sequence or 1024 heads", what);
+    // (every size by itself in front of a product with it)
+    if (c->pages > INT32_MAX || c->heads > 1024 || c->pages * c->heads > INT32_MAX || s->sequences > 65536 || s->tokens > (1 << 24) || s->width > (1 << 20) || s->width * c->page_size > (1 << 24))
+        return fail(MHIP_ERR_UNSUPPORTED, "%s: more than 65536 sequences, 2^24 tokens, 2^24 keys a sequence, 1024 heads or 2^31 pages times heads", what);
+    return MHIP_OK;
+}
+
+int check_paged(const char* what, const mhip_paged_cache* c, const mhip_sequences* s, int dtype, bool* empty) {
+    *empty = false;
+    if (const int rc = check_sizes(what, c, s)) return rc;
+    if (dtype != MHIP_BF16 && dtype != MHIP_F16) return fail(MHIP_ERR_UNSUPPORTED, "%s: dtype %d (need bf16 or f16)", what, dtype);
     if (!c->key_scales != !c->value_scales) return fail(MHIP_ERR_INVALID_ARGUMENT, "%s: scales of keys without scales of values", what);
     if (s->sequences == 0 || s->tokens == 0) { *empty = true; return MHIP_OK; }
     if (!s->starts || !s->lengths || (s->width && !s->table)) return fail(MHIP_ERR_INVALID_ARGUMENT, "%s: NULL table, lengths or starts", what);

@@ -1135,10 +1135,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_tile_kernel(PagedArgs a) 
 // The launch that serves these sizes: rows of a workgroup's tile, the workgroups that share the work, and log2 of the keys that a unit of their line stands for.
 struct Plan { int rows, shares, unit_shift; bool single; int64_t tiles; };
 
-Plan plan_of(const mhip_paged_cache* c, const mhip_sequences* s, int64_t q_heads) {
+// Of sizes that check_sizes lets pass; refused is what has more rows than the kernels' integers hold, or more tiles than a launch of a workgroup each has threads for (2^32).
+int plan_of(const mhip_paged_cache* c, const mhip_sequences* s, int64_t q_heads, Plan& p) {
+    if (q_heads <= 0 || q_heads % c->heads) return fail(MHIP_ERR_INVALID_ARGUMENT, "paged_attention: %lld query heads over %lld key heads", (long long)q_heads, (long long)c->heads);
+    if (s->sequences == 0 || s->tokens == 0) return MHIP_OK;
+    if (q_heads / c->heads >= ((1 << 30) + s->tokens - 1) / s->tokens) return fail(MHIP_ERR_UNSUPPORTED, "paged_attention: more than 2^30 rows");
     const int64_t G = q_heads / c->heads, average = (s->tokens + s->sequences - 1) / s->sequences * G;
     const int rows = average <= 16 ? 16 : average <= 32 ? 32 : average >= 256 && c->head_size == 128 && !c->key_scales ? 256 : 128;
     const double tiles = (double)(s->tokens * G / rows + (s->sequences < s->tokens ? s->sequences : s->tokens)) * c->heads;      // that there can be
+    if (rows >= 128 && tiles * (2 * rows) >= 4294967296.0) return fail(MHIP_ERR_UNSUPPORTED, "paged_attention: more tiles than a launch has workgroups");      // (two threads a row)
     const int64_t keys = s->width * c->page_size;
     auto most = [&](int shift) { return rows >= 128 ? tiles * (double)((2 * (keys + 2 * kTileCost) >> shift) + 1) : tiles * (double)((keys >> shift) + 1); };
     const bool single = s->tokens <= s->sequences && G <= rows && rows < 128;
@@ -1146,7 +1151,8 @@ Plan plan_of(const mhip_paged_cache* c, const mhip_sequences* s, int64_t q_heads
     while (most(shift) > (double)(1 << 29)) shift++;
     int shares = (rows >= 128 ? 256 / rows : rows_kernel_workgroups(rows / 16, c->head_size, single)) * compute_units();
     if (rows < 128 && most(shift) < shares) shares = (int)most(shift);                                                     // (a step is the least share)
-    return {rows, shares, shift, single, (int64_t)tiles};
+    p = {rows, shares, shift, single, (int64_t)tiles};
+    return MHIP_OK;
 }
 
 int64_t workspace_of(const mhip_paged_cache* c, const Plan& p) { return (int64_t)p.shares * (2 * p.rows * (c->head_size + 2) * 4 + 8); }
@@ -1179,22 +1185,21 @@ int launch_d(hipStream_t st, const PagedArgs& a, const Plan& p, int64_t D) {
 using namespace mhip;
 
 extern "C" int64_t mhip_paged_attention_workspace(const mhip_paged_cache* cache, const mhip_sequences* seqs, int64_t q_heads) {
-    if (!cache || !seqs || cache->heads <= 0 || q_heads <= 0 || q_heads % cache->heads || seqs->sequences <= 0 || seqs->tokens <= 0) return 0;
-    return workspace_of(cache, plan_of(cache, seqs, q_heads));
+    Plan p{};
+    return check_sizes("paged_attention_workspace", cache, seqs) || plan_of(cache, seqs, q_heads, p) ? 0 : workspace_of(cache, p);
 }
 
 extern "C" int mhip_paged_attention(void* stream, const mhip_paged_cache* cache, const mhip_sequences* seqs, const void* q, void* o, int64_t q_heads, float scale,
                                     int is_causal, const int64_t* strides, int dtype, void* workspace, int64_t workspace_bytes) {
     bool empty;
     if (const int rc = check_paged("paged_attention", cache, seqs, dtype, &empty)) return rc;
-    if (q_heads <= 0 || q_heads % cache->heads) return fail(MHIP_ERR_INVALID_ARGUMENT, "paged_attention: %lld query heads over %lld key heads", (long long)q_heads, (long long)cache->heads);
+    Plan p{};
+    if (const int rc = plan_of(cache, seqs, q_heads, p)) return rc;
     if (empty) return MHIP_OK;
     if (!q || !o || !strides) return fail(MHIP_ERR_INVALID_ARGUMENT, "paged_attention: NULL tensor");
     if (((uintptr_t)q | (uintptr_t)o | (uintptr_t)workspace) & 15) return fail(MHIP_ERR_UNSUPPORTED, "paged_attention: tensors must be 16-byte aligned");
     for (int i = 0; i < 4; i++)
         if (strides[i] % 8) return fail(MHIP_ERR_UNSUPPORTED, "paged_attention: strides must be multiples of 8 elements");
-    if (seqs->tokens * (q_heads / cache->heads) >= 1 << 30) return fail(MHIP_ERR_UNSUPPORTED, "paged_attention: more than 2^30 rows");
-    const Plan p = plan_of(cache, seqs, q_heads);
     PagedArgs a{q, o, (const char*)cache->keys, (const char*)cache->values, cache->key_scales, cache->value_scales, sequences(cache, seqs),
                 (int)cache->pages, (int)cache->heads, (int)(q_heads / cache->heads), is_causal ? 1 : 0, p.shares, scale == 0.f ? 1e-30f : std::fabs(scale) * kLog2e, std::signbit(scale) ? 0x80008000u : 0u, {strides[0], strides[1]}, {strides[2], strides[3]},
                 nullptr, nullptr, 0, Divider((uint32_t)(q_heads / cache->heads)), Divider((uint32_t)cache->heads), Divider((uint32_t)p.shares), p.unit_shift};
@@ -1203,7 +1208,6 @@ extern "C" int mhip_paged_attention(void* stream, const mhip_paged_cache* cache,
         a.words = reinterpret_cast<uint64_t*>(a.part + 2 * (int64_t)p.shares * p.rows * (cache->head_size + 2));
         a.tag = launch_tag();
     }
-    if (p.tiles >= 1 << 30) return fail(MHIP_ERR_UNSUPPORTED, "paged_attention: more tiles than a launch has workgroups");
     hipStream_t st = as_stream(stream);
     const bool eight = cache->key_scales != nullptr;
     const int64_t D = cache->head_size;
