@@ -315,7 +315,7 @@ int mhip_paged_attention(void* stream, const mhip_paged_cache* cache, const mhip
  * its `top` most likely tokens (up to 64; 0: none, NULL) with their log probabilities [rows, top], the most likely first and the lowest index among equals.  A -inf logit has
  * probability zero; a row that holds a NaN or +inf, or nothing but -inf, yields NaN log probabilities and entropy, and its alternatives in the order of its
  * logits, a NaN above all (as mhip_argmax).  BF16, F16, F32 logits of any alignment of their type, I32 or I64 tokens; fp32 arithmetic and results.
- * The workspace (mhip_token_log_probs_workspace bytes, 0: of no use; 16-byte aligned, overwritten) lets few rows be dealt over the whole device.
+ * Fewer than 2^24 rows.  The workspace (mhip_token_log_probs_workspace bytes, 0: of no use; 16-byte aligned, overwritten) lets few rows be dealt over the whole device.
  * The reference has softmax only (Metal/Kernels/SoftmaxKernel.swift:16-215). */
 int64_t mhip_token_log_probs_workspace(int64_t rows, int64_t vocab, int top);
 int mhip_token_log_probs(void* stream, const void* logits, const void* tokens, float* log_probs, float* entropy, float* top_log_probs, int32_t* top_ids,

@@ -437,6 +437,7 @@ extern "C" int mhip_token_log_probs(void* stream, const void* logits, const void
     if (top < 0 || top > kMaxTop || top > vocab) return fail(MHIP_ERR_INVALID_ARGUMENT, "token_log_probs: %d alternatives of %lld (up to 64)", top, (long long)vocab);
     if (dtype != MHIP_BF16 && dtype != MHIP_F16 && dtype != MHIP_F32) return fail(MHIP_ERR_UNSUPPORTED, "token_log_probs: dtype %d (need bf16, f16 or f32)", dtype);
     if (token_dtype != MHIP_I32 && token_dtype != MHIP_I64) return fail(MHIP_ERR_UNSUPPORTED, "token_log_probs: token dtype %d (need i32 or i64)", token_dtype);
+    if (rows >= 1 << 24) return fail(MHIP_ERR_UNSUPPORTED, "token_log_probs: %lld rows, more than a launch has threads for", (long long)rows);      // (2^32 of them, 256 a row; rows in parts are few)
     if (rows == 0) return MHIP_OK;
     if (!logits || !tokens || !log_probs || (top && (!top_log_probs || !top_ids))) return fail(MHIP_ERR_INVALID_ARGUMENT, "token_log_probs: NULL tensor");
     if ((uintptr_t)logits % size_of(dtype) || (uintptr_t)workspace % 16) return fail(MHIP_ERR_INVALID_ARGUMENT, "token_log_probs: misaligned buffer");
@@ -451,7 +452,6 @@ extern "C" int mhip_token_log_probs(void* stream, const void* logits, const void
     }
     const int64_t per = 16 / size_of(dtype), pieces = (vocab + per - 1) / per + 1;
     a.pieces = (pieces + a.parts - 1) / a.parts;
-    if (rows * a.parts > INT32_MAX) return fail(MHIP_ERR_UNSUPPORTED, "token_log_probs: more rows than a launch has workgroups");
     hipStream_t st = as_stream(stream);
     // rows that neither are dealt nor fill the device have workgroups of eight waves.  us, four waves | eight: 300 rows of 32003 f32 with five alternatives 15.1 | 13.1, 400 of 50257 bf16 with 20 17.9 | 15.5;
     // but 64 of 128000 13.1 | 14.2, 1000 of 32000 with 20 18.3 | 19.7, 1500 of 32003 18.6 | 20.1

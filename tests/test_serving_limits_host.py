@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 
 from metalhlo_amd import _lib
-from tests.test_serving_host import attend, cache, seqs
+from tests.test_serving_host import BF16, F16, F32, I32, P, attend, cache, seqs
 
 
 def _need(c, s, heads):
@@ -34,3 +34,10 @@ def test_no_workspace_for_what_is_refused(c, s):
     c, s = cache(**c), seqs(**s)
     assert _need(c, s, max(c.heads, 1) * 2) == 0
     assert attend(c, s, heads=max(c.heads, 1) * 2) in (1, 2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows", [1 << 24, (1 << 24) + 1, 1 << 40])
+def test_more_rows_of_logits_than_a_launch_has_threads_for(rows, dtype):
+    code = _lib.load().mhip_token_log_probs(None, P, P, P, P, None, None, rows, 100, 0, dtype, I32, None, 0)
+    assert code == 2 and b"launch" in _lib.load().mhip_last_error()
