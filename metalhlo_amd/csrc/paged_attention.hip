@@ -185,6 +185,16 @@ __device__ __forceinline__ const char* value_at(const PagedArgs& a, const int32_
     return ok ? a.values + (((((int64_t)page * a.KV + head) << blocks) + ((key >> 4) & ((1 << blocks) - 1))) * (16 * D) + (key & 15)) * SIZE : nullptr;
 }
 
+// x and the two numbers of w: a row's sum is that of the rounded weights, which are the ones that its values are multiplied with.  (With the weights' own sum a mean of values that are all f16's greatest number
+// is an infinity where the rounding went up.)
+template <typename T>
+__device__ __forceinline__ float plus_two(uint32_t w, float x) {
+    typedef T two __attribute__((ext_vector_type(2)));
+    const two one = {(T)1.f, (T)1.f};
+    if constexpr (std::is_same<T, bf16_t>::value) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(two, w), one, x, false);
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(two, w), one, x, false);
+}
+
 template <typename T> struct Mfma16P;
 template <> struct Mfma16P<bf16_t> {
     __device__ static f32x4 run(u32x4 a, u32x4 b, f32x4 c) {
@@ -529,19 +539,18 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
                 const float m_new = moved_reference(m_run[x], top), use = m_new == -INFINITY ? 0.f : m_new;
                 const float alpha = weight(m_run[x], use);
                 m_run[x] = m_new;
-                float lsum = 0.f;
+                float lsum[2] = {0.f, 0.f};
 #pragma unroll
-                for (int e = 0; e < 4 * NT; e++) {
-                    sv[x][e] = weight(sv[x][e], use);
-                    lsum += sv[x][e];
+                for (int e = 0; e < 2 * NT; e++) {
+                    const uint32_t two = Mfma32A<T>::pack2(weight(sv[x][2 * e], use), weight(sv[x][2 * e + 1], use));
+                    pb[x][e >> 2][e & 3] = two;
+                    lsum[e & 1] = plus_two<T>(two, lsum[e & 1]);
                 }
-                l_run[x] = l_run[x] * alpha + lsum;
+                l_run[x] = l_run[x] * alpha + (lsum[0] + lsum[1]);
                 if (__any(alpha != 1.f)) {
 #pragma unroll
                     for (int f = 0; f < NF; f++) oacc[x][f] *= alpha;
                 }
-#pragma unroll
-                for (int e = 0; e < 2 * NT; e++) pb[x][e >> 2][e & 3] = Mfma32A<T>::pack2(sv[x][2 * e], sv[x][2 * e + 1]);
             }
         };
         auto added = [&](Block& blk, int key, const u32x4 (&pb)[TILES][NT / 2], uint32_t vs8, uint32_t absent) __attribute__((always_inline)) {
@@ -687,15 +696,6 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
 }
 
 // ---------------------------------------------------------------- many rows
-// x and the two numbers of w
-template <typename T>
-__device__ __forceinline__ float plus_two(uint32_t w, float x) {
-    typedef T two __attribute__((ext_vector_type(2)));
-    const two one = {(T)1.f, (T)1.f};
-    if constexpr (std::is_same<T, bf16_t>::value) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(two, w), one, x, false);
-    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(two, w), one, x, false);
-}
-
 // 128 rows, 32 a wave, over stages of 64 keys that lie in LDS in the queries' type, two of them: the next one is on its way in registers and is converted and put down behind this one's products.
 // Two workgroups a unit, so that one is at its products while the other is at its weights; a wave at its products goes first (s_setprio: 647 us | 639).  A stage of all eight waves of a unit takes
 // some 3000 cycles, of which the matrix units are busy 2048 (1024 a wave, two waves each), LDS 2560 (32 KB of operands a wave, and two stages that are put down) and the vector units some 2600 (the
@@ -1001,7 +1001,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_tile_kernel(PagedArgs a) 
         const float m_new = moved_reference(m_run, top), use = m_new == -INFINITY ? 0.f : m_new;
         const float alpha = weight(m_run, use);
         m_run = m_new;
-        // the sum is that of the rounded weights, which are the ones that the values are multiplied with
         float lsum[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < 2; j++)

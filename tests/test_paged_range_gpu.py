@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.paged_util import E4M3, HostCache, assert_within, attention, table_of
+from tests.paged_util import E4M3, HostCache, assert_within, attention, attention_at_once, table_of
 from tests.util import NAME
 
 pytestmark = pytest.mark.gpu
@@ -114,6 +114,49 @@ def test_products_of_scales_that_are_no_float(scale, new):
     got = _attend(q, cache, table, keys, starts, scale=scale)
     want, bound = attention(q, cache, table, keys, starts, scale=0.0)
     assert_within(got, want, bound, f"{scale} {new}")
+
+
+@EIGHT
+@NEW
+@pytest.mark.parametrize("D", [64, 128])
+def test_results_do_not_exceed_the_largest_value(new, D, eight):
+    """Weights whose rounded sum is more than the sum they are divided by make more of float16's greatest number than it holds."""
+    q, cache, table, keys, starts = _batch([new, new], [700, 90], 4, 2, D, 16, torch.float16, eight, seed=new)
+    cache.__class__ = Saturated
+    for p in table[table >= 0]:
+        if eight:
+            cache.scales[1][p] = 135
+        cache.x[1][p] = 256.0 if eight else 65504.0
+    got = _attend(q, cache, table, keys, starts, scale=0.3)
+    want, bound = attention_at_once(q, cache, table, keys, starts, scale=0.3)
+    assert bool(got.isfinite().all())
+    assert_within(got, want, bound, f"{new}")
+
+
+@HALF
+@EIGHT
+@NEW
+def test_many_small_weights_beside_a_large_one(new, eight, dtype):
+    """One key in 512 has weight 1, the others 2 ** -14.7, below float16's normal numbers: together they are a fiftieth and no rounding may lose them."""
+    rng = np.random.default_rng(new)
+    B, N, page, D = 2, 2048 + new, 64, 64
+    table, pages = table_of([N] * B, page, rng)
+    cache = HostCache(pages, 1, page, D, dtype, eight, fill=0.0)
+    for b in range(B):
+        for i in range(-(-N // page)):
+            p = table[b, i]
+            at = torch.arange(i * page, (i + 1) * page)
+            cache.x[0][p, 0, :, 0] = torch.where(at % 512 == 3, 0.0, -1.0)
+            cache.x[1][p, 0] = torch.where(at % 512 == 3, 1.0, 0.5)[:, None]
+            if eight:
+                cache.scales[0][p], cache.scales[1][p] = 127, 127
+    starts = [0, new, 2 * new]
+    q = torch.zeros(2 * new, 2, D, dtype=dtype)
+    q[:, :, 0] = 10.1875                                      # exp(-10.1875) = 2 ** -14.7
+    for causal in (False, True):
+        got = _attend(q, cache, table, [N] * B, starts, scale=1.0, is_causal=causal)
+        want, bound = attention_at_once(q, cache, table, [N] * B, starts, scale=1.0, is_causal=causal)
+        assert_within(got, want, bound, f"{new} {causal}")
 
 
 # ---------------------------------------------------------------- more keys than the table reaches
