@@ -42,13 +42,13 @@ __device__ __forceinline__ u32x4 to_vector(const float* x) {
     for (int e = 0; e < 8; e++) t.v[e] = Elem<T>::from_f32(x[e]);
     return __builtin_bit_cast(u32x4, t);
 }
-// four e4m3 of x * inv; e4m3 has no infinities, so what is not finite becomes NaN
-__device__ __forceinline__ uint32_t pack8(const float* x, float inv) {
+// four e4m3 of x * inv, of `most` at most where that is finite; e4m3 has no infinities, so what is not finite becomes NaN
+__device__ __forceinline__ uint32_t pack8(const float* x, float inv, float most) {
     float y[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         y[e] = x[e] * inv;
-        y[e] = fabsf(y[e]) <= 448.f ? y[e] : __builtin_nanf("");
+        y[e] = fabsf(y[e]) <= 448.f ? __builtin_amdgcn_fmed3f(y[e], -most, most) : __builtin_nanf("");
     }
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
@@ -57,7 +57,7 @@ __device__ __forceinline__ uint32_t pack8(const float* x, float inv) {
 __device__ __forceinline__ uint32_t moved8(uint32_t w, float factor) {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
     const float x[4] = {lo[0], lo[1], hi[0], hi[1]};
-    return pack8(x, factor);
+    return pack8(x, factor, 448.f);
 }
 __device__ __forceinline__ float finite_max(float m, float x) { return fmaxf(m, fabsf(x) < INFINITY ? fabsf(x) : 0.f); }
 
@@ -101,14 +101,16 @@ struct Fill {
 };
 
 // the scale's byte for a page whose new tokens reach `top`, and whether the old ones have to follow it
+// most: under the scale 2^120 what would be rounded to 256, which is 2^128, ends at the number below it (247 becomes 240, not quite half a step from 256)
 struct Scale {
-    float inv, factor;
+    float inv, factor, most;
     int byte;
     bool moves;
     __device__ __forceinline__ Scale(float top, int was, bool begun) {
         was = begun ? max(was, 1) : 0;
         byte = max(scale_byte(top), was);
         inv = scale_of(254 - byte);
+        most = byte == 247 ? 247.f : 448.f;
         moves = begun && byte > was;
         factor = scale_of(127 + was - byte > 0 ? 127 + was - byte : 1);
     }
@@ -230,10 +232,11 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
                     for (int e = 0; e < 16; e++) top = finite_max(top, y[t][e]);
                 }
             }
-            float inv = 1.f;
+            float inv = 1.f, most = 448.f;
             if (EIGHT && !is_q) {
                 const Scale sc(of_page(top, head), was, s0 > 0);
                 inv = sc.inv;
+                most = sc.most;
                 if (sc.moves) move_keys(a.keys + page_head * page * D, s0, D, sc.factor, threadIdx.x, 64 * WAVES);
                 if (threadIdx.x == 0) scales_out[page_head] = (uint8_t)sc.byte;
             }
@@ -247,8 +250,8 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
                     put_stream<u32x4>(out + d2, to_vector<T>(y[t] + 8));
                 } else {
                     char* out = a.keys + (page_head * page + slot) * D;
-                    put_stream<u32x2>(out + d1, u32x2{pack8(y[t], inv), pack8(y[t] + 4, inv)});
-                    put_stream<u32x2>(out + d2, u32x2{pack8(y[t] + 8, inv), pack8(y[t] + 12, inv)});
+                    put_stream<u32x2>(out + d1, u32x2{pack8(y[t], inv, most), pack8(y[t] + 4, inv, most)});
+                    put_stream<u32x2>(out + d2, u32x2{pack8(y[t] + 8, inv, most), pack8(y[t] + 12, inv, most)});
                 }
             }
         }
@@ -307,7 +310,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
             top = finite_max(finite_max(top, y[0][t]), y[1][t]);
         }
         const Scale sc(of_page(top, head), was, s0 > 0);
-        const float inv = sc.inv;
+        const float inv = sc.inv, most = sc.most;
         if (sc.moves) move_values(a.values + page_head * page * D, s0, D, sc.factor, threadIdx.x, 64 * WAVES);
         if (threadIdx.x == 0) scales_out[page_head] = (uint8_t)sc.byte;
         if (!mine) continue;
@@ -317,14 +320,14 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
             if (all) {
                 uint32_t w[kMine / 4];
 #pragma unroll
-                for (int e = 0; e < kMine / 4; e++) w[e] = pack8(y[j] + 4 * e, inv);
+                for (int e = 0; e < kMine / 4; e++) w[e] = pack8(y[j] + 4 * e, inv, most);
                 __builtin_memcpy(__builtin_assume_aligned(a.values + at16, kMine), w, kMine);
             } else {
 #pragma unroll
                 for (int t = 0; t < kMine; t++) {
                     if (slot + t < s0 || slot + t >= s1) continue;
                     const float four[4] = {y[j][t], 0.f, 0.f, 0.f};
-                    a.values[at16 + t] = (char)(pack8(four, inv) & 255);
+                    a.values[at16 + t] = (char)(pack8(four, inv, most) & 255);
                 }
             }
         }
@@ -367,7 +370,7 @@ __global__ __launch_bounds__(256) void append_few_kernel(AppendArgs a) {
         if (turned) turn(y, y + 8, co, si);
     };
     const int n = f.slot1 - f.slot0;
-    float y0[16], inv = 1.f;
+    float y0[16], inv = 1.f, most = 448.f;
     row_of(0, y0);
     if (EIGHT && !is_q) {
         float top = 0.f;
@@ -391,6 +394,7 @@ __global__ __launch_bounds__(256) void append_few_kernel(AppendArgs a) {
         }
         const Scale sc(top, was, f.slot0 > 0);
         inv = sc.inv;
+        most = sc.most;
         if (sc.moves) {
             if (is_v) move_values(a.values + page_head * page * D, f.slot0, D, sc.factor, l, kLanes);
             else move_keys(a.keys + page_head * page * D, f.slot0, D, sc.factor, l, kLanes);
@@ -411,7 +415,7 @@ __global__ __launch_bounds__(256) void append_few_kernel(AppendArgs a) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 if constexpr (EIGHT) {
-                    const uint32_t w = pack8(y + e, inv);
+                    const uint32_t w = pack8(y + e, inv, most);
 #pragma unroll
                     for (int j = 0; j < 4; j++) a.values[at16 + (e + j) * kBlock] = (char)(w >> 8 * j);
                 } else {
@@ -425,8 +429,8 @@ __global__ __launch_bounds__(256) void append_few_kernel(AppendArgs a) {
             *reinterpret_cast<u32x4*>(out + d2) = to_vector<T>(y + 8);
         } else {
             char* out = a.keys + (page_head * page + slot) * D;
-            *reinterpret_cast<u32x2*>(out + d1) = u32x2{pack8(y, inv), pack8(y + 4, inv)};
-            *reinterpret_cast<u32x2*>(out + d2) = u32x2{pack8(y + 8, inv), pack8(y + 12, inv)};
+            *reinterpret_cast<u32x2*>(out + d1) = u32x2{pack8(y, inv, most), pack8(y + 4, inv, most)};
+            *reinterpret_cast<u32x2*>(out + d2) = u32x2{pack8(y + 8, inv, most), pack8(y + 12, inv, most)};
         }
     }
 }

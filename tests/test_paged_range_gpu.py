@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.paged_util import E4M3, HostCache, assert_within, attention, attention_at_once, table_of
+from tests.paged_util import E4M3, HostCache, assert_within, attention, attention_at_once, half_step, table_of
 from tests.util import NAME
 
 pytestmark = pytest.mark.gpu
@@ -157,6 +157,26 @@ def test_many_small_weights_beside_a_large_one(new, eight, dtype):
         got = _attend(q, cache, table, [N] * B, starts, scale=1.0, is_causal=causal)
         want, bound = attention_at_once(q, cache, table, [N] * B, starts, scale=1.0, is_causal=causal)
         assert_within(got, want, bound, f"{new} {causal}")
+
+
+def test_bfloat16s_greatest_numbers_stay_finite():
+    """An append rounds 3.38e38 to what a scale of 2 ** 120 has below 2 ** 128, half a step away at most."""
+    from metalhlo_amd import kernels
+    big = torch.finfo(torch.bfloat16).max
+    for tokens in (1, 21):
+        c = kernels.paged_cache(2, 2, 16, 64, E4M3)
+        x = torch.full((tokens, 2, 64), big, dtype=torch.bfloat16, device="cuda")
+        x[:, :, ::2] *= -1
+        kernels.paged_append(c, x, x, ints([[0, 1]]), ints([tokens]), ints([0, tokens]))
+        held = [c.keys.float()[0, :, :1].double() * 2.0 ** (c.key_scales[0].double() - 127)[:, None, None],
+                c.values.float()[0, :, 0, :, :1].transpose(1, 2).double() * 2.0 ** (c.value_scales[0].double() - 127)[:, None, None]]
+        for h in held:
+            assert (h.abs() <= big).all() and ((h - x[0][:, None].double()).abs() <= 2.0 ** -4 * big).all()
+        if tokens > 1:                                          # (a sum of these is beyond fp32)
+            continue
+        got = kernels.paged_attention(torch.zeros(tokens, 2, 64, dtype=torch.bfloat16, device="cuda"), c, ints([[0, 1]]), ints([tokens]), ints([0, tokens]))
+        # one rounding of the result, and one of the weight
+        assert ((got.double() - held[1].transpose(0, 1)).abs() <= 1.01 * 2 * half_step(torch.bfloat16) * big).all()
 
 
 # ---------------------------------------------------------------- more keys than the table reaches
