@@ -219,3 +219,39 @@ def test_append_to_sequences_longer_than_their_table(lengths, new, width, eight,
         kernels.paged_append(c, k, v, ints(t), ints(lengths), ints(starts), q=q, freqs=freqs, out=out)
         results.append([out] + [held.view(torch.uint8) for held in c if held is not None])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+# ---------------------------------------------------------------- both, as a program uses them
+@HALF
+@pytest.mark.parametrize("prompts,H,KV,D,page", [([37, 1, 80], 8, 2, 64, 16), ([300, 150, 33], 4, 2, 128, 64), ([20, 5, 16], 6, 3, 96, 32)], ids=str)
+def test_attention_over_what_appends_have_left(prompts, H, KV, D, page, dtype):
+    """Prompts, pieces behind them and single tokens onto an 8-bit cache; every step's attention against the bytes and scales that are held then."""
+    from metalhlo_amd import kernels
+    rng = np.random.default_rng(D)
+    steps = [prompts, [1, 1, 1], [5, 0, 2], [1, 1, 1], [40, 3, 0], [1, 1, 1]]
+    table, pages = table_of([sum(s[b] for s in steps) for b in range(3)], page, rng)
+    c = kernels.paged_cache(pages, KV, page, D, E4M3)
+    freqs = torch.from_numpy(rng.standard_normal((500, D)).astype(np.float32)).cuda()
+    done = [0, 0, 0]
+    for i, new in enumerate(steps):
+        done = [a + b for a, b in zip(done, new)]
+        starts = [0] + list(np.cumsum(new))
+        q, k, v = (torch.from_numpy(rng.standard_normal((starts[-1], h, D)).astype(np.float32) * (1 + i)).to(dtype).cuda() for h in (H, KV, KV))
+        args = (ints(table), ints(done), ints(starts))
+        q = kernels.paged_append(c, k, v, *args, q=q, freqs=freqs)
+        got = kernels.paged_attention(q, c, *args, scale=0.02)
+        held = HostCache(pages, KV, page, D, dtype, True)
+        held.x = [c.keys.float().cpu(), c.values.float().cpu().transpose(3, 4).reshape(pages, KV, page, D)]
+        held.scales = [s.cpu() for s in c[2:]]
+        want, bound = attention(q.cpu(), held, table, done, starts, scale=0.02)
+        assert_within(got, want, bound, f"step {i}")
+
+
+@EIGHT
+@pytest.mark.parametrize("new,H", [(1, 40), (1, 200), (3, 200), (20, 300)])
+def test_more_query_heads_to_a_key_head_than_a_tile_has_rows(new, H, eight):
+    q, cache, table, keys, starts = _batch([new, new], [700, 2100], H, 1, 64, 16, torch.bfloat16, eight, seed=H)
+    for causal in (True, False):
+        got = _attend(q, cache, table, keys, starts, is_causal=causal)
+        want, bound = attention_at_once(q, cache, table, keys, starts, is_causal=causal)
+        assert_within(got, want, bound, f"{new} {H}")
