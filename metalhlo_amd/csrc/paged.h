@@ -34,6 +34,13 @@ struct Sequences {
     __device__ __forceinline__ int bounded_end(int b) const { return min(max(lengths[b], 0), reach() + tokens(b)); }
 };
 
+// Between what lanes of a wave write to LDS and what others of the same wave read of it, either way round.  The hardware serves a wave's accesses to LDS in order, so that nothing waits: this keeps
+// the compiler from another order, which may not know that the addresses meet.
+__device__ __forceinline__ void wave_in_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // sum over the lanes up to this one
 __device__ __forceinline__ int wave_scan(int v) {
     auto step = [&](auto ctrl, auto rows) __attribute__((always_inline)) {

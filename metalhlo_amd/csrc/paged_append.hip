@@ -275,9 +275,11 @@ __global__ __launch_bounds__(64 * WAVES) void paged_append_kernel(AppendArgs a) 
     for (int head = head0; head < head1; head++) {
         const int64_t page_head = page_head0 + head;
         const int was = EIGHT && s0 ? scales[page_head] : 0;
+        wave_in_order();                                                  // (the head before has been read)
 #pragma unroll
         for (int i = 0; i < kReads; i++)
             if (pr < kRead) *reinterpret_cast<u32x4*>(&turned_values[wave][i * kRead + pr][8 * pc]) = raw[i];
+        wave_in_order();
         if (head + 1 < head1) ask(head + 1);
         if constexpr (!EIGHT) {
             // in 16 bits a lane writes eight tokens of one d, its neighbour the other eight: a store of the wave is a kilobyte in one piece

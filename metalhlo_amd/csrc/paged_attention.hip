@@ -364,6 +364,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
             break;
         }
     }
+    wave_in_order();                                                         // (`known`)
     int g = line.begin(blockIdx.x);
     const int stop = min(line.begin(blockIdx.x + 1), steps);
     const int page_bytes = (D * SIZE) << a.s.page_shift;
@@ -761,6 +762,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_tile_kernel(PagedArgs a) 
 
     // ---- this workgroup's share of the line.  Eight neighbours of the launch, which are on eight XCDs, take shares an eighth of the line apart: what an XCD's workgroups read at a time belongs to few heads
     known_of(a.s, known[wave], lane);
+    wave_in_order();
     int longest = 1, shortest = 1 << 30, all = 0, count = 0;
     auto add = [&](int tokens, int keys) __attribute__((always_inline)) {
         const Stretch<ROWS> st(a, tokens, keys);
