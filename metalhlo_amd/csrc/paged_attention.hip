@@ -43,7 +43,7 @@ struct PagedArgs {
     const char *keys, *values;
     const uint8_t *key_scales, *value_scales;
     Sequences s;
-    int pages, KV, G, is_causal, shares;
+    int pages, KV, G, is_causal, shares, units;
     float c;                                  // |scale| * log2(e), a tiny number instead of 0 (which times -inf is none)
     uint32_t sign;                            // 0x80008000 where the scale is negative: of the queries
     int64_t qs[2], os[2];                     // token and head strides in elements
@@ -348,10 +348,15 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
     // Shares of a few steps: a share that is the end of one tile and the beginning of another costs two rounds of first loads and of joining.  Where stretches that are rounded up to l steps fit as many
     // shares of l, every workgroup has one part of one tile.  us, plain | rounded: 16 sequences of 2800 to 4000 keys (8 heads of 128, 8 bits) 32.4 | 27.9, 64 of them 85.4 | 79.0, with four tokens each 97 | 81,
     // 24 of 600 to 6000 42.3 | 37.0, 64 of 300 to 600 25.6 | 19.2, one of 30000 22.0 | 19.8; but 30 of 450 to 900, 12 heads of 64, 18.5 | 19.4.  More than 16 steps a share: level
-    // Where there is a share for every step, shares of two make half as many parts to join; four to eight steps are quicker in as many parts.  us, one | two: 4 sequences of 4000 keys 16.0 | 12.4, with
-    // four tokens each 20.0 | 14.4, one of 8000 11.8 | 11.6, 8 of 250 to 500, 2 heads of 96, 8.0 | 7.1; but one of 1000, 12 heads of 64, 7.8 | 8.3
+    // Where there is a share for every step, shares of two make half as many parts to join, and of two steps none; three to sixteen steps that a unit each takes are quicker in as many parts.
+    // us, one | two, 8 heads of 128 in 8 bits where nothing else is said:
+    //   no more steps than units   1000 keys 9.9 | 10.8, 2000 10.0 | 10.9, 4000 10.3 | 11.1; 12 heads of 64 1000 keys 8.3 | 8.9, 3000 8.4 | 9.1; 8 sequences of 1000 11.1 | 11.9, with four tokens each 12.8 | 13.5
+    //   longer ones                6000 keys 12.1 | 11.7, 8000 12.3 | 12.0; 2 heads of 96, 15000 12.3 | 11.0
+    //   more steps                 8 sequences of 1500 15.7 | 12.3, 16 of 1000 16.4 | 12.7, 4 of 4000 16.0 | 12.4; 10 of 1000, 12 heads of 64, 10.0 | 9.2; 8 of 1500 in 16 bits 16.1 | 14.7
+    //   two steps                  8 sequences of 250 to 500, 2 heads of 96, 8.0 | 7.1
     const bool ample = line.per == 1 && !line.more;
-    if (line.per <= 16 && !(ample && longest > 2 && longest <= 8) && a.s.B <= 64) {
+    const bool apart = ample && longest > 2 && longest <= 16 && steps <= a.units;
+    if (line.per <= 16 && !apart && a.s.B <= 64) {
         const int n = steps_of(known[wave].line[lane]), tiles = tiles_of(known[wave].tokens[lane]);
         for (int l = line.per + (ample || line.more ? 1 : 0), l1 = line.per + line.per / 4 + 1; l <= l1; l++) {
             const int of = (int)(((float)n + (float)l - 0.5f) / (float)l);       // n / l, rounded up (n and l below 2^16, l of a few)
@@ -1202,7 +1207,7 @@ extern "C" int mhip_paged_attention(void* stream, const mhip_paged_cache* cache,
     for (int i = 0; i < 4; i++)
         if (strides[i] % 8) return fail(MHIP_ERR_UNSUPPORTED, "paged_attention: strides must be multiples of 8 elements");
     PagedArgs a{q, o, (const char*)cache->keys, (const char*)cache->values, cache->key_scales, cache->value_scales, sequences(cache, seqs),
-                (int)cache->pages, (int)cache->heads, (int)(q_heads / cache->heads), is_causal ? 1 : 0, p.shares, scale == 0.f ? 1e-30f : std::fabs(scale) * kLog2e, std::signbit(scale) ? 0x80008000u : 0u, {strides[0], strides[1]}, {strides[2], strides[3]},
+                (int)cache->pages, (int)cache->heads, (int)(q_heads / cache->heads), is_causal ? 1 : 0, p.shares, compute_units(), scale == 0.f ? 1e-30f : std::fabs(scale) * kLog2e, std::signbit(scale) ? 0x80008000u : 0u, {strides[0], strides[1]}, {strides[2], strides[3]},
                 nullptr, nullptr, 0, Divider((uint32_t)(q_heads / cache->heads)), Divider((uint32_t)cache->heads), Divider((uint32_t)p.shares), p.unit_shift};
     if (workspace && workspace_bytes >= workspace_of(cache, p)) {
         a.part = static_cast<float*>(workspace);
