@@ -7,7 +7,8 @@
 //             where it grows by 2^n the held values are multiplied by 2^-n and rounded, which changes none that stays above 2^-6 of the new scale.
 //
 // Bound by memory: every new value is read once and written once.  9450 tokens of 32 query and 8 key heads of 128 in 8 bits (218 MB) 46 us, 4.7 TB/s, 32000 (737 MB)
-// 140 us, 5.3 TB/s; 6300 of 16 heads of 96 in 16 bits (92 MB) 20 us, 4.5 TB/s; a decode step of 48 sequences 5.5 us and of one 4.8, which is latency.  Two kernels:
+// 140 us, 5.3 TB/s; 6300 of 16 heads of 96 in 16 bits (92 MB) 20 us, 4.5 TB/s; a decode step of 48 sequences 5.6 us and of one 4.7, which is latency.
+// Where scales grow in a decode step, which of 48 sequences' 768 some nearly always do, the few lanes of a row move the page's held values: 25 to 84 us, and 67 where all grow.  Two kernels:
 //
 //   paged_append_kernel   A wave a block of sixteen tokens, a workgroup a page (a scale needs all of its tokens), with a few heads of keys, values or queries one behind the other: the cosines and sines stay in
 //                         registers from head to head, and the next head is on its way while this one's scale is found and its values are stored.  Values pass through LDS, which turns a block's rows into its columns.
