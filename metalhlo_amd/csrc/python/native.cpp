@@ -570,9 +570,11 @@ FUNCTION(paged_append) {
         } else if (arg[8] != Py_None) {
             raise(PyExc_ValueError, "out without queries");
         }
+        // a table of no positions has no memory; nothing is read of one, and every token lies outside
+        const float* table = freqs && freqs->size(0) == 0 ? static_cast<const float*>(cache.c.keys) : f32(freqs);
         const int dt = dtype_code(k.scalar_type());
         check([&] { return mhip_paged_append(stream_of(k), &cache.c, &seqs, k.data_ptr(), v.data_ptr(), q ? q->data_ptr() : nullptr, q ? out.data_ptr() : nullptr,
-                                             q ? q->size(1) : 0, f32(freqs), freqs ? freqs->size(0) : 0, freqs ? freqs->size(1) : 0, strides, dt); });
+                                             q ? q->size(1) : 0, table, freqs ? freqs->size(0) : 0, freqs ? freqs->size(1) : 0, strides, dt); });
         if (q) return THPVariable_Wrap(std::move(out));
         Py_RETURN_NONE;
     });

@@ -221,6 +221,21 @@ def test_append_to_sequences_longer_than_their_table(lengths, new, width, eight,
     assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
+@EIGHT
+@pytest.mark.parametrize("new", [1, 40])
+def test_freqs_without_positions(new, eight):
+    """Every token lies outside of them: none is stored, and no query turned."""
+    from metalhlo_amd import kernels
+    c = kernels.paged_cache(8, 2, 16, 64, E4M3 if eight else torch.bfloat16)
+    for held in c:
+        if held is not None:
+            held.view(torch.uint8).fill_(40)
+    k, q = torch.ones(2 * new, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(2 * new, 4, 64, dtype=torch.bfloat16, device="cuda")
+    out = torch.full_like(q, 7)
+    got = kernels.paged_append(c, k, k, ints(np.arange(8).reshape(2, 4)), ints([new + 3, new]), ints([0, new, 2 * new]), q=q, freqs=torch.empty(0, 32, device="cuda"), out=out)
+    assert got is out and (out == 7).all() and all((held.view(torch.uint8) == 40).all() for held in c if held is not None)
+
+
 # ---------------------------------------------------------------- both, as a program uses them
 @HALF
 @pytest.mark.parametrize("prompts,H,KV,D,page", [([37, 1, 80], 8, 2, 64, 16), ([300, 150, 33], 4, 2, 128, 64), ([20, 5, 16], 6, 3, 96, 32)], ids=str)
