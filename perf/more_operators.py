@@ -8,7 +8,8 @@
 `run` computes them in elementary torch operations in fp32, or with `own` by the calls of `metalhlo_amd.kernels`.  Both take the same memory:
 a cache of keys [pages, heads, page, D] and values [pages, heads, page / 16, D, 16], in 16 bits or as e4m3 with a scale 2 ** (byte - 127) a page and head; weights of keys
 [pages, heads, page] in fp32; 4-bit matrices [N, K] as words [N / 16, K / 128, 64, 4] (rounded up): lane l's word s holds row l % 16 of sixteen and the eight columns
-from 32 s + 8 (l / 16) on, column 2 i in bits 4 i, column 2 i + 1 in bits 16 + 4 i; scales [N / 16, K / group, 16, 2]: scale and zero of w = (q - zero) * scale.
+from 32 s + 8 (l / 16) on, of which byte i has column i in its low four bits and column i + 4 in its high ones; scales [N / 16, K / group, 16, 2]: scale and zero of
+w = (q - zero) * scale.
 """
 import torch
 
@@ -206,7 +207,7 @@ def _plain_linear(s):
     K, N, group = c["K"], c["N"], c["group"]
     w = s["packed"]
     N16, K128 = w.shape[:2]
-    shifts = torch.tensor([0, 16, 4, 20, 8, 24, 12, 28], dtype=torch.int32, device="cuda")
+    shifts = torch.tensor([0, 8, 16, 24, 4, 12, 20, 28], dtype=torch.int32, device="cuda")
     q = ((w[..., None] >> shifts) & 15).float()                                        # [N16, K128, 64, 4, 8]
     q = q.view(N16, K128, 4, 16, 4, 8).permute(0, 3, 1, 4, 2, 5).reshape(N16 * 16, K128 * 128 // group, group)
     sz = s["scales"].float().transpose(1, 2).reshape(N16 * 16, -1, 2)
@@ -397,7 +398,7 @@ def _exact_linear(s):
         for word in range(4):
             part = s["packed"][:, :, 16 * quarter:16 * quarter + 16, word]              # [N16, K128, 16]
             for e in range(8):
-                w[:, :, 32 * word + 8 * quarter + e::128] = ((part >> (4 * (e // 2) + 16 * (e % 2))) & 15).double().transpose(1, 2)
+                w[:, :, 32 * word + 8 * quarter + e::128] = ((part >> (8 * (e % 4) + 4 * (e // 4))) & 15).double().transpose(1, 2)
     w = w.view(-1, w.shape[2])[:N, :K]
     sz = s["scales"].double().transpose(1, 2).reshape(-1, s["scales"].shape[1], 2)[:N]
     of = torch.arange(K, device="cuda") // group
