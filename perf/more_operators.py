@@ -143,7 +143,7 @@ def prepare(case, seed):
         scales[:, -(-K // group):] = 0                           # behind the last column and the last row
         if N % 16:
             scales[-1, :, N % 16:] = 0
-        return dict(case=c, x=normal(rows, K), packed=packed, scales=scales, bias=normal(N, dtype=torch.float32) if c["bias"] else None,
+        return dict(case=c, x=normal(rows, K), packed=packed, scales=scales, bias=normal(N) if c["bias"] else None,
                     residual=normal(rows, N) if c["residual"] else None)
 
     lengths, new = _counts(c)
@@ -214,7 +214,7 @@ def _plain_linear(s):
     w = ((q - sz[..., 1:]) * sz[..., :1]).view(N16 * 16, K128 * 128)[:N, :K]
     y = torch.matmul(s["x"].float(), w.t())
     if s["bias"] is not None:
-        y = y + s["bias"]
+        y = y + s["bias"].float()
     if c["activation"] == "gelu":
         y = 0.5 * y * (1.0 + torch.tanh(0.7978845608028654 * (y + 0.044715 * y * y * y)))
     elif c["activation"] == "silu":
@@ -377,7 +377,7 @@ def work(case):
     c = case
     if c["kind"] == "linear":
         M, K, N = c["rows"], c["K"], c["N"]
-        return dict(bytes=N * K / 2 + 4.0 * N * -(-K // c["group"]) + 2.0 * M * (K + N * (2 if c["residual"] else 1)) + (4.0 * N if c["bias"] else 0.0), flops=2.0 * M * N * K)
+        return dict(bytes=N * K / 2 + 4.0 * N * -(-K // c["group"]) + 2.0 * M * (K + N * (2 if c["residual"] else 1)) + (2.0 * N if c["bias"] else 0.0), flops=2.0 * M * N * K)
     lengths, new = _counts(c)
     T, H, KV, D, held = sum(new), c["H"], c["KV"], c["D"], 1 if c["eight"] else 2
     if c["kind"] == "evict":
