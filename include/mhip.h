@@ -210,6 +210,27 @@ int mhip_attend_project_layer_ok(int64_t B, int64_t S, int64_t H, int64_t D, int
 int mhip_attend_project_layer(void* stream, const void* qkv, const float* w, const float* bias, const void* residual, void* c, int64_t B, int64_t S, int64_t H,
                               int64_t D, int64_t N, int dtype, int n_ahead, const mhip_weights* ahead);
 
+/* Weights in 4 bits: W [N, K], W[n][k] = (q - zero) * scale with q in 0 .. 15 and a scale and a zero for each n and `group` (32, 64 or 128) neighbouring k.
+ *   words   [ceil(N / 16)][ceil(K / 128)][64][4] 32-bit words: word s of lane l of block (t, b) holds row 16 t + l % 16 and columns 128 b + 32 s + 8 (l / 16) + 0 .. 7, column i (0 .. 3) in the low four
+ *           bits of byte i and column i + 4 in its high ones
+ *   scales  [ceil(N / 16)][128 / group * ceil(K / 128)][16][2]: scale and zero of row 16 t + i, BF16 or F16
+ * What lies behind N or K holds zeros (words there may hold anything).  16-byte aligned. */
+typedef struct {
+    const void* words;
+    const void* scales;
+    int64_t N, K, group;
+} mhip_w4;
+/* Writes `out`'s words and scales (dtype BF16 or F16) from w, whose element (n, k) is at n * stride_n + k * stride_k: F32, BF16 or F16, finite.  Of each group lo = min(w, 0) and hi = max(w, 0),
+ * scale = (hi - lo) / 15 rounded to dtype, zero = round(-lo / scale), q = round(w / scale) + zero within 0 .. 15. */
+int mhip_quantize_w4(void* stream, const void* w, int64_t stride_n, int64_t stride_k, const mhip_w4* out, int w_dtype, int dtype);
+/* c [M, N] = act(x [M, K] . W^T + bias) (+ residual [M, N]); x, scales, bias [N], residual and c of dtype BF16 or F16, bias and residual may be NULL.  fp32 sums of exact products and
+ * one rounding.  From 129 rows on W is rounded to dtype, once, in the workspace (mhip_linear_w4_workspace bytes, 0: of no use; 16-byte aligned, overwritten), and the product is
+ * mhip_gemm_residual's; with less, or none, it is not.  The last bits of a row may depend on the number of rows.
+ * The reference has no such layer (its matmul: Compiler/CodeGenerator.swift:4797-4850). */
+int64_t mhip_linear_w4_workspace(int64_t M, const mhip_w4* w, int dtype);
+int mhip_linear_w4(void* stream, const void* x, const mhip_w4* w, const void* bias, const void* residual, void* c, int64_t M, int activation, int dtype, void* workspace,
+                   int64_t workspace_bytes);
+
 /* Attention -------------------------------------------------------------- */
 
 /* O = softmax(scale * Q K^T + mask, causal) V.

@@ -1,0 +1,405 @@
+// Linear layers whose weights are held in 4 bits: C = act(x W^T + bias) (+ residual), W[n][k] = (q - z) s with a 4-bit q and, for each n and `group` neighbouring k,
+// a scale s and a zero z in the tensors' 16-bit type.
+//
+//   words   [N / 16][K / 128][64][4]   the operand of v_mfma_f32_16x16x32 as its lanes want it: lane l's word s holds row l % 16 of sixteen and the columns 32 s + 8 (l / 16) + 0 .. 7,
+//                                      column i and column i + 4 in the low and the high half of byte i.  A wave reads a kilobyte in one go, and a lane's sixteen bytes feed four products.
+//   scales  [N / 16][K / group][16]    pairs of scale and zero; a lane of the result holds four neighbouring rows, whose pairs are sixteen bytes
+// both rounded up to whole sixteens and 128s.
+//
+// A byte 0 .. 15 is that number times 2^-9 as e4m3, across the border of its subnormals: one v_cvt_scalef32_pk per two weights makes 16-bit numbers q, exactly, of bytes that a mask and a shift have made.
+// The products of q and x are added over a group in the matrix unit, and so is x itself (an operand of ones, so that each lane of the result has the sum of its own row): what a group
+// adds to a result is s (sum q x - z sum x), in fp32 and of numbers that are exact.
+//
+// Few rows: w4_rows_kernel, whose time is that of reading W.  Many: W is rounded to 16 bits into the workspace and multiplied by mhip_gemm (kManyRows).
+#include <algorithm>
+
+#include "gemm_common.h"
+
+namespace mhip {
+namespace {
+
+constexpr int kWaves = 8, kBlockK = 128;
+
+struct W4Args {
+    const void* x;
+    const u32x4* words;
+    const uint32_t* scales;           // pairs
+    const void *bias, *residual;
+    void* c;
+    int M, N, K, act;
+    int n16, k128;
+    int whole;                        // four columns of a row of C lie on 8 bytes, and so do the bias' and the residual's
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_rsrc(const void* p, uint32_t bytes) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000); }
+
+// the eight numbers of a word
+template <typename T>
+__device__ __forceinline__ u32x4 numbers(uint32_t w) {
+    const uint32_t low = w & 0x0F0F0F0Fu, high = (w >> 4) & 0x0F0F0F0Fu;
+    if constexpr (std::is_same<T, bf16_t>::value)
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(low, 512.f, false)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(low, 512.f, true)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(high, 512.f, false)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(high, 512.f, true))};
+    else
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(low, 512.f, false)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(low, 512.f, true)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(high, 512.f, false)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(high, 512.f, true))};
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (std::is_same<T, bf16_t>::value) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// the halves of a pair
+template <typename T>
+__device__ __forceinline__ float low_half(uint32_t w) { return Elem<T>::to_f32(__builtin_bit_cast(T, (uint16_t)w)); }
+template <typename T>
+__device__ __forceinline__ float high_half(uint32_t w) { return Elem<T>::to_f32(__builtin_bit_cast(T, (uint16_t)(w >> 16))); }
+
+// 16 NT columns of C and 16 MT rows a workgroup, whose waves split K by blocks of 128.  U blocks of a wave are on their way at a time.
+// EVEN: rows of x lie on 16 bytes; else x is read number by number.
+template <typename T, int GROUP, int MT, int NT, int U, bool EVEN>
+__global__ __launch_bounds__(64 * kWaves) void w4_rows_kernel(W4Args g) {
+    constexpr int kGroups = kBlockK / GROUP, kSteps = GROUP / 32;
+    __shared__ f32x4 sums[kWaves][NT * MT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & 15, lg = lane >> 4;
+    const int tile0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
+    const int rows = min(g.M - m0, 16 * MT);
+    const __amdgpu_buffer_rsrc_t rx = w4_rsrc(static_cast<const T*>(g.x) + (int64_t)m0 * g.K, (uint32_t)rows * (uint32_t)g.K * 2);
+
+    struct Block { u32x4 w[NT], scale[NT][kGroups], x[MT][4]; };
+    const u32x4* wp[NT];
+    const uint32_t* sp[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        const int64_t tile = min(tile0 + i, g.n16 - 1);
+        wp[i] = g.words + tile * g.k128 * 64 + lane;
+        sp[i] = g.scales + tile * g.k128 * (kGroups * 16) + 4 * lg;
+    }
+    uint32_t xo[MT];                                                       // (a row behind the last is the last again; nothing is stored of it)
+#pragma unroll
+    for (int i = 0; i < MT; i++) xo[i] = (uint32_t)min(16 * i + li, rows - 1) * (uint32_t)g.K * 2;
+
+    auto load = [&](Block& b, int kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            b.w[i] = __builtin_nontemporal_load(wp[i] + (int64_t)kb * 64);
+#pragma unroll
+            for (int j = 0; j < kGroups; j++) b.scale[i][j] = *reinterpret_cast<const u32x4*>(sp[i] + ((int64_t)kb * kGroups + j) * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const int k = kb * kBlockK + 32 * s + 8 * lg;
+                if constexpr (EVEN) {
+                    b.x[i][s] = __builtin_amdgcn_raw_buffer_load_b128(rx, k < g.K ? xo[i] + 2 * k : kOob, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t lo = __builtin_amdgcn_raw_buffer_load_b16(rx, k + 2 * e < g.K ? xo[i] + 2 * (k + 2 * e) : kOob, 0, 0);
+                        const uint32_t hi = __builtin_amdgcn_raw_buffer_load_b16(rx, k + 2 * e + 1 < g.K ? xo[i] + 2 * (k + 2 * e + 1) : kOob, 0, 0);
+                        b.x[i][s][e] = (lo & 0xFFFFu) | hi << 16;
+                    }
+                }
+            }
+    };
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const uint32_t one = std::is_same<T, bf16_t>::value ? 0x3F803F80u : 0x3C003C00u;
+    const u32x4 ones = {one, one, one, one};
+    auto multiply = [&](const Block& b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < kGroups; j++) {
+            f32x4 part[NT][MT], total[MT];
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                total[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < NT; i++) part[i][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int s = j * kSteps; s < (j + 1) * kSteps; s++) {
+#pragma unroll
+                for (int m = 0; m < MT; m++) total[m] = product<T>(ones, b.x[m][s], total[m]);
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    const u32x4 q = numbers<T>(b.w[i][s]);
+#pragma unroll
+                    for (int m = 0; m < MT; m++) part[i][m] = product<T>(q, b.x[m][s], part[i][m]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float scale = low_half<T>(b.scale[i][j][r]), zero = high_half<T>(b.scale[i][j][r]);
+#pragma unroll
+                    for (int m = 0; m < MT; m++) acc[i][m][r] = fmaf(scale, fmaf(-zero, total[m][r], part[i][m][r]), acc[i][m][r]);
+                }
+        }
+    };
+    Block blk[U];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (wave + u * kWaves < g.k128) load(blk[u], wave + u * kWaves);
+    for (int kb = wave; kb < g.k128; kb += U * kWaves) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (kb + u * kWaves >= g.k128) break;
+            multiply(blk[u]);
+            if (kb + (u + U) * kWaves < g.k128) load(blk[u], kb + (u + U) * kWaves);
+        }
+    }
+
+    // ---- the waves' sums, as their lanes hold them: lane (li, lg) has row li of C's sixteen and columns 4 lg .. 4 lg + 3
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int m = 0; m < MT; m++) sums[wave][i * MT + m][lane] = acc[i][m];
+    __syncthreads();
+    for (int t = wave; t < NT * MT; t += kWaves) {
+        f32x4 sum = sums[0][t][lane];
+#pragma unroll
+        for (int w = 1; w < kWaves; w++) sum += sums[w][t][lane];
+        const int row = 16 * (t % MT) + li, col = (tile0 + t / MT) * 16 + 4 * lg;
+        if (row >= rows || col >= g.N) continue;
+        const int64_t at = (int64_t)(m0 + row) * g.N + col;
+        T* c = static_cast<T*>(g.c) + at;
+        const T *res = static_cast<const T*>(g.residual) + at, *bias = static_cast<const T*>(g.bias) + col;
+        Pack4<T> o, r{}, b{};
+        const int n = min(g.N - col, 4);
+        if (g.whole) {
+            if (g.bias) b = *reinterpret_cast<const Pack4<T>*>(bias);
+            if (g.residual) r = *reinterpret_cast<const Pack4<T>*>(res);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (g.bias && e < n) b.v[e] = bias[e];
+                if (g.residual && e < n) r.v[e] = res[e];
+            }
+        }
+        dispatch_act(g.act, [&](auto act_tag) {
+            constexpr int ACT = decltype(act_tag)::value;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float y = apply_act_c<ACT>(g.bias ? sum[e] + Elem<T>::to_f32(b.v[e]) : sum[e]);
+                o.v[e] = Elem<T>::from_f32(g.residual ? y + Elem<T>::to_f32(r.v[e]) : y);
+            }
+        });
+        if (g.whole) {
+            *reinterpret_cast<Pack4<T>*>(c) = o;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (e < n) c[e] = o.v[e];
+        }
+    }
+}
+
+// W as 16-bit numbers [N][stride] (zeros behind K), each rounded once: a wave a kilobyte of words.
+template <typename T, int GROUP>
+__global__ __launch_bounds__(256) void w4_widen_kernel(const u32x4* words, const uint32_t* scales, T* out, int N, int K, int n16, int k128, int stride) {
+    constexpr int kGroups = kBlockK / GROUP;
+    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    for (int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); unit < (int64_t)n16 * k128; unit += (int64_t)gridDim.x * 4) {
+        const int tile = (int)(unit / k128), kb = (int)(unit - (int64_t)tile * k128), n = tile * 16 + li;
+        const u32x4 w = __builtin_nontemporal_load(words + unit * 64 + lane);
+        if (n >= N) continue;
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const int k = kb * kBlockK + 32 * s + 8 * lg;
+            const uint32_t pair = scales[(unit * kGroups + 32 * s / GROUP) * 16 + li];
+            const float scale = low_half<T>(pair), zero = high_half<T>(pair);
+            if (k >= stride) continue;
+            Vec16<T> v;
+#pragma unroll
+            for (int e = 0; e < 8; e++) v.v[e] = Elem<T>::from_f32(k + e < K ? ((float)((w[s] >> (8 * (e & 3) + 4 * (e >> 2))) & 15) - zero) * scale : 0.f);
+            store16(out + (int64_t)n * stride + k, v);
+        }
+    }
+}
+
+// x [M][K] with rows of `stride` (zeros behind K)
+__global__ __launch_bounds__(256) void w4_pad_kernel(const uint16_t* x, uint16_t* out, int64_t all, int K, int stride) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / stride;
+        const int k = (int)(i - row * stride);
+        out[i] = k < K ? x[row * K + k] : 0;
+    }
+}
+
+// The words, scales and zeros of a matrix: of each group lo = min(w, 0) and hi = max(w, 0), s = (hi - lo) / 15 rounded to T, z = round(-lo / s), q = round(w / s) + z within 0 .. 15, so that
+// zero is held exactly and the ends of the range to half a step.  A wave a kilobyte of words: lane l has the 32 weights that its words will hold.
+template <typename S, typename T, int GROUP>
+__global__ __launch_bounds__(256) void w4_quantize_kernel(const S* w, int64_t stride_n, int64_t stride_k, u32x4* words, uint32_t* scales, int N, int K, int n16, int k128) {
+    constexpr int kGroups = kBlockK / GROUP, kSteps = GROUP / 32;
+    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    const float most = std::is_same<T, bf16_t>::value ? 0x1.FEp127f : 65504.f;
+    for (int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); unit < (int64_t)n16 * k128; unit += (int64_t)gridDim.x * 4) {
+        const int tile = (int)(unit / k128), kb = (int)(unit - (int64_t)tile * k128), n = tile * 16 + li;
+        u32x4 out;
+#pragma unroll
+        for (int j = 0; j < kGroups; j++) {
+            float v[kSteps][8], lo = 0.f, hi = 0.f;
+#pragma unroll
+            for (int s = 0; s < kSteps; s++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int k = kb * kBlockK + 32 * (j * kSteps + s) + 8 * lg + e;
+                    v[s][e] = n < N && k < K ? Elem<S>::to_f32(w[n * stride_n + k * stride_k]) : 0.f;
+                    lo = fminf(lo, v[s][e]);
+                    hi = fmaxf(hi, v[s][e]);
+                }
+            lo = fminf(lo, __shfl_xor(lo, 16, 64));
+            hi = fmaxf(hi, __shfl_xor(hi, 16, 64));
+            lo = fminf(lo, __shfl_xor(lo, 32, 64));
+            hi = fmaxf(hi, __shfl_xor(hi, 32, 64));
+            const T held = Elem<T>::from_f32(fminf(hi / 15.f - lo / 15.f, most));
+            const float scale = Elem<T>::to_f32(held), zero = scale > 0.f ? fminf(rintf(-lo / scale), 15.f) : 0.f;
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
+                uint32_t word = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float q = scale > 0.f ? fminf(fmaxf(rintf(v[s][e] / scale) + zero, 0.f), 15.f) : 0.f;
+                    word |= (uint32_t)q << (8 * (e & 3) + 4 * (e >> 2));
+                }
+                out[j * kSteps + s] = word;
+            }
+            if (lg == 0)
+                scales[(unit * kGroups + j) * 16 + li] = (uint32_t)__builtin_bit_cast(uint16_t, held) | (uint32_t)__builtin_bit_cast(uint16_t, Elem<T>::from_f32(zero)) << 16;
+        }
+        words[unit * 64 + lane] = out;
+    }
+}
+
+// Rows from which on W is widened in front of a product.
+constexpr int64_t kManyRows = 129;
+
+int check_w4(const char* what, const mhip_w4* w, int dtype) {
+    if (!w) return fail(MHIP_ERR_INVALID_ARGUMENT, "%s: NULL weights", what);
+    if (w->N < 0 || w->K < 0) return fail(MHIP_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+    if (w->group != 32 && w->group != 64 && w->group != 128) return fail(MHIP_ERR_UNSUPPORTED, "%s: groups of %lld columns (need 32, 64 or 128)", what, (long long)w->group);
+    if (dtype != MHIP_BF16 && dtype != MHIP_F16) return fail(MHIP_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
+    if (w->N > (1 << 24) || w->K > (1 << 22)) return fail(MHIP_ERR_UNSUPPORTED, "%s: more than 2^24 rows or 2^22 columns", what);
+    return MHIP_OK;
+}
+
+// (workgroups of 256; the kernels go on where there is more)
+int64_t blocks_for(int64_t n) { return std::min<int64_t>(n, 1 << 20); }
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// The widened W, a copy of x where its rows are off 16 bytes, and what the product itself can use.
+struct Wide { int64_t stride, w, x, gemm; };
+Wide wide_of(int64_t M, const mhip_w4* w, bool even, int dtype) {
+    Wide r{};
+    r.stride = even ? w->K : up(w->K, 64);
+    r.w = up(w->N * r.stride * 2, 256);
+    r.x = even ? 0 : up(M * r.stride * 2, 256);
+    r.gemm = mhip_gemm_workspace(M, w->N, r.stride, 1, 0, 1, dtype);
+    return r;
+}
+
+template <typename T, int GROUP, int MT, int NT, int U>
+int launch_rows(hipStream_t st, const W4Args& a, bool even) {
+    const dim3 grid((unsigned)((a.n16 + NT - 1) / NT), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
+    if (even) hipLaunchKernelGGL((w4_rows_kernel<T, GROUP, MT, NT, U, true>), grid, dim3(64 * kWaves), 0, st, a);
+    else hipLaunchKernelGGL((w4_rows_kernel<T, GROUP, MT, NT, 1, false>), grid, dim3(64 * kWaves), 0, st, a);
+    return check_launch("linear_w4");
+}
+
+template <typename T, int GROUP>
+int launch_group(hipStream_t st, const W4Args& a, bool even) {
+    if (a.M <= 16) return launch_rows<T, GROUP, 1, 1, 4>(st, a, even);
+    if (a.M <= 32) return launch_rows<T, GROUP, 2, 1, 2>(st, a, even);
+    return launch_rows<T, GROUP, 4, 1, 1>(st, a, even);
+}
+
+template <typename F>
+int by_group(int64_t group, F&& f) {
+    if (group == 32) return f(std::integral_constant<int, 32>{});
+    if (group == 64) return f(std::integral_constant<int, 64>{});
+    return f(std::integral_constant<int, 128>{});
+}
+
+template <typename T>
+int run_w4(hipStream_t st, const W4Args& a, const mhip_w4* w, int dtype, void* workspace, int64_t bytes) {
+    const bool even = !((w->K & 7) || ((uintptr_t)a.x & 15));
+    if (a.M >= kManyRows && workspace) {
+        const Wide wide = wide_of(a.M, w, even, dtype);
+        if (bytes >= wide.w + wide.x) {
+            char* room = static_cast<char*>(workspace);
+            T* wt = reinterpret_cast<T*>(room);
+            const unsigned units = (unsigned)blocks_for(((int64_t)a.n16 * a.k128 + 3) / 4);
+            const int rc = by_group(w->group, [&](auto group) {
+                hipLaunchKernelGGL((w4_widen_kernel<T, decltype(group)::value>), dim3(units), dim3(256), 0, st, a.words, a.scales, wt, a.N, a.K, a.n16, a.k128, (int)wide.stride);
+                return check_launch("linear_w4");
+            });
+            if (rc) return rc;
+            const void* x = a.x;
+            if (!even) {
+                x = room + wide.w;
+                const int64_t all = a.M * wide.stride;
+                hipLaunchKernelGGL(w4_pad_kernel, dim3((unsigned)blocks_for((all + 255) / 256)), dim3(256), 0, st, static_cast<const uint16_t*>(a.x), reinterpret_cast<uint16_t*>(room + wide.w), all, a.K, (int)wide.stride);
+                if (const int rc2 = check_launch("linear_w4")) return rc2;
+            }
+            const int64_t left = bytes - wide.w - wide.x;
+            return mhip_gemm_ws(st, x, wt, a.bias, a.residual, a.c, a.M, a.N, wide.stride, 1, 0, 0, (int64_t)a.M * a.N, 0, 1, a.act, dtype, left > 0 ? room + wide.w + wide.x : nullptr, left);
+        }
+    }
+    return by_group(w->group, [&](auto group) { return launch_group<T, decltype(group)::value>(st, a, even); });
+}
+
+}  // namespace
+}  // namespace mhip
+
+using namespace mhip;
+
+extern "C" int mhip_quantize_w4(void* stream, const void* w, int64_t stride_n, int64_t stride_k, const mhip_w4* out, int w_dtype, int dtype) {
+    if (const int rc = check_w4("quantize_w4", out, dtype)) return rc;
+    if (w_dtype != MHIP_F32 && w_dtype != MHIP_BF16 && w_dtype != MHIP_F16) return fail(MHIP_ERR_UNSUPPORTED, "quantize_w4: weights of dtype %d", w_dtype);
+    if (out->N == 0 || out->K == 0) return MHIP_OK;
+    if (!w || !out->words || !out->scales) return fail(MHIP_ERR_INVALID_ARGUMENT, "quantize_w4: NULL tensor");
+    if (((uintptr_t)out->words | (uintptr_t)out->scales) & 15) return fail(MHIP_ERR_UNSUPPORTED, "quantize_w4: words and scales must be 16-byte aligned");
+    const int n16 = (int)((out->N + 15) / 16), k128 = (int)((out->K + 127) / 128);
+    const int64_t blocks = blocks_for(((int64_t)n16 * k128 + 3) / 4);
+    auto go = [&](auto source, auto type) {
+        using S = decltype(source);
+        using T = decltype(type);
+        return by_group(out->group, [&](auto group) {
+            hipLaunchKernelGGL((w4_quantize_kernel<S, T, decltype(group)::value>), dim3((unsigned)blocks), dim3(256), 0, as_stream(stream), static_cast<const S*>(w), stride_n, stride_k,
+                               static_cast<u32x4*>(const_cast<void*>(out->words)), static_cast<uint32_t*>(const_cast<void*>(out->scales)), (int)out->N, (int)out->K, n16, k128);
+            return check_launch("quantize_w4");
+        });
+    };
+    auto with = [&](auto type) { return w_dtype == MHIP_F32 ? go(float{}, type) : w_dtype == MHIP_BF16 ? go(bf16_t{}, type) : go(f16_t{}, type); };
+    return dtype == MHIP_BF16 ? with(bf16_t{}) : with(f16_t{});
+}
+
+extern "C" int64_t mhip_linear_w4_workspace(int64_t M, const mhip_w4* w, int dtype) {
+    if (M < kManyRows || check_w4("linear_w4_workspace", w, dtype) || w->N == 0 || w->K == 0) return 0;
+    const Wide even = wide_of(M, w, true, dtype), odd = wide_of(M, w, false, dtype);
+    // (whether x lies on 16 bytes is not known here)
+    return w->K & 7 ? odd.w + odd.x + odd.gemm : std::max(even.w + even.gemm, odd.w + odd.x + odd.gemm);
+}
+
+extern "C" int mhip_linear_w4(void* stream, const void* x, const mhip_w4* w, const void* bias, const void* residual, void* c, int64_t M, int activation, int dtype, void* workspace,
+                              int64_t workspace_bytes) {
+    if (const int rc = check_w4("linear_w4", w, dtype)) return rc;
+    if (M < 0) return fail(MHIP_ERR_INVALID_ARGUMENT, "linear_w4: negative size");
+    if (activation < MHIP_ACT_NONE || activation > MHIP_ACT_GELU_ERF) return fail(MHIP_ERR_INVALID_ARGUMENT, "linear_w4: activation %d", activation);
+    if (M > (1 << 21)) return fail(MHIP_ERR_UNSUPPORTED, "linear_w4: more than 2^21 rows");
+    if (M == 0 || w->N == 0) return MHIP_OK;
+    if (w->K == 0) return fail(MHIP_ERR_UNSUPPORTED, "linear_w4: rows of no columns");
+    if (!x || !w->words || !w->scales || !c) return fail(MHIP_ERR_INVALID_ARGUMENT, "linear_w4: NULL tensor");
+    if (((uintptr_t)w->words | (uintptr_t)w->scales | (uintptr_t)workspace) & 15) return fail(MHIP_ERR_UNSUPPORTED, "linear_w4: words, scales and workspace must be 16-byte aligned");
+    const W4Args a{x, static_cast<const u32x4*>(w->words), static_cast<const uint32_t*>(w->scales), bias, residual, c, (int)M, (int)w->N, (int)w->K, activation,
+                   (int)((w->N + 15) / 16), (int)((w->K + 127) / 128), !(w->N & 3) && !(((uintptr_t)c | (uintptr_t)bias | (uintptr_t)residual) & 7)};
+    return dtype == MHIP_BF16 ? run_w4<bf16_t>(as_stream(stream), a, w, dtype, workspace, workspace_bytes) : run_w4<f16_t>(as_stream(stream), a, w, dtype, workspace, workspace_bytes);
+}

@@ -645,6 +645,74 @@ FUNCTION(token_log_probs) {
     });
 }
 
+// ---- weights in 4 bits
+
+// (words, scales, N, K, group) of a W4
+mhip_w4 w4_of(PyObject* o, at::ScalarType type) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 5) raise(PyExc_TypeError, "expected a W4");
+    const at::Tensor &words = dense(PyTuple_GET_ITEM(o, 0)), &scales = dense(PyTuple_GET_ITEM(o, 1));
+    const int64_t N = integer(PyTuple_GET_ITEM(o, 2)), K = integer(PyTuple_GET_ITEM(o, 3)), group = integer(PyTuple_GET_ITEM(o, 4));
+    if (N < 0 || K < 0 || N > INT32_MAX || K > INT32_MAX || (group != 32 && group != 64 && group != 128)) raise(PyExc_ValueError, "a W4 has N rows of K columns in groups of 32, 64 or 128");
+    const int64_t n16 = (N + 15) / 16, k128 = (K + 127) / 128;
+    if (words.scalar_type() != at::kInt || words.sizes() != at::IntArrayRef({n16, k128, 64, 4})) raise(PyExc_ValueError, "words must be int32 [N / 16, K / 128, 64, 4], rounded up");
+    if (scales.sizes() != at::IntArrayRef({n16, k128 * (128 / group), 16, 2})) raise(PyExc_ValueError, "scales must be [N / 16, K / group, 16, 2], rounded up to whole 128s of K");
+    if (scales.scalar_type() != type) raise(PyExc_TypeError, "scales must be of x's type");
+    on_current_device(words);
+    on_current_device(scales);
+    return {words.data_ptr(), scales.data_ptr(), N, K, group};
+}
+
+// quantize_w4(weight, group, dtype code, trans_b) -> (words, scales, N, K, group)
+FUNCTION(quantize_w4) {
+    return guarded(n, 4, [&] {
+        const at::Tensor& w = tensor(arg[0]);
+        on_current_device(w);
+        const int64_t group = integer(arg[1]), dt = integer(arg[2]);
+        const bool trans = truth(arg[3]);
+        if (w.dim() != 2) raise(PyExc_ValueError, "weight must be a matrix");
+        if (group != 32 && group != 64 && group != 128) raise(PyExc_ValueError, "groups are of 32, 64 or 128 columns");
+        if (dt != MHIP_BF16 && dt != MHIP_F16) raise(PyExc_TypeError, "scales are bfloat16 or float16");
+        const int64_t N = w.size(trans ? 0 : 1), K = w.size(trans ? 1 : 0), n16 = (N + 15) / 16, k128 = (K + 127) / 128;
+        const int wt = dtype_code(w.scalar_type());
+        at::Tensor words = empty({n16, k128, 64, 4}, at::kInt, w), scales = empty({n16, k128 * (128 / group), 16, 2}, dt == MHIP_BF16 ? at::kBFloat16 : at::kHalf, w);
+        const mhip_w4 out{words.data_ptr(), scales.data_ptr(), N, K, group};
+        check([&] { return mhip_quantize_w4(stream_of(w), w.data_ptr(), w.stride(trans ? 0 : 1), w.stride(trans ? 1 : 0), &out, wt, (int)dt); });
+        PyObject *a = THPVariable_Wrap(std::move(words)), *b = THPVariable_Wrap(std::move(scales));
+        PyObject* r = a && b ? Py_BuildValue("(OOLLL)", a, b, (long long)N, (long long)K, (long long)group) : nullptr;
+        Py_XDECREF(a);
+        Py_XDECREF(b);
+        return r;
+    });
+}
+
+// linear_w4(x, W4, bias, residual, activation code) -> [.., N]
+FUNCTION(linear_w4) {
+    return guarded(n, 5, [&] {
+        const at::Tensor& x = dense(arg[0]);
+        on_current_device(x);
+        const int dt = dtype_code(x.scalar_type()), act = (int)integer(arg[4]);
+        if (dt != MHIP_BF16 && dt != MHIP_F16) raise(PyExc_TypeError, "linear_w4 needs bfloat16 or float16 tensors");
+        const mhip_w4 w = w4_of(arg[1], x.scalar_type());
+        const at::Tensor *bias = optional_dense(arg[2]), *res = optional_dense(arg[3]);
+        if (x.dim() < 1 || x.size(-1) != w.K || w.K == 0) raise(PyExc_ValueError, "x must be [.., K]");
+        c10::SmallVector<int64_t, 8> shape(x.sizes().begin(), x.sizes().end());
+        shape.back() = w.N;
+        for (const at::Tensor* t : {bias, res})
+            if (t) {
+                on_current_device(*t);
+                if (t->scalar_type() != x.scalar_type()) raise(PyExc_TypeError, "bias and residual must be of x's type");
+            }
+        if (bias && (bias->dim() != 1 || bias->size(0) != w.N)) raise(PyExc_ValueError, "bias must be [N]");
+        const int64_t M = x.numel() / w.K;
+        if (res && res->sizes() != at::IntArrayRef(shape)) raise(PyExc_ValueError, "residual must have the result's shape");
+        at::Tensor c = empty(shape, x.scalar_type(), x);
+        const at::Tensor work = workspace(mhip_linear_w4_workspace(M, &w, dt), x);
+        check([&] { return mhip_linear_w4(stream_of(x), x.data_ptr(), &w, ptr(bias), ptr(res), c.data_ptr(), M, act, dt, work.defined() ? work.data_ptr() : nullptr,
+                                          work.defined() ? work.numel() : 0); });
+        return THPVariable_Wrap(std::move(c));
+    });
+}
+
 // argmax(x, 64-bit indices?, with values?)
 FUNCTION(argmax) {
     return guarded(n, 3, [&]() -> PyObject* {
@@ -677,7 +745,7 @@ FUNCTION(bind) {
 
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {ENTRY(softmax), ENTRY(layer_norm), ENTRY(rms_norm), ENTRY(bias_gelu), ENTRY(matmul), ENTRY(linear), ENTRY(linear_layer), ENTRY(matmul_sums), ENTRY(tied_head), ENTRY(finish_norm), ENTRY(causal_attention), ENTRY(attend_project), ENTRY(attend_project_layer),
-                          ENTRY(flash_attention), ENTRY(argmax), ENTRY(paged_append), ENTRY(paged_attention), ENTRY(token_log_probs),
+                          ENTRY(flash_attention), ENTRY(argmax), ENTRY(paged_append), ENTRY(paged_attention), ENTRY(token_log_probs), ENTRY(quantize_w4), ENTRY(linear_w4),
                           ENTRY(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -138,6 +138,27 @@ def tied_head_served(M: int, N: int, K: int, dtype) -> bool:
     return bool(_lib.load().mhip_tied_head_ok(M, N, K, DTYPE_CODE[dtype]))
 
 
+class W4(NamedTuple):
+    """A matrix [N, K] in 4 bits, W[n][k] = (q - zero) * scale with a scale and a zero for each n and `group` (32, 64 or 128) neighbouring k: `words` int32 [ceil(N / 16), ceil(K / 128), 64, 4], lane l's
+    word s of a block holding row l % 16 of sixteen and the eight columns from 32 s + 8 (l / 16) on, column i in the low and column i + 4 in the high bits of byte i; `scales`
+    [ceil(N / 16), 128 / group * ceil(K / 128), 16, 2] (scale, zero) in bfloat16 or float16.  What lies behind N and K has scale and zero 0."""
+    words: torch.Tensor
+    scales: torch.Tensor
+    N: int
+    K: int
+    group: int
+
+
+def quantize_w4(weight, group: int = 128, dtype=torch.bfloat16, trans_b: bool = False) -> W4:
+    """weight [K, N], or [N, K] with trans_b, of any strides in fp32 or 16 bits (finite) as a W4 with scales in `dtype`: a group's range, zero included, in fifteen steps."""
+    return W4(*(_native or _host()).quantize_w4(weight, group, DTYPE_CODE[dtype], trans_b))
+
+
+def linear_w4(x, weight: W4, bias=None, activation: str = "none", residual=None):
+    """act(x [.., K] @ W^T + bias) (+ residual) with W in 4 bits; x, scales, bias and residual of one 16-bit type.  The last bits of a row may depend on how many there are."""
+    return (_native or _host()).linear_w4(x, weight, bias, residual, ACTIVATION_CODE[activation])
+
+
 def matmul_sums(a, b, parts: int):
     """The fp32 sums of so many shares of K of a [M, K] @ b [K, N] in a 16-bit type: [parts, M, N], for finish_norm."""
     return (_native or _host()).matmul_sums(a, b, parts)
