@@ -332,6 +332,16 @@ int64_t mhip_paged_attention_workspace(const mhip_paged_cache* cache, const mhip
 int mhip_paged_attention(void* stream, const mhip_paged_cache* cache, const mhip_sequences* seqs, const void* q, void* o, int64_t q_heads, float scale,
                          int is_causal, const int64_t* strides, int dtype, void* workspace, int64_t workspace_bytes);
 
+/* Eviction: of each sequence and head the last `recent` of its keys stay, and of those in front of them the `keep` of greatest weight (weights [pages, heads, page_size] in fp32; of equal ones the
+ * first, NaN above all); positions that the table names no page for hold none.  What stays moves to the front in its order, keys, values and weights: to the pages of `into` [sequences, into_width],
+ * which holds min(keep + recent, width * page_size) keys at least and whose pages the call reads nothing from, or with NULL within the sequence's own.  left [sequences] (not lengths) gets how
+ * many they are: the new lengths.  Slots behind the last one stay as they were.  A place whose page is none of the cache's takes no key.  8 bits: a page that takes keys gets the greatest of
+ * the scales of the pages they come from, under which values are rounded anew.  seqs: table, lengths, sequences and width are used.  In place pages belong to one sequence; keys that are rotated stay so.
+ * The workspace is needed: mhip_paged_evict_workspace says how much is of use and, in `least`, what suffices; 16-byte aligned, overwritten. */
+int64_t mhip_paged_evict_workspace(const mhip_paged_cache* cache, const mhip_sequences* seqs, int64_t keep, int64_t recent, int in_place, int64_t* least);
+int mhip_paged_evict(void* stream, const mhip_paged_cache* cache, const mhip_sequences* seqs, float* weights, int64_t keep, int64_t recent, const int32_t* into, int64_t into_width,
+                     int32_t* left, void* workspace, int64_t workspace_bytes);
+
 /* Of each row of logits [rows, vocab]: the log probability of tokens[row] (NaN for one outside [0, vocab)), the distribution's entropy in nats (may be NULL), and
  * its `top` most likely tokens (up to 64; 0: none, NULL) with their log probabilities [rows, top], the most likely first and the lowest index among equals.  A -inf logit has
  * probability zero; a row that holds a NaN or +inf, or nothing but -inf, yields NaN log probabilities and entropy, and its alternatives in the order of its

@@ -77,7 +77,25 @@ __device__ __forceinline__ int sequence_of(int B, int u, F units, int& first) {
 // 2^(byte - 127); the byte 0, which no append writes, as 1
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __builtin_bit_cast(float, max(byte, 1u) << 23); }
 
-// What the two entry points ask of a cache and of sequences before anything is planned or launched: their sizes, and then what they point to.
+// four e4m3 of x * inv, of `most` at most where that is finite; e4m3 has no infinities, so what is not finite becomes NaN
+__device__ __forceinline__ uint32_t pack8(const float* x, float inv, float most) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        y[e] = x[e] * inv;
+        y[e] = fabsf(y[e]) <= 448.f ? __builtin_amdgcn_fmed3f(y[e], -most, most) : __builtin_nanf("");
+    }
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+}
+// the held values of four tokens or d under the grown scale
+__device__ __forceinline__ uint32_t moved8(uint32_t w, float factor) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    const float x[4] = {lo[0], lo[1], hi[0], hi[1]};
+    return pack8(x, factor, 448.f);
+}
+
+// What the entry points ask of a cache and of sequences before anything is planned or launched: their sizes, and then what they point to.
 int check_sizes(const char* what, const mhip_paged_cache* c, const mhip_sequences* s);
 int check_paged(const char* what, const mhip_paged_cache* c, const mhip_sequences* s, int dtype, bool* empty);
 

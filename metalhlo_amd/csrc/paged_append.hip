@@ -43,23 +43,6 @@ __device__ __forceinline__ u32x4 to_vector(const float* x) {
     for (int e = 0; e < 8; e++) t.v[e] = Elem<T>::from_f32(x[e]);
     return __builtin_bit_cast(u32x4, t);
 }
-// four e4m3 of x * inv, of `most` at most where that is finite; e4m3 has no infinities, so what is not finite becomes NaN
-__device__ __forceinline__ uint32_t pack8(const float* x, float inv, float most) {
-    float y[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        y[e] = x[e] * inv;
-        y[e] = fabsf(y[e]) <= 448.f ? __builtin_amdgcn_fmed3f(y[e], -most, most) : __builtin_nanf("");
-    }
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
-}
-// the held values of four tokens or d under the grown scale
-__device__ __forceinline__ uint32_t moved8(uint32_t w, float factor) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-    const float x[4] = {lo[0], lo[1], hi[0], hi[1]};
-    return pack8(x, factor, 448.f);
-}
 __device__ __forceinline__ float finite_max(float m, float x) { return fmaxf(m, fabsf(x) < INFINITY ? fabsf(x) : 0.f); }
 
 // The exponent byte of the least scale of at least 2^-126 with amax <= 448 * scale (448 = 1.75 * 2^8).

@@ -609,6 +609,44 @@ FUNCTION(paged_attention) {
     });
 }
 
+// weights of keys: fp32 [pages, heads, page]
+float* key_weights(PyObject* o, const Cache& cache) {
+    const at::Tensor& w = dense(o);
+    on_current_device(w);
+    if (w.scalar_type() != at::kFloat) raise(PyExc_TypeError, "weights must be fp32");
+    if (w.sizes() != at::IntArrayRef({cache.c.pages, cache.c.heads, cache.c.page_size})) raise(PyExc_ValueError, "weights must be [pages, heads, page]");
+    return w.data_ptr<float>();
+}
+
+// paged_evict(cache, weights, table, lengths, keep, recent, into or None) -> new lengths
+FUNCTION(paged_evict) {
+    return guarded(n, 7, [&] {
+        const Cache cache = cache_of(arg[0]);
+        float* weights = key_weights(arg[1], cache);
+        const at::Tensor &table = dense(arg[2]), &lengths = dense(arg[3]);
+        const int64_t keep = integer(arg[4]), recent = integer(arg[5]);
+        const at::Tensor* into = optional_dense(arg[6]);
+        for (const at::Tensor* t : {&table, &lengths, into})
+            if (t) {
+                on_current_device(*t);
+                if (t->scalar_type() != at::kInt) raise(PyExc_TypeError, "table, lengths and into must be int32");
+            }
+        if (table.dim() != 2 || lengths.dim() != 1 || lengths.size(0) != table.size(0)) raise(PyExc_ValueError, "table must be [sequences, width] and lengths [sequences]");
+        if (into && (into->dim() != 2 || into->size(0) != table.size(0))) raise(PyExc_ValueError, "into must be [sequences, width]");
+        if (keep < 0 || recent < 0) raise(PyExc_ValueError, "keys to keep are negative");
+        if (into && into->size(1) * cache.c.page_size < std::min(keep + recent, table.size(1) * cache.c.page_size)) raise(PyExc_ValueError, "into has no room for what stays");
+        const mhip_sequences seqs{table.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), nullptr, table.size(0), table.size(1), 0};
+        at::Tensor left = empty({table.size(0)}, at::kInt, table);
+        int64_t least = 0;
+        const int64_t bytes = mhip_paged_evict_workspace(&cache.c, &seqs, keep, recent, into == nullptr, &least);
+        at::Tensor work = workspace(bytes, table);
+        if (!work.defined() && least > 0) work = empty({least}, at::kByte, table);        // (without room for the list there is no answer)
+        check([&] { return mhip_paged_evict(stream_of(table), &cache.c, &seqs, weights, keep, recent, into ? into->data_ptr<int32_t>() : nullptr, into ? into->size(1) : 0, left.data_ptr<int32_t>(),
+                                            work.defined() ? work.data_ptr() : nullptr, work.defined() ? work.numel() : 0); });
+        return THPVariable_Wrap(std::move(left));
+    });
+}
+
 // token_log_probs(logits, tokens, top) -> (log probabilities, entropy[, top log probabilities, top ids])
 FUNCTION(token_log_probs) {
     return guarded(n, 3, [&] {
@@ -745,7 +783,7 @@ FUNCTION(bind) {
 
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {ENTRY(softmax), ENTRY(layer_norm), ENTRY(rms_norm), ENTRY(bias_gelu), ENTRY(matmul), ENTRY(linear), ENTRY(linear_layer), ENTRY(matmul_sums), ENTRY(tied_head), ENTRY(finish_norm), ENTRY(causal_attention), ENTRY(attend_project), ENTRY(attend_project_layer),
-                          ENTRY(flash_attention), ENTRY(argmax), ENTRY(paged_append), ENTRY(paged_attention), ENTRY(token_log_probs), ENTRY(quantize_w4), ENTRY(linear_w4),
+                          ENTRY(flash_attention), ENTRY(argmax), ENTRY(paged_append), ENTRY(paged_attention), ENTRY(token_log_probs), ENTRY(paged_evict), ENTRY(quantize_w4), ENTRY(linear_w4),
                           ENTRY(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

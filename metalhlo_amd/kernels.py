@@ -242,6 +242,15 @@ def paged_attention(q, cache: PagedCache, table, lengths, starts, scale: Optiona
     return (_native or _host()).paged_attention(q, cache, table, lengths, starts, scale, is_causal, out)
 
 
+def paged_evict(cache: PagedCache, weights, table, lengths, keep: int, recent: int, into=None):
+    """Shortens every sequence to the last `recent` of its keys and, of those in front of them, the `keep` whose weight is greatest in each head (`weights` fp32 [pages, heads, page],
+    as `paged_attention_weighed` adds it up; of equal ones the first, NaN above all).  They move to the front in their order, their weights along, within the sequence's own pages or to those of
+    `into` [sequences, width] (room for all of them, and pages that the call reads nothing from); returns the new lengths.  In place a page belongs to one sequence.  Slots behind the new
+    length stay as they were.  8 bits: a page takes the greatest scale of those its keys come from.  Keys keep the rotation they have been appended with: the tokens that follow
+    take the places behind what is left, and are turned by their own positions in front of the append."""
+    return (_native or _host()).paged_evict(cache, weights, table, lengths, keep, recent, into)
+
+
 def token_log_probs(logits, tokens, top: int = 0):
     """(log probability of each token, entropy of each row's distribution) of logits [.., vocab] and tokens [..] (int32 or int64; one outside the vocabulary yields NaN),
     and with `top` (up to 64) also (log probabilities, ids) of the most likely tokens [.., top], the lowest id among equals.  fp32 results."""
