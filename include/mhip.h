@@ -332,6 +332,21 @@ int64_t mhip_paged_attention_workspace(const mhip_paged_cache* cache, const mhip
 int mhip_paged_attention(void* stream, const mhip_paged_cache* cache, const mhip_sequences* seqs, const void* q, void* o, int64_t q_heads, float scale,
                          int is_causal, const int64_t* strides, int dtype, void* workspace, int64_t workspace_bytes);
 
+/* The same for sequences that have a prefix in common, which is read once for all of them: o = softmax(scale * q [K_prefix; K_own]^T, causal) [V_prefix; V_own].  The prefix's first prefix_length[0] keys
+ * lie in the pages prefix [prefix_width] of the same cache; all of it is device memory.  Every token sees all of them; its sequence's own keys, which seqs describes as ever (lengths count them alone), it sees by the causal rule.
+ * An empty prefix, and a sequence without keys of its own, are allowed; a token without any keys yields zeros.  o may be q, and overlaps nothing else.
+ * The workspace is needed: mhip_paged_attention_shared_workspace says how much is of use and, in `least`, what suffices; 16-byte aligned, overwritten. */
+int64_t mhip_paged_attention_shared_workspace(const mhip_paged_cache* cache, int64_t prefix_width, const mhip_sequences* seqs, int64_t q_heads, int64_t* least);
+int mhip_paged_attention_shared(void* stream, const mhip_paged_cache* cache, const int32_t* prefix, int64_t prefix_width, const int32_t* prefix_length, const mhip_sequences* seqs, const void* q, void* o,
+                                int64_t q_heads, float scale, int is_causal, const int64_t* strides, int dtype, void* workspace, int64_t workspace_bytes);
+
+/* mhip_paged_attention, bit for bit, that also adds the weights it gives up: weights [pages, heads, page_size] in fp32 of each key get the sum over the call's tokens and the query heads of the key's head of
+ * the softmax weight.  Keys of the call's own tokens begin at zero whatever is there; those of sequences without tokens, and slots that hold no key, stay as they are.  A page belongs to one sequence.
+ * A key of a row whose scores hold a NaN gets NaN.  o overlaps nothing of the call.  Sums are fp32 in a fixed order.  The workspace is needed (`least` as above). */
+int64_t mhip_paged_attention_weighed_workspace(const mhip_paged_cache* cache, const mhip_sequences* seqs, int64_t q_heads, int64_t* least);
+int mhip_paged_attention_weighed(void* stream, const mhip_paged_cache* cache, const mhip_sequences* seqs, const void* q, void* o, float* weights, int64_t q_heads, float scale, int is_causal,
+                                 const int64_t* strides, int dtype, void* workspace, int64_t workspace_bytes);
+
 /* Eviction: of each sequence and head the last `recent` of its keys stay, and of those in front of them the `keep` of greatest weight (weights [pages, heads, page_size] in fp32; of equal ones the
  * first, NaN above all); positions that the table names no page for hold none.  What stays moves to the front in its order, keys, values and weights: to the pages of `into` [sequences, into_width],
  * which holds min(keep + recent, width * page_size) keys at least and whose pages the call reads nothing from, or with NULL within the sequence's own.  left [sequences] (not lengths) gets how

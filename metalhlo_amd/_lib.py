@@ -60,6 +60,10 @@ SIGNATURES = {
     "mhip_paged_append": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _i32]),
     "mhip_paged_attention_workspace": (_i64, [_vp, _vp, _i64]),
     "mhip_paged_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _f32, _i32, _vp, _i32, _vp, _i64]),
+    "mhip_paged_attention_shared_workspace": (_i64, [_vp, _i64, _vp, _i64, _vp]),
+    "mhip_paged_attention_shared": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _f32, _i32, _vp, _i32, _vp, _i64]),
+    "mhip_paged_attention_weighed_workspace": (_i64, [_vp, _vp, _i64, _vp]),
+    "mhip_paged_attention_weighed": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _f32, _i32, _vp, _i32, _vp, _i64]),
     "mhip_paged_evict_workspace": (_i64, [_vp, _vp, _i64, _i64, _i32, _vp]),
     "mhip_paged_evict": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64]),
     "mhip_quantize_w4": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _i32]),

@@ -618,6 +618,75 @@ float* key_weights(PyObject* o, const Cache& cache) {
     return w.data_ptr<float>();
 }
 
+// the workspace of a call that needs `least` of it
+at::Tensor needed(int64_t bytes, int64_t least, const at::Tensor& like) {
+    at::Tensor work = workspace(bytes, like);
+    if (!work.defined() && least > 0) work = empty({least}, at::kByte, like);
+    return work;
+}
+
+// paged_attention_shared(q, cache, prefix, prefix_length, table, lengths, starts, scale or None, is_causal, out)
+FUNCTION(paged_attention_shared) {
+    return guarded(n, 10, [&] {
+        const Cache cache = cache_of(arg[1]);
+        int64_t strides[4];
+        const at::Tensor& q = head_rows(arg[0], cache, strides);
+        const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
+        if (H == 0 || cache.c.heads == 0 || H % cache.c.heads) raise(PyExc_ValueError, "the query heads must be a multiple of the cache's heads");
+        const at::Tensor &prefix = dense(arg[2]), &length = dense(arg[3]);
+        for (const at::Tensor* t : {&prefix, &length}) {
+            on_current_device(*t);
+            if (t->scalar_type() != at::kInt) raise(PyExc_TypeError, "prefix and prefix_length must be int32");
+        }
+        if (prefix.dim() != 1 || length.numel() != 1) raise(PyExc_ValueError, "prefix must be [pages] and prefix_length hold one number");
+        const mhip_sequences seqs = sequences_of(arg[4], arg[5], arg[6], T);
+        const float scale = arg[7] == Py_None ? 1.f / std::sqrt((float)D) : (float)number(arg[7]);
+        const bool causal = truth(arg[8]);
+        at::Tensor out;
+        if (arg[9] == Py_None) {
+            out = empty({T, H, D}, q.scalar_type(), q);
+            strides[2] = H * D;
+            strides[3] = D;
+        } else {
+            out = head_rows(arg[9], cache, strides + 2);
+            if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type()) raise(PyExc_ValueError, "out must have q's shape and type");
+            no_overlap(out, "out must not overlap itself");
+        }
+        const int dt = dtype_code(q.scalar_type());
+        int64_t least = 0;
+        const int64_t bytes = mhip_paged_attention_shared_workspace(&cache.c, prefix.size(0), &seqs, H, &least);
+        const at::Tensor work = needed(bytes, least, q);
+        check([&] { return mhip_paged_attention_shared(stream_of(q), &cache.c, prefix.data_ptr<int32_t>(), prefix.size(0), length.data_ptr<int32_t>(), &seqs, q.data_ptr(), out.data_ptr(), H, scale,
+                                                       causal, strides, dt, work.defined() ? work.data_ptr() : nullptr, work.defined() ? work.numel() : 0); });
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// paged_attention_weighed(q, cache, weights, table, lengths, starts, scale or None, is_causal)
+FUNCTION(paged_attention_weighed) {
+    return guarded(n, 8, [&] {
+        const Cache cache = cache_of(arg[1]);
+        int64_t strides[4];
+        const at::Tensor& q = head_rows(arg[0], cache, strides);
+        const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
+        if (H == 0 || cache.c.heads == 0 || H % cache.c.heads) raise(PyExc_ValueError, "the query heads must be a multiple of the cache's heads");
+        float* weights = key_weights(arg[2], cache);
+        const mhip_sequences seqs = sequences_of(arg[3], arg[4], arg[5], T);
+        const float scale = arg[6] == Py_None ? 1.f / std::sqrt((float)D) : (float)number(arg[6]);
+        const bool causal = truth(arg[7]);
+        at::Tensor out = empty({T, H, D}, q.scalar_type(), q);
+        strides[2] = H * D;
+        strides[3] = D;
+        const int dt = dtype_code(q.scalar_type());
+        int64_t least = 0;
+        const int64_t bytes = mhip_paged_attention_weighed_workspace(&cache.c, &seqs, H, &least);
+        const at::Tensor work = needed(bytes, least, q);
+        check([&] { return mhip_paged_attention_weighed(stream_of(q), &cache.c, &seqs, q.data_ptr(), out.data_ptr(), weights, H, scale, causal, strides, dt, work.defined() ? work.data_ptr() : nullptr,
+                                                        work.defined() ? work.numel() : 0); });
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
 // paged_evict(cache, weights, table, lengths, keep, recent, into or None) -> new lengths
 FUNCTION(paged_evict) {
     return guarded(n, 7, [&] {
@@ -639,8 +708,7 @@ FUNCTION(paged_evict) {
         at::Tensor left = empty({table.size(0)}, at::kInt, table);
         int64_t least = 0;
         const int64_t bytes = mhip_paged_evict_workspace(&cache.c, &seqs, keep, recent, into == nullptr, &least);
-        at::Tensor work = workspace(bytes, table);
-        if (!work.defined() && least > 0) work = empty({least}, at::kByte, table);        // (without room for the list there is no answer)
+        const at::Tensor work = needed(bytes, least, table);
         check([&] { return mhip_paged_evict(stream_of(table), &cache.c, &seqs, weights, keep, recent, into ? into->data_ptr<int32_t>() : nullptr, into ? into->size(1) : 0, left.data_ptr<int32_t>(),
                                             work.defined() ? work.data_ptr() : nullptr, work.defined() ? work.numel() : 0); });
         return THPVariable_Wrap(std::move(left));
@@ -783,7 +851,7 @@ FUNCTION(bind) {
 
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {ENTRY(softmax), ENTRY(layer_norm), ENTRY(rms_norm), ENTRY(bias_gelu), ENTRY(matmul), ENTRY(linear), ENTRY(linear_layer), ENTRY(matmul_sums), ENTRY(tied_head), ENTRY(finish_norm), ENTRY(causal_attention), ENTRY(attend_project), ENTRY(attend_project_layer),
-                          ENTRY(flash_attention), ENTRY(argmax), ENTRY(paged_append), ENTRY(paged_attention), ENTRY(token_log_probs), ENTRY(paged_evict), ENTRY(quantize_w4), ENTRY(linear_w4),
+                          ENTRY(flash_attention), ENTRY(argmax), ENTRY(paged_append), ENTRY(paged_attention), ENTRY(token_log_probs), ENTRY(paged_attention_shared), ENTRY(paged_attention_weighed), ENTRY(paged_evict), ENTRY(quantize_w4), ENTRY(linear_w4),
                           ENTRY(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -242,6 +242,19 @@ def paged_attention(q, cache: PagedCache, table, lengths, starts, scale: Optiona
     return (_native or _host()).paged_attention(q, cache, table, lengths, starts, scale, is_causal, out)
 
 
+def paged_attention_shared(q, cache: PagedCache, prefix, prefix_length, table, lengths, starts, scale: Optional[float] = None, is_causal: bool = True,
+                           out: Optional[torch.Tensor] = None):
+    """`paged_attention` of sequences that have a prefix in common, which is read once for all of them: the first `prefix_length` (int32 [1]) keys of the pages `prefix` (int32 [width]) of the same cache
+    lie in front of each sequence's own, which `table` and `lengths` describe alone.  Every token sees the whole prefix, and of its own sequence what `is_causal` says."""
+    return (_native or _host()).paged_attention_shared(q, cache, prefix, prefix_length, table, lengths, starts, scale, is_causal, out)
+
+
+def paged_attention_weighed(q, cache: PagedCache, weights, table, lengths, starts, scale: Optional[float] = None, is_causal: bool = True):
+    """`paged_attention` (the same bits) that also adds up in `weights` (fp32 [pages, heads, page]) how much weight each key is given, by all tokens of the call and all query heads of its
+    head: what `paged_evict` goes by.  Keys of the call's own tokens begin at zero, whatever their slots held.  A page belongs to one sequence of the call."""
+    return (_native or _host()).paged_attention_weighed(q, cache, weights, table, lengths, starts, scale, is_causal)
+
+
 def paged_evict(cache: PagedCache, weights, table, lengths, keep: int, recent: int, into=None):
     """Shortens every sequence to the last `recent` of its keys and, of those in front of them, the `keep` whose weight is greatest in each head (`weights` fp32 [pages, heads, page],
     as `paged_attention_weighed` adds it up; of equal ones the first, NaN above all).  They move to the front in their order, their weights along, within the sequence's own pages or to those of
