@@ -224,8 +224,8 @@ typedef struct {
  * scale = (hi - lo) / 15 rounded to dtype, zero = round(-lo / scale), q = round(w / scale) + zero within 0 .. 15. */
 int mhip_quantize_w4(void* stream, const void* w, int64_t stride_n, int64_t stride_k, const mhip_w4* out, int w_dtype, int dtype);
 /* c [M, N] = act(x [M, K] . W^T + bias) (+ residual [M, N]); x, scales, bias [N], residual and c of dtype BF16 or F16, bias and residual may be NULL.  fp32 sums of exact products and
- * one rounding.  From 129 rows on W is rounded to dtype, once, in the workspace (mhip_linear_w4_workspace bytes, 0: of no use; 16-byte aligned, overwritten), and the product is
- * mhip_gemm_residual's; with less, or none, it is not.  The last bits of a row may depend on the number of rows.
+ * one rounding.  The workspace (mhip_linear_w4_workspace bytes, 0: of no use; 16-byte aligned, overwritten) lets few rows deal K over the device; from 129 rows on W is
+ * rounded to dtype in it, once, and the product is mhip_gemm_residual's.  With less, or none, neither is done.  The last bits of a row may depend on the number of rows.
  * The reference has no such layer (its matmul: Compiler/CodeGenerator.swift:4797-4850). */
 int64_t mhip_linear_w4_workspace(int64_t M, const mhip_w4* w, int dtype);
 int mhip_linear_w4(void* stream, const void* x, const mhip_w4* w, const void* bias, const void* residual, void* c, int64_t M, int activation, int dtype, void* workspace,

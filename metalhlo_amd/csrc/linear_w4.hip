@@ -13,25 +13,27 @@
 // Few rows: w4_rows_kernel, whose time is that of reading W.  Many: W is rounded to 16 bits into the workspace and multiplied by mhip_gemm (kManyRows).
 #include <algorithm>
 
-#include "gemm_common.h"
+#include "arrive.h"
 
 namespace mhip {
 namespace {
 
-constexpr int kWaves = 8, kBlockK = 128;
+constexpr int kBlockK = 128;
 
 struct W4Args {
     const void* x;
-    const u32x4* words;
+    const u32x4* words4;
     const uint32_t* scales;           // pairs
     const void *bias, *residual;
     void* c;
     int M, N, K, act;
     int n16, k128;
     int whole;                        // four columns of a row of C lie on 8 bytes, and so do the bias' and the residual's
+    int even;                         // rows of x lie on 16 bytes
+    int parts, per, chunk;            // of K: workgroups that share it, blocks of one, blocks of x in LDS at a time where that is not known at compile time
+    float* sums;                      // [row block][strip][part]
+    uint64_t *words, tag;
 };
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_rsrc(const void* p, uint32_t bytes) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000); }
 
 // the eight numbers of a word
 template <typename T>
@@ -57,121 +59,196 @@ __device__ __forceinline__ float low_half(uint32_t w) { return Elem<T>::to_f32(_
 template <typename T>
 __device__ __forceinline__ float high_half(uint32_t w) { return Elem<T>::to_f32(__builtin_bit_cast(T, (uint16_t)(w >> 16))); }
 
-// 16 NT columns of C and 16 MT rows a workgroup, whose waves split K by blocks of 128.  U blocks of a wave are on their way at a time.
-// EVEN: rows of x lie on 16 bytes; else x is read number by number.
-template <typename T, int GROUP, int MT, int NT, int U, bool EVEN>
-__global__ __launch_bounds__(64 * kWaves) void w4_rows_kernel(W4Args g) {
-    constexpr int kGroups = kBlockK / GROUP, kSteps = GROUP / 32;
-    __shared__ f32x4 sums[kWaves][NT * MT][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// A workgroup of WN x WK waves has 16 WN columns of C, 16 MT rows and a part of K: wave (wn, wk) the wn-th sixteen columns and every WK-th block of 128.  U blocks of a wave are on their way at a time.
+// x lies in LDS: read from memory by each wave for itself it is 4 MT times as many bytes as W's, through an L2 (24 rows, 5120 x 5120, 19.3 us so, 13.5 now).  In two chunks of CU WK blocks of K, ROWS rows
+// at most, one multiplied while the next is on its way in registers (one chunk at a time, 64 rows of 4096 x 4096, 18.6 us | 14.5); or, CU = 0, of a few rows all of a part at once (one token of 8192 x 8192,
+// two chunks of sixteen blocks 15.8 | so 12.0).
+// Where K is dealt over workgroups (parts), the last of them to arrive adds the parts up in order (arrive.h).
+template <typename T, int GROUP, int MT, int WN, int WK, int U, int CU, int ROWS>
+__global__ __launch_bounds__(64 * WN * WK) void w4_rows_kernel(W4Args g) {
+    constexpr int kGroups = kBlockK / GROUP, kSteps = GROUP / 32, kThreads = 64 * WN * WK;
+    constexpr bool kWhole = CU == 0;                                       // (CU: see below)
+    static_assert(U % (kWhole ? 1 : CU) == 0, "a turn of the words is whole chunks of x");
+    constexpr int kChunk = CU * WK, kRowPieces = kWhole ? 1 : kChunk * (kBlockK / 8), kStride = kChunk * (kBlockK * 2) + 16;
+    constexpr int kPieces = kWhole ? 4 : (ROWS * kRowPieces + kThreads - 1) / kThreads;      // of x, that a thread has on their way
+    extern __shared__ __attribute__((aligned(16))) char smem[];              // x's chunk, then the waves' sums
+    __shared__ int last;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wk = wave / WN;
     const int li = lane & 15, lg = lane >> 4;
-    const int tile0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
-    const int rows = min(g.M - m0, 16 * MT);
-    const __amdgpu_buffer_rsrc_t rx = w4_rsrc(static_cast<const T*>(g.x) + (int64_t)m0 * g.K, (uint32_t)rows * (uint32_t)g.K * 2);
+    const int strip = blockIdx.x / g.parts, part = blockIdx.x - strip * g.parts, m0 = blockIdx.y * (16 * MT), rows = min(g.M - m0, 16 * MT);
+    const int tile = strip * WN + wn, p0 = part * g.per, p1 = min(p0 + g.per, g.k128);
+    uint64_t* const word = g.words ? g.words + (int64_t)blockIdx.y * (gridDim.x / g.parts) + strip : nullptr;
+    uint64_t seen = 0;
+    if (g.parts > 1 && threadIdx.x == 0) seen = arrive_look(word);
 
-    struct Block { u32x4 w[NT], scale[NT][kGroups], x[MT][4]; };
-    const u32x4* wp[NT];
-    const uint32_t* sp[NT];
-#pragma unroll
-    for (int i = 0; i < NT; i++) {
-        const int64_t tile = min(tile0 + i, g.n16 - 1);
-        wp[i] = g.words + tile * g.k128 * 64 + lane;
-        sp[i] = g.scales + tile * g.k128 * (kGroups * 16) + 4 * lg;
-    }
-    uint32_t xo[MT];                                                       // (a row behind the last is the last again; nothing is stored of it)
-#pragma unroll
-    for (int i = 0; i < MT; i++) xo[i] = (uint32_t)min(16 * i + li, rows - 1) * (uint32_t)g.K * 2;
-
+    struct Block { u32x4 w, scale[kGroups]; };
+    const int64_t at = (int64_t)min(tile, g.n16 - 1) * g.k128;
+    const u32x4* wp = g.words4 + at * 64 + lane;
+    const uint32_t* sp = g.scales + at * (kGroups * 16) + 4 * lg;
     auto load = [&](Block& b, int kb) __attribute__((always_inline)) {
+        b.w = __builtin_nontemporal_load(wp + (int64_t)kb * 64);
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-            b.w[i] = __builtin_nontemporal_load(wp[i] + (int64_t)kb * 64);
-#pragma unroll
-            for (int j = 0; j < kGroups; j++) b.scale[i][j] = *reinterpret_cast<const u32x4*>(sp[i] + ((int64_t)kb * kGroups + j) * 16);
-        }
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int s = 0; s < 4; s++) {
-                const int k = kb * kBlockK + 32 * s + 8 * lg;
-                if constexpr (EVEN) {
-                    b.x[i][s] = __builtin_amdgcn_raw_buffer_load_b128(rx, k < g.K ? xo[i] + 2 * k : kOob, 0, 0);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const uint32_t lo = __builtin_amdgcn_raw_buffer_load_b16(rx, k + 2 * e < g.K ? xo[i] + 2 * (k + 2 * e) : kOob, 0, 0);
-                        const uint32_t hi = __builtin_amdgcn_raw_buffer_load_b16(rx, k + 2 * e + 1 < g.K ? xo[i] + 2 * (k + 2 * e + 1) : kOob, 0, 0);
-                        b.x[i][s][e] = (lo & 0xFFFFu) | hi << 16;
-                    }
-                }
-            }
+        for (int j = 0; j < kGroups; j++) b.scale[j] = *reinterpret_cast<const u32x4*>(sp + ((int64_t)kb * kGroups + j) * 16);
     };
-    f32x4 acc[NT][MT];
+    // ---- x: rows sixteen bytes longer than they are, so that sixteen rows' pieces lie in different banks; zeros behind K
+    const T* const x = static_cast<const T*>(g.x) + (int64_t)m0 * g.K;
+    auto piece = [&](int row, int k) __attribute__((always_inline)) {
+        const T* p = x + (int64_t)row * g.K + k;
+        u32x4 v = {0, 0, 0, 0};
+        if (g.even) {
+            if (k < g.K) v = *reinterpret_cast<const u32x4*>(p);
+        } else {
 #pragma unroll
-    for (int i = 0; i < NT; i++)
+            for (int e = 0; e < 8; e++)
+                if (k + e < g.K) v[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[e]) << 16 * (e & 1);
+        }
+        return v;
+    };
+    u32x4 ahead[kPieces];
+    const int stride = kWhole ? g.chunk * (kBlockK * 2) + 16 : kStride;
+    int xo[MT];                                                            // (rows behind the last are the last again; nothing is stored of them)
 #pragma unroll
-        for (int j = 0; j < MT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int m = 0; m < MT; m++) xo[m] = min(16 * m + li, (kWhole ? rows : ROWS) - 1) * stride + 16 * lg;
+
+    f32x4 acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; m++) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
     const uint32_t one = std::is_same<T, bf16_t>::value ? 0x3F803F80u : 0x3C003C00u;
     const u32x4 ones = {one, one, one, one};
-    auto multiply = [&](const Block& b) __attribute__((always_inline)) {
+    auto multiply = [&](const Block& b, const char* from, int place) __attribute__((always_inline)) {          // `place`: of the block in the chunk
 #pragma unroll
         for (int j = 0; j < kGroups; j++) {
-            f32x4 part[NT][MT], total[MT];
+            f32x4 part[MT], total[MT];
 #pragma unroll
-            for (int m = 0; m < MT; m++) {
-                total[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < NT; i++) part[i][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
+            for (int m = 0; m < MT; m++) part[m] = total[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = j * kSteps; s < (j + 1) * kSteps; s++) {
+                const u32x4 q = numbers<T>(b.w[s]);
 #pragma unroll
-                for (int m = 0; m < MT; m++) total[m] = product<T>(ones, b.x[m][s], total[m]);
-#pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    const u32x4 q = numbers<T>(b.w[i][s]);
-#pragma unroll
-                    for (int m = 0; m < MT; m++) part[i][m] = product<T>(q, b.x[m][s], part[i][m]);
+                for (int m = 0; m < MT; m++) {
+                    const u32x4 x = *reinterpret_cast<const u32x4*>(from + xo[m] + place * (kBlockK * 2) + 64 * s);
+                    part[m] = product<T>(q, x, part[m]);
+                    total[m] = product<T>(ones, x, total[m]);
                 }
             }
 #pragma unroll
-            for (int i = 0; i < NT; i++)
+            for (int r = 0; r < 4; r++) {
+                const float scale = low_half<T>(b.scale[j][r]), zero = high_half<T>(b.scale[j][r]);
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float scale = low_half<T>(b.scale[i][j][r]), zero = high_half<T>(b.scale[i][j][r]);
-#pragma unroll
-                    for (int m = 0; m < MT; m++) acc[i][m][r] = fmaf(scale, fmaf(-zero, total[m][r], part[i][m][r]), acc[i][m][r]);
-                }
+                for (int m = 0; m < MT; m++) acc[m][r] = fmaf(scale, fmaf(-zero, total[m][r], part[m][r]), acc[m][r]);
+            }
         }
     };
+    // ---- a block's words are asked for U blocks ahead
     Block blk[U];
 #pragma unroll
     for (int u = 0; u < U; u++)
-        if (wave + u * kWaves < g.k128) load(blk[u], wave + u * kWaves);
-    for (int kb = wave; kb < g.k128; kb += U * kWaves) {
+        if (p0 + wk + u * WK < p1) load(blk[u], p0 + wk + u * WK);
+    if constexpr (kWhole) {
+        for (int c0 = p0; c0 < p1; c0 += g.chunk) {
+            const int c1 = min(c0 + g.chunk, p1), pieces = (c1 - c0) * (kBlockK / 8);
+            if (c0 > p0) __syncthreads();                                    // (the chunk before has been read)
+            for (int i0 = threadIdx.x; i0 < rows * pieces; i0 += kPieces * kThreads) {
+                int to[kPieces];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (kb + u * kWaves >= g.k128) break;
-            multiply(blk[u]);
-            if (kb + (u + U) * kWaves < g.k128) load(blk[u], kb + (u + U) * kWaves);
+                for (int j = 0; j < kPieces; j++) {
+                    const int i = min(i0 + j * kThreads, rows * pieces - 1), row = i / pieces, at = i - row * pieces;
+                    to[j] = row * stride + at * 16;
+                    ahead[j] = piece(row, c0 * kBlockK + at * 8);
+                }
+#pragma unroll
+                for (int j = 0; j < kPieces; j++) *reinterpret_cast<u32x4*>(smem + to[j]) = ahead[j];
+            }
+            __syncthreads();
+            for (int kb = c0 + wk; kb < c1; kb += U * WK) {
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (kb + u * WK >= c1) break;
+                    multiply(blk[u], smem, kb + u * WK - c0);
+                    if (kb + (u + U) * WK < p1) load(blk[u], kb + (u + U) * WK);
+                }
+            }
+        }
+    } else {
+        auto fetch = [&](int c0) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < kPieces; j++) {
+                const int i = threadIdx.x + j * kThreads;
+                ahead[j] = piece(min(i / kRowPieces, rows - 1), c0 * kBlockK + i % kRowPieces * 8);
+            }
+        };
+        fetch(p0);
+        int which = 0;
+        for (int turn = p0; turn < p1; turn += U * WK) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (u % (kWhole ? 1 : CU) == 0) {
+                    const int c0 = turn + u * WK;
+                    if (c0 >= p1) break;
+                    char* const to = smem + which * (ROWS * kStride);         // (whose last readers have passed the barrier of the chunk between)
+#pragma unroll
+                    for (int j = 0; j < kPieces; j++) {
+                        const int i = threadIdx.x + j * kThreads;
+                        if (kPieces * kThreads == ROWS * kRowPieces || i < ROWS * kRowPieces) *reinterpret_cast<u32x4*>(to + i / kRowPieces * kStride + i % kRowPieces * 16) = ahead[j];
+                    }
+                    __syncthreads();
+                    if (c0 + kChunk < p1) fetch(c0 + kChunk);
+                    which ^= 1;
+                }
+                const int kb = turn + u * WK + wk;
+                if (kb < p1) {
+                    multiply(blk[u], smem + (which ^ 1) * (ROWS * kStride), u % (kWhole ? 1 : CU) * WK + wk);
+                    if (kb + U * WK < p1) load(blk[u], kb + U * WK);
+                }
+            }
         }
     }
+    if (g.parts > 1 && threadIdx.x == 0) arrive_claim(word, seen, g.tag);
 
-    // ---- the waves' sums, as their lanes hold them: lane (li, lg) has row li of C's sixteen and columns 4 lg .. 4 lg + 3
-#pragma unroll
-    for (int i = 0; i < NT; i++)
-#pragma unroll
-        for (int m = 0; m < MT; m++) sums[wave][i * MT + m][lane] = acc[i][m];
+    // ---- sums, as their lanes hold them: lane (li, lg) has row li of C's sixteen and columns 4 lg .. 4 lg + 3.  Item t of the workgroup's is lane t % 64 of row group t / 64 % MT of its tile t / (64 MT)
+    constexpr int kItems = WN * MT * 64, kMine = (kItems + kThreads - 1) / kThreads;
     __syncthreads();
-    for (int t = wave; t < NT * MT; t += kWaves) {
-        f32x4 sum = sums[0][t][lane];
+    f32x4* sums = reinterpret_cast<f32x4*>(smem);
 #pragma unroll
-        for (int w = 1; w < kWaves; w++) sum += sums[w][t][lane];
-        const int row = 16 * (t % MT) + li, col = (tile0 + t / MT) * 16 + 4 * lg;
-        if (row >= rows || col >= g.N) continue;
-        const int64_t at = (int64_t)(m0 + row) * g.N + col;
-        T* c = static_cast<T*>(g.c) + at;
-        const T *res = static_cast<const T*>(g.residual) + at, *bias = static_cast<const T*>(g.bias) + col;
+    for (int m = 0; m < MT; m++) sums[(wk * WN + wn) * (MT * 64) + m * 64 + lane] = acc[m];
+    __syncthreads();
+    f32x4 sum[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; i++) {
+        const int t = min((int)threadIdx.x + i * kThreads, kItems - 1);
+        sum[i] = sums[t];
+#pragma unroll
+        for (int w = 1; w < WK; w++) sum[i] += sums[w * kItems + t];
+    }
+    if (g.parts > 1) {
+        const int64_t strips = gridDim.x / g.parts, own = ((int64_t)blockIdx.y * strips + strip) * g.parts;
+        const __amdgpu_buffer_rsrc_t rs = parts_rsrc(reinterpret_cast<const char*>(g.sums) + own * (kItems * 16));
+#pragma unroll
+        for (int i = 0; i < kMine; i++)
+            if ((int)threadIdx.x + i * kThreads < kItems) store_part(rs, (uint32_t)(part * kItems + (int)threadIdx.x + i * kThreads) * 16, sum[i]);
+        if (!arrive_last(word, g.parts, &last)) return;
+#pragma unroll
+        for (int i = 0; i < kMine; i++) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int q0 = 0; q0 < g.parts; q0 += 4) {
+            f32x4 v[4][kMine];
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int i = 0; i < kMine; i++) v[q][i] = load_part(rs, (uint32_t)(min(q0 + q, g.parts - 1) * kItems + min((int)threadIdx.x + i * kThreads, kItems - 1)) * 16);
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int i = 0; i < kMine; i++)
+                    if (q0 + q < g.parts) sum[i] += v[q][i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kMine; i++) {
+        const int t = threadIdx.x + i * kThreads, row = 16 * (t / 64 % MT) + (t & 15), col = (strip * WN + t / (64 * MT)) * 16 + 4 * (t >> 4 & 3);
+        if (t >= kItems || row >= rows || col >= g.N) continue;
+        const int64_t place = (int64_t)(m0 + row) * g.N + col;
+        T* c = static_cast<T*>(g.c) + place;
+        const T *res = static_cast<const T*>(g.residual) + place, *bias = static_cast<const T*>(g.bias) + col;
         Pack4<T> o, r{}, b{};
         const int n = min(g.N - col, 4);
         if (g.whole) {
@@ -188,7 +265,7 @@ __global__ __launch_bounds__(64 * kWaves) void w4_rows_kernel(W4Args g) {
             constexpr int ACT = decltype(act_tag)::value;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float y = apply_act_c<ACT>(g.bias ? sum[e] + Elem<T>::to_f32(b.v[e]) : sum[e]);
+                const float y = apply_act_c<ACT>(g.bias ? sum[i][e] + Elem<T>::to_f32(b.v[e]) : sum[i][e]);
                 o.v[e] = Elem<T>::from_f32(g.residual ? y + Elem<T>::to_f32(r.v[e]) : y);
             }
         });
@@ -306,19 +383,56 @@ Wide wide_of(int64_t M, const mhip_w4* w, bool even, int dtype) {
     return r;
 }
 
-template <typename T, int GROUP, int MT, int NT, int U>
-int launch_rows(hipStream_t st, const W4Args& a, bool even) {
-    const dim3 grid((unsigned)((a.n16 + NT - 1) / NT), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
-    if (even) hipLaunchKernelGGL((w4_rows_kernel<T, GROUP, MT, NT, U, true>), grid, dim3(64 * kWaves), 0, st, a);
-    else hipLaunchKernelGGL((w4_rows_kernel<T, GROUP, MT, NT, 1, false>), grid, dim3(64 * kWaves), 0, st, a);
+// How few rows are dealt.  Up to kFew rows: a workgroup four waves that share K of sixteen columns; more: eight waves, four to each sixteen of 32 columns, so that x is read once for these.
+// (us, 16 columns | 32 | 64 | 128 a workgroup: 64 rows of 4096 x 4096 22.5 | 14.3 | 14.7 | 21.7, 16 of 4096 x 14336 - | 13.9 | 15.9 | 17.7, 40 of 1000 x 3000 - | 7.0 | 9.7 | 13.8; but 24 of 5120 x 5120
+// 19.3 | 15.0 | 13.4 | 15.6)
+// Parts: as many as make the device's waves (kWavesWanted, of which few rows have more) busy at once, four blocks for each wave at least, since a part is written and read again (64 rows of 4096 x 4096:
+// two blocks a wave 22.7, four 14.7).
+constexpr int kFew = 4, kWavesWanted = 2560, kWavesOfFew = 4096, kLdsOfFew = 64 << 10;
+struct Few { int mt, wn, wk, strips, blocks, parts, per, chunk; int64_t bytes; };
+Few few_of(int64_t M, int group, int n16, int k128, bool deal) {
+    Few f{};
+    f.mt = M <= 16 ? 1 : M <= 32 || group == 32 ? 2 : 4;                     // (four sets of sums and four groups' pairs do not fit the registers)
+    f.wn = M <= kFew ? 1 : 2;
+    f.wk = 4;
+    f.strips = (n16 + f.wn - 1) / f.wn;
+    f.blocks = (int)((M + 16 * f.mt - 1) / (16 * f.mt));
+    f.parts = 1;
+    if (deal) {
+        const int64_t waves = (int64_t)f.strips * f.blocks * f.wn * f.wk;
+        const int most = std::max(k128 / (4 * f.wk), 1);
+        f.parts = (int)std::min<int64_t>(std::min<int64_t>(((M <= kFew ? kWavesOfFew : kWavesWanted) + waves / 2) / std::max<int64_t>(waves, 1), most), 64);
+        f.parts = std::max(f.parts, 1);
+    }
+    f.per = (k128 + f.parts - 1) / f.parts;
+    f.parts = (k128 + f.per - 1) / f.per;
+    f.chunk = std::min(kLdsOfFew / ((int)std::min<int64_t>(M, kFew) * (kBlockK * 2) + 16), f.per);
+    f.bytes = f.parts > 1 ? up((int64_t)f.strips * f.blocks * 8, 16) + (int64_t)f.strips * f.blocks * f.parts * f.wn * f.mt * 1024 : 0;
+    return f;
+}
+
+template <typename T, int GROUP, int MT, int WN, int WK, int U, int CU, int ROWS>
+int launch_rows(hipStream_t st, const W4Args& a, const Few& f) {
+    constexpr int kSums = WK * WN * MT * 1024, kLds = std::max(2 * ROWS * (CU * WK * kBlockK * 2 + 16), kSums);
+    const int lds = CU == 0 ? std::max(a.M * (f.chunk * (kBlockK * 2) + 16), kSums) : kLds;
+    auto kern = w4_rows_kernel<T, GROUP, MT, WN, WK, U, CU, ROWS>;
+    if (CU && kLds > 64 << 10) {
+        static const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+        if (err != hipSuccess) return fail(MHIP_ERR_LAUNCH, "linear_w4: cannot reserve %d bytes of LDS: %s", kLds, hipGetErrorString(err));
+    }
+    hipLaunchKernelGGL(kern, dim3((unsigned)(f.strips * f.parts), (unsigned)f.blocks), dim3(64 * WN * WK), lds, st, a);
     return check_launch("linear_w4");
 }
 
 template <typename T, int GROUP>
-int launch_group(hipStream_t st, const W4Args& a, bool even) {
-    if (a.M <= 16) return launch_rows<T, GROUP, 1, 1, 4>(st, a, even);
-    if (a.M <= 32) return launch_rows<T, GROUP, 2, 1, 2>(st, a, even);
-    return launch_rows<T, GROUP, 4, 1, 1>(st, a, even);
+int launch_group(hipStream_t st, const W4Args& a, const Few& f) {
+    constexpr int U = GROUP == 32 ? 2 : 4;                                   // (words ahead: what the registers hold; four groups' pairs are as many as their weights)
+    if (f.wn == 1) return launch_rows<T, GROUP, 1, 1, 4, U, 0, kFew>(st, a, f);
+    if (f.mt == 1) return launch_rows<T, GROUP, 1, 2, 4, U, 2, 16>(st, a, f);
+    if constexpr (GROUP != 32) {
+        if (f.mt == 4) return launch_rows<T, GROUP, 4, 2, 4, U, 1, 64>(st, a, f);
+    }
+    return launch_rows<T, GROUP, 2, 2, 4, U, 1, 32>(st, a, f);
 }
 
 template <typename F>
@@ -329,21 +443,20 @@ int by_group(int64_t group, F&& f) {
 }
 
 template <typename T>
-int run_w4(hipStream_t st, const W4Args& a, const mhip_w4* w, int dtype, void* workspace, int64_t bytes) {
-    const bool even = !((w->K & 7) || ((uintptr_t)a.x & 15));
+int run_w4(hipStream_t st, W4Args a, const mhip_w4* w, int dtype, void* workspace, int64_t bytes) {
     if (a.M >= kManyRows && workspace) {
-        const Wide wide = wide_of(a.M, w, even, dtype);
+        const Wide wide = wide_of(a.M, w, a.even, dtype);
         if (bytes >= wide.w + wide.x) {
             char* room = static_cast<char*>(workspace);
             T* wt = reinterpret_cast<T*>(room);
             const unsigned units = (unsigned)blocks_for(((int64_t)a.n16 * a.k128 + 3) / 4);
             const int rc = by_group(w->group, [&](auto group) {
-                hipLaunchKernelGGL((w4_widen_kernel<T, decltype(group)::value>), dim3(units), dim3(256), 0, st, a.words, a.scales, wt, a.N, a.K, a.n16, a.k128, (int)wide.stride);
+                hipLaunchKernelGGL((w4_widen_kernel<T, decltype(group)::value>), dim3(units), dim3(256), 0, st, a.words4, a.scales, wt, a.N, a.K, a.n16, a.k128, (int)wide.stride);
                 return check_launch("linear_w4");
             });
             if (rc) return rc;
             const void* x = a.x;
-            if (!even) {
+            if (!a.even) {
                 x = room + wide.w;
                 const int64_t all = a.M * wide.stride;
                 hipLaunchKernelGGL(w4_pad_kernel, dim3((unsigned)blocks_for((all + 255) / 256)), dim3(256), 0, st, static_cast<const uint16_t*>(a.x), reinterpret_cast<uint16_t*>(room + wide.w), all, a.K, (int)wide.stride);
@@ -353,7 +466,17 @@ int run_w4(hipStream_t st, const W4Args& a, const mhip_w4* w, int dtype, void* w
             return mhip_gemm_ws(st, x, wt, a.bias, a.residual, a.c, a.M, a.N, wide.stride, 1, 0, 0, (int64_t)a.M * a.N, 0, 1, a.act, dtype, left > 0 ? room + wide.w + wide.x : nullptr, left);
         }
     }
-    return by_group(w->group, [&](auto group) { return launch_group<T, decltype(group)::value>(st, a, even); });
+    Few f = few_of(a.M, (int)w->group, a.n16, a.k128, true);
+    if (f.bytes > 0 && (!workspace || bytes < f.bytes)) f = few_of(a.M, (int)w->group, a.n16, a.k128, false);
+    a.parts = f.parts;
+    a.per = f.per;
+    a.chunk = f.chunk;
+    if (f.parts > 1) {
+        a.words = static_cast<uint64_t*>(workspace);
+        a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + up((int64_t)f.strips * f.blocks * 8, 16));
+        a.tag = launch_tag();
+    }
+    return by_group(w->group, [&](auto group) { return launch_group<T, decltype(group)::value>(st, a, f); });
 }
 
 }  // namespace
@@ -383,7 +506,8 @@ extern "C" int mhip_quantize_w4(void* stream, const void* w, int64_t stride_n, i
 }
 
 extern "C" int64_t mhip_linear_w4_workspace(int64_t M, const mhip_w4* w, int dtype) {
-    if (M < kManyRows || check_w4("linear_w4_workspace", w, dtype) || w->N == 0 || w->K == 0) return 0;
+    if (M <= 0 || check_w4("linear_w4_workspace", w, dtype) || w->N == 0 || w->K == 0) return 0;
+    if (M < kManyRows) return few_of(M, (int)w->group, (int)((w->N + 15) / 16), (int)((w->K + 127) / 128), true).bytes;
     const Wide even = wide_of(M, w, true, dtype), odd = wide_of(M, w, false, dtype);
     // (whether x lies on 16 bytes is not known here)
     return w->K & 7 ? odd.w + odd.x + odd.gemm : std::max(even.w + even.gemm, odd.w + odd.x + odd.gemm);
@@ -400,6 +524,7 @@ extern "C" int mhip_linear_w4(void* stream, const void* x, const mhip_w4* w, con
     if (!x || !w->words || !w->scales || !c) return fail(MHIP_ERR_INVALID_ARGUMENT, "linear_w4: NULL tensor");
     if (((uintptr_t)w->words | (uintptr_t)w->scales | (uintptr_t)workspace) & 15) return fail(MHIP_ERR_UNSUPPORTED, "linear_w4: words, scales and workspace must be 16-byte aligned");
     const W4Args a{x, static_cast<const u32x4*>(w->words), static_cast<const uint32_t*>(w->scales), bias, residual, c, (int)M, (int)w->N, (int)w->K, activation,
-                   (int)((w->N + 15) / 16), (int)((w->K + 127) / 128), !(w->N & 3) && !(((uintptr_t)c | (uintptr_t)bias | (uintptr_t)residual) & 7)};
+                   (int)((w->N + 15) / 16), (int)((w->K + 127) / 128), !(w->N & 3) && !(((uintptr_t)c | (uintptr_t)bias | (uintptr_t)residual) & 7),
+                   !((w->K & 7) || ((uintptr_t)x & 15)), 1, 0, 0, nullptr, nullptr, 0};
     return dtype == MHIP_BF16 ? run_w4<bf16_t>(as_stream(stream), a, w, dtype, workspace, workspace_bytes) : run_w4<f16_t>(as_stream(stream), a, w, dtype, workspace, workspace_bytes);
 }
