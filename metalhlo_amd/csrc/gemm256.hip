@@ -350,7 +350,12 @@ bool gemm256_eligible(const GemmArgs& g, int64_t batch, int trans_a, int trans_b
 int launch_gemm256(hipStream_t s, const GemmArgs& g, int64_t batch, int trans_a, int trans_b,
                    int dtype, int bw, int ring) {
     if (bw == 384) return launch_gemm384(s, g, batch, trans_a, trans_b, dtype);
-    if (bw == 192) return launch_gemm192(s, g, batch, trans_a, trans_b, dtype);                     // 128-row tiles
+    if (bw == 192) {                                                                                // 128-row tiles
+        // (whole ones: with `partial` it leaves its tiles' sums there, for gemm_mid.hip's split of K, and a caller's workspace is no such request)
+        GemmArgs whole = g;
+        whole.partial = nullptr;
+        return launch_gemm192(s, whole, batch, trans_a, trans_b, dtype);
+    }
     if (bw == 288) return launch_gemm288(s, g, batch, trans_a, trans_b, dtype);
     if (bw == 128 && ring == 3) return launch_gemm_pair(s, g, batch, trans_a, trans_b, dtype);      // two workgroups per compute unit
     if (dtype == MHIP_BF16) return family256<bf16_t>(s, g, batch, trans_a, trans_b, bw, ring);
