@@ -462,7 +462,7 @@ int run_w4(hipStream_t st, W4Args a, const mhip_w4* w, int dtype, void* workspac
                 hipLaunchKernelGGL(w4_pad_kernel, dim3((unsigned)blocks_for((all + 255) / 256)), dim3(256), 0, st, static_cast<const uint16_t*>(a.x), reinterpret_cast<uint16_t*>(room + wide.w), all, a.K, (int)wide.stride);
                 if (const int rc2 = check_launch("linear_w4")) return rc2;
             }
-            const int64_t left = bytes - wide.w - wide.x;
+            const int64_t left = std::min(bytes - wide.w - wide.x, wide.gemm);
             return mhip_gemm_ws(st, x, wt, a.bias, a.residual, a.c, a.M, a.N, wide.stride, 1, 0, 0, (int64_t)a.M * a.N, 0, 1, a.act, dtype, left > 0 ? room + wide.w + wide.x : nullptr, left);
         }
     }
