@@ -54,12 +54,15 @@ struct PagedArgs {
     Divider by_group, by_heads, by_shares;    // G, KV, shares
     int unit_shift;                           // log2 of the keys that one unit of the line stands for
     float* more = nullptr;                    // kLeaves, kGoesOn: [T, H, D] sums and [T, H] pairs of reference maximum and sum; kTells: [T, H] pairs of reference maximum and 1 / sum
-    int last = 1;                             // kLeaves: the last of `starts`, between whose least and greatest the call's rows lie
+    int last = 1;                             // kLeaves: the last of `starts`, in front of whose greatest the call's rows lie
+    int32_t* dealt = nullptr;                 // kLeaves: [KV, tiles] pairs, where a tile's parts are (Split; no parts: it is whole, in `more`)
+    int tiles = 0;
 };
 
 // What becomes of a row's sums:
 //   kPlain    the result
-//   kLeaves   they are left with their reference maximum and sum, for what goes on from them.  There is one sequence, whose rows are those of all of the call's
+//   kLeaves   they are left with their reference maximum and sum, for what goes on from them: a whole tile's for its rows, a part's as parts that nobody here puts together.  There is one
+//             sequence, whose rows are those of all of the call's
 //   kGoesOn   the result, of them and of what has been left for the row
 //   kTells    the result, and the reference maximum and one over the sum of the weights before they are rounded (paged_weighed.hip)
 enum Form { kPlain, kLeaves, kGoesOn, kTells };
@@ -89,20 +92,19 @@ struct Line {
 // line are made for.
 struct Known { int start[64], tokens[64], keys[64], line[64]; };
 struct Found { int b, before, start, tokens, keys, line; };
+// By a wave: the rows of a call from the first of its tensors to the end of the last sequence.
+__device__ __forceinline__ int rows_of_all(const PagedArgs& a, int lane) {
+    float end = 0.f;                                                        // (whole numbers of up to 2^24)
+    for (int i = lane; i <= a.last; i += 64) end = fmaxf(end, (float)min(max(a.s.starts[i], 0), a.s.T));
+    return (int)wave_max(end);
+}
 template <int FORM>
 __device__ __forceinline__ void known_of(const PagedArgs& a, Known& known, int lane) {
     const Sequences& s = a.s;
     if constexpr (FORM == kLeaves) {
-        float low = (float)s.T, high = 0.f;                                 // (whole numbers of up to 2^24)
-        for (int i = lane; i <= a.last; i += 64) {
-            const float at = (float)min(max(s.starts[i], 0), s.T);
-            low = fminf(low, at);
-            high = fmaxf(high, at);
-        }
-        low = -wave_max(-low);
-        high = wave_max(high);
-        known.start[lane] = lane ? 0 : (int)low;
-        known.tokens[lane] = lane ? 0 : max((int)high - (int)low, 0);
+        known.start[lane] = 0;
+        const int rows = rows_of_all(a, lane);
+        known.tokens[lane] = lane ? 0 : rows;
         known.keys[lane] = known.line[lane] = lane ? 0 : s.keys(0);
         return;
     }
@@ -144,6 +146,12 @@ struct Split { int first, parts; };
 __device__ __forceinline__ Split split_of(const Line& line, int shares, int share, int origin, int length) {
     const int first = min(max(line.owner(origin), 0), share);
     return {first, min(line.owner(origin + length - 1) - first + 1, min(kMostParts, shares - first))};
+}
+
+// kLeaves: of the workgroup that a tile begins in
+__device__ __forceinline__ void deal(const PagedArgs& a, int at, const Split& split, bool parted) {
+    a.dealt[2 * at] = split.first;
+    a.dealt[2 * at + 1] = parted ? split.parts : 0;
 }
 
 // Words at an address that is the same in all lanes, and that no launch writes while another reads them: read by scalar loads.
@@ -280,6 +288,12 @@ __device__ __forceinline__ void tell(const PagedArgs& a, int token, int query, f
     at[1] = exact != 0.f ? 1.f / exact : 0.f;
 }
 
+// Item idx of a tile's sums: its row and which four numbers of it
+template <int ROWS, int D>
+__device__ __forceinline__ int row_of_item(int idx) { return ROWS > 32 ? idx / (64 * (D / 8)) * 32 + (idx & 31) : idx / (D / 4); }
+template <int ROWS, int D>
+__device__ __forceinline__ int four_of_item(int idx) { return ROWS > 32 ? (idx >> 6) % (D / 8) * 2 + (idx >> 5 & 1) : idx % (D / 4); }
+
 // By the last workgroup of a tile: its parts put together in order.  `rows`: of the tile, from row `row0` of the sequence that starts at token `start`.
 // The sums of a tile of few rows lie row by row, those of many as the lanes of their waves hold them (the stores pass the L2: sixteen bytes of each of 64 rows at a time went to memory as such).
 template <typename T, int ROWS, int D, int THREADS, int FORM>
@@ -287,8 +301,8 @@ __device__ __forceinline__ void join(const PagedArgs& a, const Split& split, int
     constexpr int kFours = D / 4, kAll = (ROWS * kFours + THREADS - 1) / THREADS;             // fours of numbers of a row; a thread's of a full tile
     constexpr bool kByLanes = ROWS > 32;
     const int all = kByLanes ? (rows + 31) / 32 * 32 * kFours : rows * kFours;
-    auto row_of = [](int idx) { return kByLanes ? idx / (64 * (D / 8)) * 32 + (idx & 31) : idx / kFours; };
-    auto four_of = [](int idx) { return kByLanes ? (idx >> 6) % (D / 8) * 2 + (idx >> 5 & 1) : idx % kFours; };
+    auto row_of = [](int idx) { return row_of_item<ROWS, D>(idx); };
+    auto four_of = [](int idx) { return four_of_item<ROWS, D>(idx); };
     // AHEAD parts of ITEMS fours are asked for at once, sixteen loads that arrive after one latency: with one four at a time the sixteen of a tile of 128 rows took 40 us
     auto put = [&](auto ahead, auto items) __attribute__((always_inline)) {
         constexpr int AHEAD = decltype(ahead)::value, ITEMS = decltype(items)::value < kAll ? decltype(items)::value : kAll;
@@ -459,7 +473,8 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
         const bool parted = s1 - s0 < mine;
         const Split split = parted ? split_of(line, a.shares, blockIdx.x, origin, mine) : Split{0, 1};
         uint64_t seen = 0;
-        if (parted && threadIdx.x == 0) seen = arrive_look(a.words + split.first);
+        if (FORM != kLeaves && parted && threadIdx.x == 0) seen = arrive_look(a.words + split.first);
+        if (FORM == kLeaves && s0 == 0 && threadIdx.x == 0) deal(a, head * a.tiles + tile, split, parted);
 
         // ---- queries: row li of each tile.  d of step s: see d_of
         auto d_of = [&](int s) __attribute__((always_inline)) {
@@ -724,7 +739,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
             }
         }
 
-        if (parted && threadIdx.x == 0) arrive_claim(a.words + split.first, seen, a.tag);
+        if (FORM != kLeaves && parted && threadIdx.x == 0) arrive_claim(a.words + split.first, seen, a.tag);
         // ---- the waves' states, four sums a thread: O^T tile f holds d = 16 f + 4 g + e of group g
         if (segment) __syncthreads();                                        // (the segment before has been read)
 #pragma unroll
@@ -776,6 +791,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
                 if (FORM == kTells && four == 0) store_part(own.exact + row, e);
             }
         }
+        if (FORM == kLeaves) continue;
         if (parted && arrive_last(a.words + split.first, split.parts, &last)) join<T, ROWS, D, 64 * WAVES, FORM>(a, split, first, head, tile * tile_rows, here);
     }
 }
@@ -926,7 +942,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_tile_kernel(PagedArgs a) 
     const bool parted = off0 > 0 || off1 < length;
     const Split split = parted ? split_of(line, a.shares, share, origin, length) : Split{0, 1};
     uint64_t seen = 0;
-    if (parted && threadIdx.x == 0) seen = arrive_look(a.words + split.first);
+    if (FORM != kLeaves && parted && threadIdx.x == 0) seen = arrive_look(a.words + split.first);
+    if (FORM == kLeaves && off0 == 0 && threadIdx.x == 0) deal(a, head * a.tiles + tile, split, parted);
 
     u32x4 qf[NS];
     {
@@ -1223,7 +1240,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_tile_kernel(PagedArgs a) 
         }
         continue;
     }
-    if (threadIdx.x == 0) arrive_claim(a.words + split.first, seen, a.tag);
+    if (FORM != kLeaves && threadIdx.x == 0) arrive_claim(a.words + split.first, seen, a.tag);
     const Parts<ROWS, D> own(a, 2 * share + (off0 ? 0 : 1));
     if (row < rows) {
         const __amdgpu_buffer_rsrc_t rs = parts_rsrc(own.sums);
@@ -1236,6 +1253,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_tile_kernel(PagedArgs a) 
         if (lh == 0) store_two(own.state + 2 * r, m_run, l_run);
         if (FORM == kTells && lh == 0) store_part(own.exact + r, told);
     }
+    if (FORM == kLeaves) continue;
     if (arrive_last(a.words + split.first, split.parts, &last)) join<T, ROWS, D, kThreads, FORM>(a, split, first, head, tile * ROWS, min(ROWS, rows - tile * ROWS));
     }
 }

@@ -32,6 +32,9 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return x != x ? 0xFFFFFFFFu : u >> 31 ? ~u : u | 0x80000000u;
 }
 
+// PER: sixty-fours of positions of a wave, whose weights it keeps in registers (no more than the table reaches, a sixteenth of it a wave); 0: they are read again for each pass.
+// us, two sequences of 50000 positions and 8 heads, read again | kept: 114 | 33; 32 sequences of 2800 to 4000 19 | 10.
+template <int PER>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(SelectArgs a) {
     __shared__ int bins[kBins];
     __shared__ int found[2];                                                // the bin that the keep-th lies in; how many lie above it
@@ -41,41 +44,62 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(SelectArgs
     const int n = min(max(a.lengths[b], 0), a.width << a.page_shift), first = max(n - a.recent, 0);
     const int32_t* table = a.table + (int64_t)b * a.width;
     const int mask = (1 << a.page_shift) - 1;
+    // a wave a stretch of positions, sixty-four at a time
+    const int per = (n + 64 * kSelectWaves - 1) / (64 * kSelectWaves), p0 = wave * per * 64;
     // 0 where the table names no page
     auto key_at = [&](int pos) __attribute__((always_inline)) {
         const int page = table[pos >> a.page_shift];
         return (uint32_t)page < (uint32_t)a.pages ? ordered(a.weights[(((int64_t)page * a.KV + h) << a.page_shift) + (pos & mask)]) : 0u;
     };
+    uint32_t kept[PER ? PER : 1];
+    if constexpr (PER > 0) {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int pos = p0 + 64 * i + lane;
+            kept[i] = i < per && pos < n ? key_at(pos) : 0u;
+            if (PER > 16 && i % 8 == 7) __builtin_amdgcn_sched_barrier(0);     // (eight at a time: more addresses do not fit the registers)
+        }
+    }
+    // f(position, key) for a wave's positions, in order, all lanes at a time (key 0 behind the last)
+    auto each = [&](auto f) __attribute__((always_inline)) {
+        if constexpr (PER > 0) {
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (i < per) f(p0 + 64 * i + lane, kept[i]);
+        } else {
+            for (int i = 0; i < per; i++) {
+                const int pos = p0 + 64 * i + lane;
+                f(pos, pos < n ? key_at(pos) : 0u);
+            }
+        }
+    };
 
     // ---- the keep-th greatest: `known` are its upper bits, `wanted` its place among those that have them
     uint32_t known = 0;
     int wanted = a.keep;
-    bool all = false;                                                       // all in front stay
-    if (first <= a.keep) all = true;
+    bool all = first <= a.keep;                                             // all in front stay
     for (int pass = 0; pass < 3 && !all && a.keep > 0; pass++) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, count = pass == 2 ? 1024 : 2048;
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, count = pass == 2 ? 1024 : 2048, above = pass == 1 ? 21 : 10;
         for (int i = threadIdx.x; i < kBins; i += kSelectThreads) bins[i] = 0;
         __syncthreads();
-        for (int pos = threadIdx.x; pos < first; pos += kSelectThreads) {
-            const uint32_t key = key_at(pos);
-            const bool agrees = pass == 0 || key >> (pass == 1 ? 21 : 10) == known >> (pass == 1 ? 21 : 10);
-            if (key && agrees) atomicAdd(&bins[(key >> shift) & (count - 1)], 1);
-        }
+        each([&](int pos, uint32_t key) __attribute__((always_inline)) {
+            if (key && pos < first && (pass == 0 || key >> above == known >> above)) atomicAdd(&bins[(key >> shift) & (count - 1)], 1);
+        });
         __syncthreads();
         if (wave == 0) {
             // lane l has the l-th of 64 stretches from the top
-            const int per = count / 64;
+            const int stretch = count / 64;
             int mine = 0;
-            for (int i = 0; i < per; i++) mine += bins[count - 1 - (lane * per + i)];
+            for (int i = 0; i < stretch; i++) mine += bins[count - 1 - (lane * stretch + i)];
             const int upto = wave_scan(mine);
             const uint64_t m = __ballot(upto >= wanted);
             if (!m) {
                 if (lane == 0) found[0] = -1;                               // (fewer than `keep` have a page)
             } else if (lane == __builtin_ctzll(m)) {
-                int above = upto - mine, i = 0;
-                while (above + bins[count - 1 - (lane * per + i)] < wanted) above += bins[count - 1 - (lane * per + i++)];
-                found[0] = count - 1 - (lane * per + i);
-                found[1] = above;
+                int over = upto - mine, i = 0;
+                while (over + bins[count - 1 - (lane * stretch + i)] < wanted) over += bins[count - 1 - (lane * stretch + i++)];
+                found[0] = count - 1 - (lane * stretch + i);
+                found[1] = over;
             }
         }
         __syncthreads();
@@ -86,24 +110,18 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(SelectArgs
         }
         __syncthreads();
     }
-    // what stays: keys above `known`, the first `wanted` that equal it, and the last ones
+    // what stays: keys above `border`, the first `wanted` that equal it, and the last ones
     const uint32_t border = all ? 0u : a.keep > 0 ? known : 0xFFFFFFFFu;
     if (all || a.keep == 0) wanted = 0;
 
-    // ---- a wave a stretch of positions: counted, then written
-    const int per = ((n + kSelectWaves - 1) / kSelectWaves + 63) & ~63, p0 = min(wave * per, n), p1 = min(p0 + per, n);
-    auto look = [&](int pos, bool& is_sure, bool& is_tie) __attribute__((always_inline)) {
-        const uint32_t key = pos < p1 ? key_at(pos) : 0u;
-        is_sure = key && (pos >= first || (key > border));
-        is_tie = key && pos < first && key == border && wanted > 0;
-    };
+    // ---- counted, then written
+    auto is_sure = [&](int pos, uint32_t key) __attribute__((always_inline)) { return key && (pos >= first || key > border); };
+    auto is_tie = [&](int pos, uint32_t key) __attribute__((always_inline)) { return key && pos < first && key == border && wanted > 0; };
     int n_sure = 0, n_ties = 0;
-    for (int pos = p0; pos < p1; pos += 64) {
-        bool is_sure, is_tie;
-        look(pos + lane, is_sure, is_tie);
-        n_sure += __builtin_popcountll(__ballot(is_sure));
-        n_ties += __builtin_popcountll(__ballot(is_tie));
-    }
+    each([&](int pos, uint32_t key) __attribute__((always_inline)) {
+        n_sure += __builtin_popcountll(__ballot(is_sure(pos, key)));
+        n_ties += __builtin_popcountll(__ballot(is_tie(pos, key)));
+    });
     if (lane == 0) { sure[wave] = n_sure; ties[wave] = n_ties; }
     __syncthreads();
     int at = 0, tied = 0, total = 0, total_ties = 0;
@@ -117,16 +135,15 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(SelectArgs
     if (h == 0 && threadIdx.x == 0) a.left[b] = total;
     int32_t* list = a.list + (int64_t)blockIdx.x * a.cap;
     const uint64_t below = ((uint64_t)1 << lane) - 1;
-    for (int pos = p0; pos < p1; pos += 64) {
-        bool is_sure, is_tie;
-        look(pos + lane, is_sure, is_tie);
-        const uint64_t tie_mask = __ballot(is_tie);
-        const bool stays = is_sure || (is_tie && tied + __builtin_popcountll(tie_mask & below) < wanted);
+    each([&](int pos, uint32_t key) __attribute__((always_inline)) {
+        const bool tie = is_tie(pos, key);
+        const uint64_t tie_mask = __ballot(tie);
+        const bool stays = is_sure(pos, key) || (tie && tied + __builtin_popcountll(tie_mask & below) < wanted);
         const uint64_t m = __ballot(stays);
-        if (stays) list[at + __builtin_popcountll(m & below)] = pos + lane;
+        if (stays) list[at + __builtin_popcountll(m & below)] = pos;
         at += __builtin_popcountll(m);
         tied += __builtin_popcountll(tie_mask);
-    }
+    });
 }
 
 // A cache and the pages that sequences have in it; without a table sequence b has pages b * width + 0 .. width - 1.
@@ -230,21 +247,38 @@ __global__ __launch_bounds__(kWindow) void evict_move_kernel(MoveArgs a) {
                 *reinterpret_cast<u32x4*>(a.to.keys + ((((int64_t)into[j] << a.page_shift) + at) * kPer + p % kPer) * 16) = v[j];
             }
         }
-        // ---- values: a thread has sixteen tokens of a d
+        // ---- values: a thread has sixteen tokens of a d.  They come from a few blocks, whose sixteen tokens of a d are sixteen neighbouring numbers: what a block has for them is read in one go, and
+        // numbers change places in registers (one load for each 120 us, 32 sequences of 3400 keys cut to 1750)
         for (int p0 = 0; p0 < (here + kBlock - 1) / kBlock * D; p0 += kWindow) {
             const int p = p0 + t, block = p / D, d = p % D;
             const int into = block * kBlock < here ? to_row[min(block, kWindow / kBlock - 1)] : -1;
             uint32_t v[4 * SIZE] = {};
             uint32_t held = 0;                                              // bit e: token e has a value
             if (into >= 0) {
+                uint32_t from[4 * SIZE] = {};
+                int64_t was = -1;                                           // which block `from` is
 #pragma unroll
                 for (int e = 0; e < kBlock; e++) {
                     const int token = block * kBlock + e, r = from_row[token], s = from_slot[token];
                     if (r < 0) continue;
                     held |= 1u << e;
-                    const char* at = a.from.values + ((((int64_t)r << (a.page_shift - 4)) + (s >> 4)) * D + d) * (16 * SIZE) + (s & 15) * SIZE;
-                    if constexpr (EIGHT) v[e >> 2] |= (uint32_t)*reinterpret_cast<const uint8_t*>(at) << 8 * (e & 3);
-                    else v[e >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t*>(at) << 16 * (e & 1);
+                    const int64_t source = ((int64_t)r << (a.page_shift - 4)) + (s >> 4);
+                    if (source != was) {
+                        was = source;
+                        const u32x4* at = reinterpret_cast<const u32x4*>(a.from.values + (source * D + d) * (16 * SIZE));
+#pragma unroll
+                        for (int q = 0; q < SIZE; q++) {
+                            const u32x4 w = at[q];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) from[4 * q + k] = w[k];
+                        }
+                    }
+                    constexpr int kPerWord = 4 / SIZE;
+                    const int word = (s & 15) / kPerWord, shift = (s & 15) % kPerWord * 8 * SIZE;
+                    uint32_t x = from[0];
+#pragma unroll
+                    for (int k = 1; k < 4 * SIZE; k++) x = word == k ? from[k] : x;
+                    v[e / kPerWord] |= (x >> shift & (EIGHT ? 0xFFu : 0xFFFFu)) << (e % kPerWord * 8 * SIZE);
                 }
             }
             settled();
@@ -379,8 +413,14 @@ extern "C" int mhip_paged_evict(void* stream, const mhip_paged_cache* cache, con
     char* room = static_cast<char*>(workspace);
     hipStream_t st = as_stream(stream);
     const SelectArgs sel{weights, seqs->table, seqs->lengths, reinterpret_cast<int32_t*>(room), left, (int)seqs->width, (int)cache->pages, (int)cache->heads, page_shift, (int)keep, (int)recent, least.cap};
-    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)(B * cache->heads)), dim3(kSelectThreads), 0, st, sel);
-    if (const int rc = check_launch("paged_evict")) return rc;
+    auto select = [&](auto per) {
+        hipLaunchKernelGGL(evict_select_kernel<decltype(per)::value>, dim3((unsigned)(B * cache->heads)), dim3(kSelectThreads), 0, st, sel);
+        return check_launch("paged_evict");
+    };
+    using std::integral_constant;
+    const int rc_select = reach <= 4 * kSelectThreads ? select(integral_constant<int, 4>{}) : reach <= 16 * kSelectThreads ? select(integral_constant<int, 16>{})
+                        : reach <= 64 * kSelectThreads ? select(integral_constant<int, 64>{}) : select(integral_constant<int, 0>{});
+    if (rc_select) return rc_select;
     const Pool here{(char*)cache->keys, (char*)cache->values, cache->key_scales, cache->value_scales, weights, seqs->table, (int)seqs->width, (int)cache->pages};
     Pool there = here, between{};
     if (into) {
