@@ -32,10 +32,11 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return x != x ? 0xFFFFFFFFu : u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// PER: sixty-fours of positions of a wave, whose weights it keeps in registers (no more than the table reaches, a sixteenth of it a wave); 0: they are read again for each pass.
-// us, two sequences of 50000 positions and 8 heads, read again | kept: 114 | 33; 32 sequences of 2800 to 4000 19 | 10.
-template <int PER>
+// PER: sixty-fours of positions of a wave, whose weights it keeps in registers (no more than the table reaches, a sixteenth of it a wave); LDS: as many more that lie there; PER 0: they are read again for each pass.
+// us, two sequences of 50000 positions and 8 heads, read again | kept: 114 | 65; 32 sequences of 2800 to 4000 19 | 14.
+template <int PER, int LDS>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(SelectArgs a) {
+    __shared__ uint32_t more[LDS ? LDS * kSelectThreads : 1];
     __shared__ int bins[kBins];
     __shared__ int found[2];                                                // the bin that the keep-th lies in; how many lie above it
     __shared__ int sure[kSelectWaves], ties[kSelectWaves];
@@ -53,12 +54,28 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(SelectArgs
     };
     uint32_t kept[PER ? PER : 1];
     if constexpr (PER > 0) {
+        // (all pages are asked for, and then all weights)
+        auto fill = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int pos = p0 + 64 * i + lane;
-            kept[i] = i < per && pos < n ? key_at(pos) : 0u;
-            if (PER > 16 && i % 8 == 7) __builtin_amdgcn_sched_barrier(0);     // (eight at a time: more addresses do not fit the registers)
+            for (int i = 0; i < PER; i++) {
+                const int pos = p0 + 64 * (base + i) + lane;
+                kept[i] = base + i < per && pos < n ? (uint32_t)table[pos >> a.page_shift] : 0xFFFFFFFFu;
+            }
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int pos = p0 + 64 * (base + i) + lane;
+                const bool there = kept[i] < (uint32_t)a.pages;
+                float w = 0.f;
+                if (there) w = a.weights[(((int64_t)kept[i] * a.KV + h) << a.page_shift) + (pos & mask)];
+                kept[i] = there ? ordered(w) : 0u;
+            }
+        };
+        if constexpr (LDS > 0) {
+            fill(PER);
+#pragma unroll
+            for (int i = 0; i < LDS; i++) more[i * kSelectThreads + threadIdx.x] = kept[i];
         }
+        fill(0);
     }
     // f(position, key) for a wave's positions, in order, all lanes at a time (key 0 behind the last)
     auto each = [&](auto f) __attribute__((always_inline)) {
@@ -66,6 +83,8 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(SelectArgs
 #pragma unroll
             for (int i = 0; i < PER; i++)
                 if (i < per) f(p0 + 64 * i + lane, kept[i]);
+            if constexpr (LDS > 0)
+                for (int i = PER; i < per; i++) f(p0 + 64 * i + lane, more[(i - PER) * kSelectThreads + threadIdx.x]);
         } else {
             for (int i = 0; i < per; i++) {
                 const int pos = p0 + 64 * i + lane;
@@ -175,7 +194,7 @@ __global__ __launch_bounds__(kWindow) void evict_move_kernel(MoveArgs a) {
     __shared__ int from_row[kWindow], to_row[kWindow / kBlock];             // page * KV + head, -1 for none
     __shared__ int from_slot[kWindow];
     __shared__ int scale[2][kWindow], top[2][kWindow / kBlock];              // of keys and of values
-    const int t = threadIdx.x;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int unit = IN_PLACE ? blockIdx.x : blockIdx.x / a.windows, b = unit / a.KV, h = unit - b * a.KV;
     const int count = (int)min((int64_t)a.left[b], a.cap), mask = (1 << a.page_shift) - 1;
     for (int w = IN_PLACE ? 0 : blockIdx.x - unit * a.windows; w * kWindow < count; w++) {
@@ -247,67 +266,86 @@ __global__ __launch_bounds__(kWindow) void evict_move_kernel(MoveArgs a) {
                 *reinterpret_cast<u32x4*>(a.to.keys + ((((int64_t)into[j] << a.page_shift) + at) * kPer + p % kPer) * 16) = v[j];
             }
         }
-        // ---- values: a thread has sixteen tokens of a d.  They come from a few blocks, whose sixteen tokens of a d are sixteen neighbouring numbers: what a block has for them is read in one go, and
-        // numbers change places in registers (one load for each 120 us, 32 sequences of 3400 keys cut to 1750)
-        for (int p0 = 0; p0 < (here + kBlock - 1) / kBlock * D; p0 += kWindow) {
-            const int p = p0 + t, block = p / D, d = p % D;
-            const int into = block * kBlock < here ? to_row[min(block, kWindow / kBlock - 1)] : -1;
-            uint32_t v[4 * SIZE] = {};
+        // ---- values: a wave sixteen places, a lane a d of them or two.  Their tokens come from a few blocks, whose sixteen tokens of a d are sixteen neighbouring numbers: four blocks are asked for at a
+        // time, and numbers change places in registers.  (32 sequences of 3400 keys cut to 1750: a load for each number 120 us, a block's numbers in one go but block after block 105, four blocks 81.)
+        constexpr int kHalves = (D + 63) / 64, kFrom = 4, kWords = 4 * SIZE, kPerWord = 4 / SIZE;
+        typedef uint32_t Words __attribute__((ext_vector_type(kFrom * kWords)));
+        for (int block0 = 0; block0 * kBlock < here; block0 += kWindow / 64) {
+            const int block = block0 + wave, into = block * kBlock < here ? to_row[block] : -1;       // (sixteen blocks a window, four a turn)
+            uint32_t v[kHalves][kWords] = {};
             uint32_t held = 0;                                              // bit e: token e has a value
             if (into >= 0) {
-                uint32_t from[4 * SIZE] = {};
-                int64_t was = -1;                                           // which block `from` is
+                const int r = from_row[block * kBlock + (lane & 15)], s = from_slot[block * kBlock + (lane & 15)];
+                const int r1 = __shfl_up(r, 1, 64), s1 = __shfl_up(s, 1, 64);
+                held = (uint32_t)__ballot(r >= 0) & 0xFFFFu;
+                const uint32_t begins = (uint32_t)__ballot(r >= 0 && ((lane & 15) == 0 || r != r1 || s >> 4 != s1 >> 4)) & 0xFFFFu;      // tokens that are the first of their block
+                uint32_t left = begins;
+                for (int base = 0; left; base += kFrom) {
+                    Words from[kHalves];
 #pragma unroll
-                for (int e = 0; e < kBlock; e++) {
-                    const int token = block * kBlock + e, r = from_row[token], s = from_slot[token];
-                    if (r < 0) continue;
-                    held |= 1u << e;
-                    const int64_t source = ((int64_t)r << (a.page_shift - 4)) + (s >> 4);
-                    if (source != was) {
-                        was = source;
-                        const u32x4* at = reinterpret_cast<const u32x4*>(a.from.values + (source * D + d) * (16 * SIZE));
+                    for (int j = 0; j < kFrom; j++) {
+                        const int e = left ? __builtin_ctz(left) : __builtin_ctz(begins);            // (none left: the first again)
+                        left &= left - 1;
+                        const int row = __builtin_amdgcn_readlane(r, e), slot = __builtin_amdgcn_readlane(s, e);
+                        const char* at = a.from.values + (((int64_t)row << (a.page_shift - 4)) + (slot >> 4)) * (D * 16 * SIZE);
 #pragma unroll
-                        for (int q = 0; q < SIZE; q++) {
-                            const u32x4 w = at[q];
+                        for (int x = 0; x < kHalves; x++)
 #pragma unroll
-                            for (int k = 0; k < 4; k++) from[4 * q + k] = w[k];
-                        }
+                            for (int q = 0; q < SIZE; q++) {
+                                const u32x4 w = *reinterpret_cast<const u32x4*>(at + min(64 * x + lane, D - 1) * (16 * SIZE) + 16 * q);
+#pragma unroll
+                                for (int k = 0; k < 4; k++) from[x][j * kWords + 4 * q + k] = w[k];
+                            }
                     }
-                    constexpr int kPerWord = 4 / SIZE;
-                    const int word = (s & 15) / kPerWord, shift = (s & 15) % kPerWord * 8 * SIZE;
-                    uint32_t x = from[0];
 #pragma unroll
-                    for (int k = 1; k < 4 * SIZE; k++) x = word == k ? from[k] : x;
-                    v[e / kPerWord] |= (x >> shift & (EIGHT ? 0xFFu : 0xFFFFu)) << (e % kPerWord * 8 * SIZE);
+                    for (int e = 0; e < kBlock; e++) {
+                        const int j = __builtin_popcount(begins & ((2u << e) - 1)) - 1 - base;
+                        if (!(held >> e & 1) || (uint32_t)j >= (uint32_t)kFrom) continue;
+                        const int slot = __builtin_amdgcn_readlane(s, e) & 15, word = __builtin_amdgcn_readfirstlane(j * kWords + slot / kPerWord), shift = slot % kPerWord * (8 * SIZE);
+#pragma unroll
+                        for (int x = 0; x < kHalves; x++) v[x][e / kPerWord] |= (from[x][word] >> shift & (EIGHT ? 0xFFu : 0xFFFFu)) << (e % kPerWord * 8 * SIZE);
+                    }
                 }
             }
             settled();
             if (into < 0) continue;
+            float f[EIGHT ? kBlock : 1];
+            bool even = true;                                               // no number is rounded anew
             if constexpr (EIGHT) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    float f[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) f[e] = factor(1, block * kBlock + 4 * q + e);
-                    if (f[0] == 1.f && f[1] == 1.f && f[2] == 1.f && f[3] == 1.f) continue;
-                    uint32_t out = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) out |= (f[e] == 1.f ? v[q] >> 8 * e & 255 : moved8(v[q] >> 8 * e & 255, f[e]) & 255) << 8 * e;
-                    v[q] = out;
+                for (int e = 0; e < kBlock; e++) {
+                    f[e] = factor(1, block * kBlock + e);
+                    even = even && f[e] == 1.f;
                 }
             }
             const int at = (w * kWindow + block * kBlock) & mask;
-            char* out = a.to.values + ((((int64_t)into << (a.page_shift - 4)) + (at >> 4)) * D + d) * (16 * SIZE);
-            if (held == 0xFFFF) {
+            char* out = a.to.values + (((int64_t)into << (a.page_shift - 4)) + (at >> 4)) * (D * 16 * SIZE);
 #pragma unroll
-                for (int q = 0; q < SIZE; q++) reinterpret_cast<u32x4*>(out)[q] = u32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-            } else {
-                // (what lies behind the last key stays as it is)
+            for (int x = 0; x < kHalves; x++) {
+                const int d = 64 * x + lane;
+                if (D % 64 && d >= D) continue;
+                if constexpr (EIGHT) {
+                    if (!even)
 #pragma unroll
-                for (int e = 0; e < kBlock; e++) {
-                    if (!(held >> e & 1)) continue;
-                    if constexpr (EIGHT) reinterpret_cast<uint8_t*>(out)[e] = (uint8_t)(v[e >> 2] >> 8 * (e & 3));
-                    else reinterpret_cast<uint16_t*>(out)[e] = (uint16_t)(v[e >> 1] >> 16 * (e & 1));
+                        for (int q = 0; q < 4; q++) {
+                            uint32_t moved = 0;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) moved |= (f[4 * q + e] == 1.f ? v[x][q] >> 8 * e & 255 : moved8(v[x][q] >> 8 * e & 255, f[4 * q + e]) & 255) << 8 * e;
+                            v[x][q] = moved;
+                        }
+                }
+                char* to = out + d * (16 * SIZE);
+                if (held == 0xFFFF) {
+#pragma unroll
+                    for (int q = 0; q < SIZE; q++) reinterpret_cast<u32x4*>(to)[q] = u32x4{v[x][4 * q], v[x][4 * q + 1], v[x][4 * q + 2], v[x][4 * q + 3]};
+                } else {
+                    // (what lies behind the last key stays as it is)
+#pragma unroll
+                    for (int e = 0; e < kBlock; e++) {
+                        if (!(held >> e & 1)) continue;
+                        if constexpr (EIGHT) reinterpret_cast<uint8_t*>(to)[e] = (uint8_t)(v[x][e >> 2] >> 8 * (e & 3));
+                        else reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)(v[x][e >> 1] >> 16 * (e & 1));
+                    }
                 }
             }
         }
@@ -413,13 +451,16 @@ extern "C" int mhip_paged_evict(void* stream, const mhip_paged_cache* cache, con
     char* room = static_cast<char*>(workspace);
     hipStream_t st = as_stream(stream);
     const SelectArgs sel{weights, seqs->table, seqs->lengths, reinterpret_cast<int32_t*>(room), left, (int)seqs->width, (int)cache->pages, (int)cache->heads, page_shift, (int)keep, (int)recent, least.cap};
-    auto select = [&](auto per) {
-        hipLaunchKernelGGL(evict_select_kernel<decltype(per)::value>, dim3((unsigned)(B * cache->heads)), dim3(kSelectThreads), 0, st, sel);
+    auto select = [&](auto per, auto lds) {
+        hipLaunchKernelGGL((evict_select_kernel<decltype(per)::value, decltype(lds)::value>), dim3((unsigned)(B * cache->heads)), dim3(kSelectThreads), 0, st, sel);
         return check_launch("paged_evict");
     };
-    using std::integral_constant;
-    const int rc_select = reach <= 4 * kSelectThreads ? select(integral_constant<int, 4>{}) : reach <= 16 * kSelectThreads ? select(integral_constant<int, 16>{})
-                        : reach <= 64 * kSelectThreads ? select(integral_constant<int, 64>{}) : select(integral_constant<int, 0>{});
+    constexpr std::integral_constant<int, 0> kNone{};
+    constexpr std::integral_constant<int, 4> kFour{};
+    constexpr std::integral_constant<int, 16> kSixteen{};
+    constexpr std::integral_constant<int, 32> kAll{};
+    const int rc_select = reach <= 4 * kSelectThreads ? select(kFour, kNone) : reach <= 16 * kSelectThreads ? select(kSixteen, kNone) : reach <= 32 * kSelectThreads ? select(kAll, kNone)
+                        : reach <= 64 * kSelectThreads ? select(kAll, kAll) : select(kNone, kNone);
     if (rc_select) return rc_select;
     const Pool here{(char*)cache->keys, (char*)cache->values, cache->key_scales, cache->value_scales, weights, seqs->table, (int)seqs->width, (int)cache->pages};
     Pool there = here, between{};
