@@ -57,6 +57,9 @@ struct PagedArgs {
     int last = 1;                             // kLeaves: the last of `starts`, in front of whose greatest the call's rows lie
     int32_t* dealt = nullptr;                 // kLeaves: [KV, tiles] pairs, where a tile's parts are (Split; no parts: it is whole, in `more`)
     int tiles = 0;
+    float* scores = nullptr;                  // kTells, few rows: [T, H, score_stride] scores in powers of two, 2^30 bytes at most; NULL: they are not kept
+    int score_stride = 0;                     // a multiple of 64
+    uint32_t score_bytes = 0;
 };
 
 // What becomes of a row's sums:
@@ -499,6 +502,16 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
 #pragma unroll
             for (int s = 0; s < NS; s++) queries[wave][s][lane] = qf[0][s];
         }
+        // kTells: where the row's scores go, behind what there is for no row
+        uint32_t scores_at[FORM == kTells ? TILES : 1];
+        if constexpr (FORM == kTells) {
+#pragma unroll
+            for (int x = 0; x < TILES; x++) {
+                const int row = tile * tile_rows + 16 * x + li, token = a.by_group(row);
+                const bool mine = row < rows && (!SINGLE || 16 * x + li < a.G);
+                scores_at[x] = mine && a.scores ? ((uint32_t)((first + token) * a.KV * a.G + head * a.G + row - token * a.G) * (uint32_t)a.score_stride + kLane * lg) * 4 : 0x80000000u;
+            }
+        }
         auto query = [&](int x, int s) __attribute__((always_inline)) {
             if constexpr (kQueriesInLds) return queries[wave][s][lane];
             else return qf[x][s];
@@ -616,6 +629,13 @@ __global__ __launch_bounds__(64 * WAVES, rows_kernel_workgroups(TILES, D, SINGLE
 #pragma unroll
                     for (int e = 0; e < 4 * NT; e++) sv[x][e] = e < n ? sv[x][e] : -INFINITY;
                 }
+                if constexpr (FORM == kTells)
+                    if (scores_at[x] != 0x80000000u) {                       // (lanes that have no row take none of the stores' time)
+                        const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(a.scores, 0, a.score_bytes, 0x00020000);
+#pragma unroll
+                        for (int j = 0; j < NT; j++)
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{sv[x][4 * j], sv[x][4 * j + 1], sv[x][4 * j + 2], sv[x][4 * j + 3]}), to, scores_at[x] + 16 * j, 4 * key, 0);
+                    }
                 float top = sv[x][0];
 #pragma unroll
                 for (int e = 1; e < 4 * NT; e++) top = fmaxf(top, sv[x][e]);
