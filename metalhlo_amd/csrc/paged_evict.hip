@@ -3,8 +3,11 @@
 //
 //   select   evict_select_kernel, a workgroup a sequence and head: the keep-th greatest weight by its bits, eleven at a time (a histogram of those that agree with it so far), then the positions of what
 //            stays in order, of equal weights the first ones.  Weights compare as numbers, NaN above all.
-//   move     evict_move_kernel, 256 places of a sequence and head at a time.  Keys are rows of bytes; values are gathered one by one, since a block holds sixteen tokens of a d.  In 8 bits a page takes
+//   move     evict_move_kernel, 256 places of a sequence and head at a time.  Keys are rows of bytes; a block holds sixteen tokens of a d, so that values change places in registers.  In 8 bits a page takes
 //            the greatest scale of those its keys come from, under which the others are rounded anew.
+//
+// us: 32 sequences of 2800 to 4000 keys, 8 heads of 128 in 8 bits, cut to 1750 (235 MB) 94: move 81, select 14; two of up to 50000 keys, 8 heads of 96 in 16 bits, cut to 8500 in place (107 MB) 120: select 65, which is
+// 16 workgroups' whole work, gather 52, copy 26.  The move is bound by vector instructions (42 in a hundred of its cycles) and by the latency of place -> page -> block in front of them.
 //
 // A key never moves backwards, so that where it lies and where it goes are the same pages a workgroup moves a sequence and head from the front on, each step read before it is written (IN_PLACE).
 // That is one compute unit's bandwidth a head: few heads are gathered into the workspace instead, by the whole device, and copied back.
@@ -237,8 +240,8 @@ __global__ __launch_bounds__(kWindow) void evict_move_kernel(MoveArgs a) {
         if (IN_PLACE) settled();
         if (row >= 0 && to >= 0) a.to.weights[((int64_t)to << a.page_shift) + (i & mask)] = weight;
 
-        // ---- keys, 64 * 16 pieces a turn
-        constexpr int kTurn = 4;
+        // ---- keys, a piece of sixteen bytes a thread, so many turns at once
+        constexpr int kTurn = 4;                                            // (us of 32 sequences, two | four | eight: 82.5 | 81 | 119)
         for (int p0 = 0; p0 < here * kPer; p0 += kTurn * kWindow) {
             // (the row that a piece goes to is held and asked about where it is stored: with a token's number set to -1 in the first loop instead, the compiler stored pieces whose page is none)
             u32x4 v[kTurn];
