@@ -6,8 +6,8 @@
 //   move     evict_move_kernel, 256 places of a sequence and head at a time.  Keys are rows of bytes; a block holds sixteen tokens of a d, so that values change places in registers.  In 8 bits a page takes
 //            the greatest scale of those its keys come from, under which the others are rounded anew.
 //
-// us: 32 sequences of 2800 to 4000 keys, 8 heads of 128 in 8 bits, cut to 1750 (235 MB) 94: move 81, select 14; two of up to 50000 keys, 8 heads of 96 in 16 bits, cut to 8500 in place (107 MB) 120: select 65, which is
-// 16 workgroups' whole work, gather 52, copy 26.  The move is bound by vector instructions (42 in a hundred of its cycles) and by the latency of place -> page -> block in front of them.
+// us: 32 sequences of 2800 to 4000 keys, 8 heads of 128 in 8 bits, cut to 1750 (235 MB) 85: move 73, select 14; two of up to 50000 keys, 8 heads of 96 in 16 bits, cut to 8500 in place (107 MB) 121: select 65, which is
+// 16 workgroups' whole work, gather 52, copy 26.  The move is one round of workgroups, each of which waits for place -> page -> block four times over.
 //
 // A key never moves backwards, so that where it lies and where it goes are the same pages a workgroup moves a sequence and head from the front on, each step read before it is written (IN_PLACE).
 // That is one compute unit's bandwidth a head: few heads are gathered into the workspace instead, by the whole device, and copied back.
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(kWindow) void evict_move_kernel(MoveArgs a) {
         if (row >= 0 && to >= 0) a.to.weights[((int64_t)to << a.page_shift) + (i & mask)] = weight;
 
         // ---- keys, a piece of sixteen bytes a thread, so many turns at once
-        constexpr int kTurn = 4;                                            // (us of 32 sequences, two | four | eight: 82.5 | 81 | 119)
+        constexpr int kTurn = 4;                                            // (us, 32 sequences, two | four | eight: 82.5 | 81 | 119)
         for (int p0 = 0; p0 < here * kPer; p0 += kTurn * kWindow) {
             // (the row that a piece goes to is held and asked about where it is stored: with a token's number set to -1 in the first loop instead, the compiler stored pieces whose page is none)
             u32x4 v[kTurn];
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(kWindow) void evict_move_kernel(MoveArgs a) {
             }
         }
         // ---- values: a wave sixteen places, a lane a d of them or two.  Their tokens come from a few blocks, whose sixteen tokens of a d are sixteen neighbouring numbers: four blocks are asked for at a
-        // time, and numbers change places in registers.  (32 sequences of 3400 keys cut to 1750: a load for each number 120 us, a block's numbers in one go but block after block 105, four blocks 81.)
+        // time, and numbers change places in registers.  (32 sequences of 3400 keys cut to 1750: a load for each number 120 us, a block's numbers in one go but block after block 105, four blocks 81; numbers that are rounded anew four in a word and not one by one, 73.)
         constexpr int kHalves = (D + 63) / 64, kFrom = 4, kWords = 4 * SIZE, kPerWord = 4 / SIZE;
         typedef uint32_t Words __attribute__((ext_vector_type(kFrom * kWords)));
         for (int block0 = 0; block0 * kBlock < here; block0 += kWindow / 64) {
@@ -315,11 +315,10 @@ __global__ __launch_bounds__(kWindow) void evict_move_kernel(MoveArgs a) {
             float f[EIGHT ? kBlock : 1];
             bool even = true;                                               // no number is rounded anew
             if constexpr (EIGHT) {
+                const float own = factor(1, block * kBlock + (lane & 15));
+                even = !__any(own != 1.f);
 #pragma unroll
-                for (int e = 0; e < kBlock; e++) {
-                    f[e] = factor(1, block * kBlock + e);
-                    even = even && f[e] == 1.f;
-                }
+                for (int e = 0; e < kBlock; e++) f[e] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, own), e));
             }
             const int at = (w * kWindow + block * kBlock) & mask;
             char* out = a.to.values + (((int64_t)into << (a.page_shift - 4)) + (at >> 4)) * (D * 16 * SIZE);
@@ -331,10 +330,9 @@ __global__ __launch_bounds__(kWindow) void evict_move_kernel(MoveArgs a) {
                     if (!even)
 #pragma unroll
                         for (int q = 0; q < 4; q++) {
-                            uint32_t moved = 0;
-#pragma unroll
-                            for (int e = 0; e < 4; e++) moved |= (f[4 * q + e] == 1.f ? v[x][q] >> 8 * e & 255 : moved8(v[x][q] >> 8 * e & 255, f[4 * q + e]) & 255) << 8 * e;
-                            v[x][q] = moved;
+                            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(v[x][q], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(v[x][q], true);
+                            const float y[4] = {lo[0] * f[4 * q], lo[1] * f[4 * q + 1], hi[0] * f[4 * q + 2], hi[1] * f[4 * q + 3]};       // (under its own scale a number is itself again)
+                            v[x][q] = pack8(y, 1.f, 448.f);
                         }
                 }
                 char* to = out + d * (16 * SIZE);
