@@ -342,7 +342,8 @@ int mhip_paged_attention_shared(void* stream, const mhip_paged_cache* cache, con
 
 /* mhip_paged_attention, bit for bit, that also adds the weights it gives up: weights [pages, heads, page_size] in fp32 of each key get the sum over the call's tokens and the query heads of the key's head of
  * the softmax weight.  Keys of the call's own tokens begin at zero whatever is there; those of sequences without tokens, and slots that hold no key, stay as they are.  A page belongs to one sequence.
- * A key of a row whose scores hold a NaN gets NaN.  o overlaps nothing of the call.  Sums are fp32 in a fixed order.  The workspace is needed (`least` as above). */
+ * A key of a row whose scores hold a NaN gets NaN.  o overlaps nothing of the call.  Sums are fp32 in a fixed order.  The workspace is needed (`least` as above); up to 2^30
+ * bytes of what is of use are for the scores of few rows, without which the keys are read twice. */
 int64_t mhip_paged_attention_weighed_workspace(const mhip_paged_cache* cache, const mhip_sequences* seqs, int64_t q_heads, int64_t* least);
 int mhip_paged_attention_weighed(void* stream, const mhip_paged_cache* cache, const mhip_sequences* seqs, const void* q, void* o, float* weights, int64_t q_heads, float scale, int is_causal,
                                  const int64_t* strides, int dtype, void* workspace, int64_t workspace_bytes);

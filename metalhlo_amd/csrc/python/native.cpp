@@ -703,7 +703,8 @@ FUNCTION(paged_evict) {
         if (table.dim() != 2 || lengths.dim() != 1 || lengths.size(0) != table.size(0)) raise(PyExc_ValueError, "table must be [sequences, width] and lengths [sequences]");
         if (into && (into->dim() != 2 || into->size(0) != table.size(0))) raise(PyExc_ValueError, "into must be [sequences, width]");
         if (keep < 0 || recent < 0) raise(PyExc_ValueError, "keys to keep are negative");
-        if (into && into->size(1) * cache.c.page_size < std::min(keep + recent, table.size(1) * cache.c.page_size)) raise(PyExc_ValueError, "into has no room for what stays");
+        const int64_t most = (int64_t)1 << 31;                              // (more is refused below)
+        if (into && into->size(1) * cache.c.page_size < std::min(std::min(keep, most) + std::min(recent, most), table.size(1) * cache.c.page_size)) raise(PyExc_ValueError, "into has no room for what stays");
         const mhip_sequences seqs{table.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), nullptr, table.size(0), table.size(1), 0};
         at::Tensor left = empty({table.size(0)}, at::kInt, table);
         int64_t least = 0;

@@ -91,3 +91,14 @@ def test_offsets_past_32_bits(B, new, eight):
         results.append([shared, out, left, w[offset:offset + few], *(x[offset:offset + few] for x in cache if x is not None)])
     for a, b in zip(*results):
         assert torch.equal(a.view(torch.uint8) if a.dtype == torch.float8_e4m3fn else a, b.view(torch.uint8) if b.dtype == torch.float8_e4m3fn else b)
+
+
+@gpu
+def test_numbers_to_keep_that_no_integer_adds_up():
+    from metalhlo_amd import kernels
+    cache = kernels.paged_cache(4, 1, 16, 32, torch.bfloat16)
+    weights, table = torch.zeros(4, 1, 16, device="cuda"), ints([[0, 1]])
+    for keep, recent in ((2 ** 62, 2 ** 62), (2 ** 63 - 1, 1), (1, 2 ** 63 - 1), (2 ** 30 + 1, 0)):
+        for into in (None, ints([[2]]), ints([[2, 3]])):
+            with pytest.raises((ValueError, RuntimeError)):
+                kernels.paged_evict(cache, weights, table, ints([20]), keep, recent, into)
