@@ -6,8 +6,8 @@
 //   move     evict_move_kernel, 256 places of a sequence and head at a time.  Keys are rows of bytes; a block holds sixteen tokens of a d, so that values change places in registers.  In 8 bits a page takes
 //            the greatest scale of those its keys come from, under which the others are rounded anew.
 //
-// us: 32 sequences of 2800 to 4000 keys, 8 heads of 128 in 8 bits, cut to 1750 (235 MB) 85: move 73, select 14; two of up to 50000 keys, 8 heads of 96 in 16 bits, cut to 8500 in place (107 MB) 121: select 65, which is
-// 16 workgroups' whole work, gather 52, copy 26.  The move is one round of workgroups, each of which waits for place -> page -> block four times over.
+// us: 32 sequences of 2800 to 4000 keys, 8 heads of 128 in 8 bits, cut to 1750 (235 MB) 80: move 67, select 14; two of up to 50000 keys, 8 heads of 96 in 16 bits, cut to 8500 in place (107 MB) 119: select 65, which is
+// 16 workgroups' whole work, gather 53, copy 23.  The move is one round of workgroups, each of which waits for place -> page -> block four times over.
 //
 // A key never moves backwards, so that where it lies and where it goes are the same pages a workgroup moves a sequence and head from the front on, each step read before it is written (IN_PLACE).
 // That is one compute unit's bandwidth a head: few heads are gathered into the workspace instead, by the whole device, and copied back.
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(kWindow) void evict_move_kernel(MoveArgs a) {
             }
         }
         // ---- values: a wave sixteen places, a lane a d of them or two.  Their tokens come from a few blocks, whose sixteen tokens of a d are sixteen neighbouring numbers: four blocks are asked for at a
-        // time, and numbers change places in registers.  (32 sequences of 3400 keys cut to 1750: a load for each number 120 us, a block's numbers in one go but block after block 105, four blocks 81; numbers that are rounded anew four in a word and not one by one, 73.)
+        // time, and numbers change places in registers.  (32 sequences of 3400 keys cut to 1750: a load for each number 120 us, a block's numbers in one go but block after block 105, four blocks 81; numbers that are rounded anew four in a word and not one by one, 73; bytes put in their place by one instruction, 67.)
         constexpr int kHalves = (D + 63) / 64, kFrom = 4, kWords = 4 * SIZE, kPerWord = 4 / SIZE;
         typedef uint32_t Words __attribute__((ext_vector_type(kFrom * kWords)));
         for (int block0 = 0; block0 * kBlock < here; block0 += kWindow / 64) {
@@ -282,6 +282,11 @@ __global__ __launch_bounds__(kWindow) void evict_move_kernel(MoveArgs a) {
                 const int r1 = __shfl_up(r, 1, 64), s1 = __shfl_up(s, 1, 64);
                 held = (uint32_t)__ballot(r >= 0) & 0xFFFFu;
                 const uint32_t begins = (uint32_t)__ballot(r >= 0 && ((lane & 15) == 0 || r != r1 || s >> 4 != s1 >> 4)) & 0xFFFFu;      // tokens that are the first of their block
+                // of token e in lane e: the word of its block's that it lies in, counted over all blocks (behind them for none), and which bytes of that and of the word it goes to make the latter
+                const int order = __builtin_popcount(begins & ((2u << (lane & 15)) - 1)) - 1;
+                const uint32_t one = (uint32_t)(s % kPerWord * SIZE) + 4, place = (uint32_t)(lane % kPerWord) * (8 * SIZE);
+                const int words = r >= 0 ? order * kWords + (s & 15) / kPerWord : kBlock * kWords;
+                const uint32_t bytes = EIGHT ? (0x03020100u & ~(0xFFu << place)) | one << place : (0x03020100u & ~(0xFFFFu << place)) | (one | (one + 1) << 8) << place;
                 uint32_t left = begins;
                 for (int base = 0; left; base += kFrom) {
                     Words from[kHalves];
@@ -300,14 +305,18 @@ __global__ __launch_bounds__(kWindow) void evict_move_kernel(MoveArgs a) {
                                 for (int k = 0; k < 4; k++) from[x][j * kWords + 4 * q + k] = w[k];
                             }
                     }
+                    auto put = [&](auto whole) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int e = 0; e < kBlock; e++) {
-                        const int j = __builtin_popcount(begins & ((2u << e) - 1)) - 1 - base;
-                        if (!(held >> e & 1) || (uint32_t)j >= (uint32_t)kFrom) continue;
-                        const int slot = __builtin_amdgcn_readlane(s, e) & 15, word = __builtin_amdgcn_readfirstlane(j * kWords + slot / kPerWord), shift = slot % kPerWord * (8 * SIZE);
+                        for (int e = 0; e < kBlock; e++) {
+                            const int word = __builtin_amdgcn_readlane(words, e) - base * kWords;
+                            if (!decltype(whole)::value && (uint32_t)word >= (uint32_t)(kFrom * kWords)) continue;
+                            const uint32_t which = __builtin_amdgcn_readlane(bytes, e);
 #pragma unroll
-                        for (int x = 0; x < kHalves; x++) v[x][e / kPerWord] |= (from[x][word] >> shift & (EIGHT ? 0xFFu : 0xFFFFu)) << (e % kPerWord * 8 * SIZE);
-                    }
+                            for (int x = 0; x < kHalves; x++) v[x][e / kPerWord] = __builtin_amdgcn_perm(from[x][word], v[x][e / kPerWord], which);
+                        }
+                    };
+                    if (held == 0xFFFF && base == 0 && !left) put(std::true_type{});      // (all sixteen are of these blocks)
+                    else put(std::false_type{});
                 }
             }
             settled();
