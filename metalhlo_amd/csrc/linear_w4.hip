@@ -139,7 +139,7 @@ __global__ __launch_bounds__(64 * WN * WK) void w4_rows_kernel(W4Args g) {
             }
         }
     };
-    // ---- a block's words are asked for U blocks ahead
+    // ---- a block's words are asked for U blocks ahead, across the chunks of x: a wave's next block is in blk[0] again behind U WK blocks, so that all chunks but a part's last are whole turns of so many (few_of)
     Block blk[U];
 #pragma unroll
     for (int u = 0; u < U; u++)
@@ -390,6 +390,8 @@ Wide wide_of(int64_t M, const mhip_w4* w, bool even, int dtype) {
 // two blocks a wave 22.7, four 14.7).
 constexpr int kFew = 4, kWavesWanted = 2560, kWavesOfFew = 4096, kLdsOfFew = 64 << 10;
 struct Few { int mt, wn, wk, strips, blocks, parts, per, chunk; int64_t bytes; };
+// Blocks of words that a wave has on their way: what the registers hold; four groups' pairs are as many as their weights.
+constexpr int blocks_ahead(int group) { return group == 32 ? 2 : 4; }
 Few few_of(int64_t M, int group, int n16, int k128, bool deal) {
     Few f{};
     f.mt = M <= 16 ? 1 : M <= 32 || group == 32 ? 2 : 4;                     // (four sets of sums and four groups' pairs do not fit the registers)
@@ -406,7 +408,8 @@ Few few_of(int64_t M, int group, int n16, int k128, bool deal) {
     }
     f.per = (k128 + f.parts - 1) / f.parts;
     f.parts = (k128 + f.per - 1) / f.per;
-    f.chunk = std::min(kLdsOfFew / ((int)std::min<int64_t>(M, kFew) * (kBlockK * 2) + 16), f.per);
+    const int room = kLdsOfFew / ((int)std::min<int64_t>(M, kFew) * (kBlockK * 2) + 16), turn = blocks_ahead(group) * f.wk;
+    f.chunk = room < f.per ? room / turn * turn : f.per;                     // (a whole number of turns of the words: 240 | 112 | 80 | 48 blocks of one to four rows)
     f.bytes = f.parts > 1 ? up((int64_t)f.strips * f.blocks * 8, 16) + (int64_t)f.strips * f.blocks * f.parts * f.wn * f.mt * 1024 : 0;
     return f;
 }
@@ -426,7 +429,7 @@ int launch_rows(hipStream_t st, const W4Args& a, const Few& f) {
 
 template <typename T, int GROUP>
 int launch_group(hipStream_t st, const W4Args& a, const Few& f) {
-    constexpr int U = GROUP == 32 ? 2 : 4;                                   // (words ahead: what the registers hold; four groups' pairs are as many as their weights)
+    constexpr int U = blocks_ahead(GROUP);
     if (f.wn == 1) return launch_rows<T, GROUP, 1, 1, 4, U, 0, kFew>(st, a, f);
     if (f.mt == 1) return launch_rows<T, GROUP, 1, 2, 4, U, 2, 16>(st, a, f);
     if constexpr (GROUP != 32) {

@@ -344,3 +344,52 @@ def test_refusals_of_the_entry_points(lib):
     quantize = lambda w, src=16, t=1, dtype=3: lib.mhip_quantize_w4(None, src, 1, 1, w, t, dtype)  # noqa: E731
     assert quantize(held(group=1)) == 2 and quantize(held(), t=7) == 2 and quantize(held(), src=None) == 1 and quantize(held(scales=None)) == 1 and quantize(held(scales=8)) == 2 and quantize(held(K=0)) == 0
     assert lib.mhip_linear_w4_workspace(500, held(N=-1), 3) == 0 and lib.mhip_linear_w4_workspace(500, None, 3) == 0
+
+
+# ---- rows whose part of K is more than x's room in LDS
+
+def wide_layer(N, K, group, dtype, seed):
+    from metalhlo_amd import kernels
+    n16, k128, g = -(-N // 16), -(-K // 128), torch.Generator(device="cuda").manual_seed(seed)
+    words = torch.randint(-2 ** 31, 2 ** 31, (n16, k128, 64, 4), generator=g, device="cuda", dtype=torch.int32)
+    scales = torch.empty(n16, k128 * (128 // group), 16, 2, device="cuda")
+    scales[..., 0].uniform_(0.05, 0.15, generator=g)
+    scales[..., 1] = torch.randint(0, 16, scales.shape[:3], generator=g, device="cuda")
+    scales[:, -(-K // group):] = 0
+    scales.view(n16, -1, 16, 2)[-1, :, N - 16 * (n16 - 1):] = 0
+    return kernels.W4(words, scales.to(dtype), N, K, group)
+
+
+def rows_of(w, tiles):
+    """(q, scale, zero) [16 tiles, K] in 64 bits of those sixteens of rows."""
+    from metalhlo_amd import kernels
+    some = kernels.W4(w.words[tiles], w.scales[tiles], 16 * len(tiles), w.K, w.group)
+    return tuple(t[:, :w.K] for t in unpacked(some))
+
+
+@gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("N,K", [(28672, 8192), (12000, 8200), (12288, 12288), (11008, 16384), (8192, 28672)])
+def test_few_rows_of_wide_layers(M, N, K, group):
+    """One to five rows through layers that are long and wide, whose K few workgroups or none share."""
+    from metalhlo_amd import kernels
+    w = wide_layer(N, K, group, torch.bfloat16, K + M)
+    x = normal((M, K), torch.bfloat16, M)
+    got = kernels.linear_w4(x, w)
+    tiles = [0, 1, N // 32, N // 16 - 1]
+    parts = rows_of(w, tiles)
+    check(got.view(M, N // 16, 16)[:, tiles].reshape(M, -1), x, parts)
+
+
+@gpu
+@TYPES
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,K", [(1, 31000), (1, 40001), (2, 15873), (2, 33000), (3, 10625), (3, 20000), (4, 8065), (4, 9000), (4, 30001), (5, 20000)])
+def test_few_rows_of_a_long_K_without_a_workspace(M, K, group, dtype):
+    from metalhlo_amd import _lib, kernels
+    w = wide_layer(48, K, group, dtype, K)
+    x, out = normal((M, K), dtype), torch.full((M, 48), 7, dtype=dtype, device="cuda")
+    held = Held(w.words.data_ptr(), w.scales.data_ptr(), 48, K, group)
+    _lib.check(_lib.load().mhip_linear_w4(torch.cuda.current_stream().cuda_stream, x.data_ptr(), ctypes.byref(held), None, None, out.data_ptr(), M, 0, kernels.DTYPE_CODE[dtype], None, 0))
+    check(out, x, rows_of(w, [0, 1, 2]))
