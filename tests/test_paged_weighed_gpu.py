@@ -262,6 +262,36 @@ def test_other_streams_and_graphs(new, eight):
 
 
 @gpu
+@EIGHT
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+@pytest.mark.parametrize("new,row", [(2, 0), (3, 0), (3, 1), (4, 2), (9, 3), (9, 5)])
+def test_a_row_that_is_not_finite_gives_later_keys_nothing(new, row, what, eight):
+    """Of a prompt's tokens one whose scores are not finite: the keys that it sees get NaN, those of later tokens do not, whether the scores are kept in the workspace or formed again."""
+    from metalhlo_amd import _lib, kernels
+    from tests.test_serving_host import Cache, Sequences
+    lib = _lib.load()
+    for context in (28, 29, 30, 31):
+        q, cache, table, keys, starts, before = make([new] * 2, [20, context], 4, 2, 64, 16, torch.bfloat16, eight, width=8)
+        q[starts[1] + row, 1, 5] = what
+        held, qd, t, n, s = cache.to_device(), q.cuda(), ints(table), ints(keys), ints(starts)
+        c = Cache(held.keys.data_ptr(), held.values.data_ptr(), *(0 if x is None else x.data_ptr() for x in held[2:]), *held.keys.shape)
+        seqs = Sequences(t.data_ptr(), n.data_ptr(), s.data_ptr(), 2, 8, 2 * new)
+        least = ctypes.c_int64()
+        need = lib.mhip_paged_attention_weighed_workspace(ctypes.byref(c), ctypes.byref(seqs), 4, ctypes.byref(least))
+        assert need > least.value > 0
+        room, strides = torch.empty(need, dtype=torch.uint8, device="cuda"), (ctypes.c_int64 * 4)(4 * 64, 64, 4 * 64, 64)
+        for size in (least.value, need):
+            out, weights = torch.empty_like(qd), before.cuda()
+            _lib.check(lib.mhip_paged_attention_weighed(torch.cuda.current_stream().cuda_stream, ctypes.byref(c), ctypes.byref(seqs), qd.data_ptr(), out.data_ptr(), weights.data_ptr(), 4, 0.125, 1,
+                                                        strides, kernels.DTYPE_CODE[torch.bfloat16], room.data_ptr(), size))
+            w = weights.cpu()
+            for b in range(2):
+                for i in range(keys[b]):
+                    at = w[int(table[b, i // 16]), :, i % 16]
+                    assert bool(torch.isnan(at[0])) == (b == 1 and i <= context + row) and torch.isfinite(at[1]), (context, size == need, b, i)
+
+
+@gpu
 @pytest.mark.parametrize("dtype,eight", [(torch.bfloat16, False), (torch.float16, True)], ids=["bf16", "f16 8bit"])
 def test_a_run_of_steps(dtype, eight):
     """Prompts, decode steps and evictions as a program takes them, behind a prefix in common and with 4-bit projections: every step's operators against plain ones over the keys that are left."""
