@@ -8,7 +8,8 @@
 //
 // A byte 0 .. 15 is that number times 2^-9 as e4m3, across the border of its subnormals: one v_cvt_scalef32_pk per two weights makes 16-bit numbers q, exactly, of bytes that a mask and a shift have made.
 // The products of q and x are added over a group in the matrix unit, and so is x itself (an operand of ones, so that each lane of the result has the sum of its own row): what a group
-// adds to a result is s (sum q x - z sum x), in fp32 and of numbers that are exact.
+// adds to a result is s (sum q x - z sum x), in fp32 and of numbers that are exact.  Of an infinite x, and of a bf16 x whose sums pass fp32's range, that makes a NaN or an infinity where W x need not have one: results
+// that are not finite are added up once more, weight by weight.
 //
 // Few rows: w4_rows_kernel, whose time is that of reading W.  Many: W is rounded to 16 bits into the workspace and multiplied by mhip_gemm (kManyRows).
 #include <algorithm>
@@ -242,10 +243,42 @@ __global__ __launch_bounds__(64 * WN * WK) void w4_rows_kernel(W4Args g) {
                     if (q0 + q < g.parts) sum[i] += v[q][i];
         }
     }
+    // Four neighbouring results by themselves, from row `first` of sixteen on: s (q - z) is a number, and x meets it as it is.  (A thread's own loop over K, a millisecond for 28672 columns, and over at once where x holds a NaN.)
+    auto by_weights = [&](int row, int sixteen, int first) __attribute__((always_inline)) {
+        f32x4 y = {0.f, 0.f, 0.f, 0.f};
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(g.words4 + (int64_t)sixteen * g.k128 * 64 + first);
+        const uint32_t* pairs = g.scales + (int64_t)sixteen * g.k128 * (kGroups * 16) + first;
+#pragma unroll 1
+        for (int k = 0; k < g.K; k += 8) {
+            const u32x4 eight = piece(row, k);
+            const int64_t kb = k / kBlockK;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint32_t word = words[(kb * 64 + 16 * (k / 8 % 4) + r) * 4 + k / 32 % 4], pair = pairs[(k / GROUP) * (int64_t)16 + r];
+                const float scale = low_half<T>(pair), zero = high_half<T>(pair);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float q = (float)(word >> (8 * (e & 3) + 4 * (e >> 2)) & 15);
+                    y[r] = fmaf(scale * (q - zero), e & 1 ? high_half<T>(eight[e >> 1]) : low_half<T>(eight[e >> 1]), y[r]);
+                }
+            }
+            if (y[0] != y[0] && y[1] != y[1] && y[2] != y[2] && y[3] != y[3]) break;
+        }
+        return y;
+    };
 #pragma unroll
     for (int i = 0; i < kMine; i++) {
         const int t = threadIdx.x + i * kThreads, row = 16 * (t / 64 % MT) + (t & 15), col = (strip * WN + t / (64 * MT)) * 16 + 4 * (t >> 4 & 3);
         if (t >= kItems || row >= rows || col >= g.N) continue;
+        bool finite = true;
+#pragma unroll
+        for (int e = 0; e < 4; e++) finite = finite && fabsf(sum[i][e]) < INFINITY;
+        if (!finite) {
+            const f32x4 y = by_weights(row, col / 16, col % 16);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (!(fabsf(sum[i][e]) < INFINITY)) sum[i][e] = y[e];
+        }
         const int64_t place = (int64_t)(m0 + row) * g.N + col;
         T* c = static_cast<T*>(g.c) + place;
         const T *res = static_cast<const T*>(g.residual) + place, *bias = static_cast<const T*>(g.bias) + col;

@@ -393,3 +393,67 @@ def test_few_rows_of_a_long_K_without_a_workspace(M, K, group, dtype):
     held = Held(w.words.data_ptr(), w.scales.data_ptr(), 48, K, group)
     _lib.check(_lib.load().mhip_linear_w4(torch.cuda.current_stream().cuda_stream, x.data_ptr(), ctypes.byref(held), None, None, out.data_ptr(), M, 0, kernels.DTYPE_CODE[dtype], None, 0))
     check(out, x, rows_of(w, [0, 1, 2]))
+
+
+# ---- infinities and great numbers.  A row whose sums of groups are not finite is added up weight by weight: K + 3 roundings at most of numbers whose magnitudes add up to S
+
+def same_as_infinite(got, x, parts):
+    """Rows in which W x holds infinities are these, NaN where they cancel or meet a weight of zero."""
+    q, s, z = parts
+    terms = ((q - z) * s)[None] * x.double().cpu()[:, None]                  # [rows, N, K]
+    want = terms.sum(2)
+    assert not torch.isfinite(want).any()
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[~torch.isnan(want)], want[~torch.isnan(want)])
+
+
+@gpu
+@TYPES
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M", [1, 3, 16, 30, 100])
+def test_infinities(M, group, dtype):
+    from metalhlo_amd import kernels
+    words, scales, parts = random_w4(50, 1100, group, dtype, M, whole=group != 64)
+    w = layer(words, scales, parts, group)
+    x = normal((M, 1100), dtype, M)
+    clean = kernels.linear_w4(x, w)
+    rows = sorted({0, M // 2, M - 1})
+    inf = float("inf")
+    for places in ([(7, inf)], [(1099, -inf)], [(40, inf), (700, inf)], [(500, inf), (501, -inf)]):
+        one = x.clone()
+        for row in rows:
+            for k, v in places:
+                one[row, k] = v
+        got, rest = kernels.linear_w4(one, w), [r for r in range(M) if r not in rows]
+        same_as_infinite(got[rows], one[rows], parts)
+        assert torch.equal(got[rest], clean[rest])
+        bias, residual = normal((50,), dtype, 2), normal((M, 50), dtype, 3)
+        both = kernels.linear_w4(one, w, bias, "relu", residual)[rows].float()
+        plain = got[rows].float().relu() + residual[rows].float()
+        assert torch.equal(both[got[rows] == inf], plain[got[rows] == inf]) and ((both - residual[rows].float())[got[rows] == -inf] == 0).all()
+        one[rows[0], 3] = float("nan")
+        assert torch.isnan(kernels.linear_w4(one, w)[rows[0]]).all()
+
+
+@gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,K", [(1, 264), (3, 4104), (12, 1000), (30, 264), (100, 1001)])
+def test_great_numbers(M, K, group):
+    """Groups whose sums of q x are beyond the greatest fp32 number, in results that are not."""
+    from metalhlo_amd import kernels
+    words, scales, parts = random_w4(50, K, group, torch.bfloat16, M)
+    scales = scales * torch.tensor([0.125, 1.0], dtype=torch.bfloat16)
+    parts = (parts[0], parts[1] * 0.125, parts[2])
+    w, x = layer(words, scales, parts, group), normal((M, K), torch.bfloat16)
+    rows = sorted({0, M // 2, M - 1})
+    for row in rows:
+        for k, sign in ((0, 1), (3, 1), (9, -1), (17, 1), (30, 1), (K - 1, -1)):
+            x[row, k] = sign * 2.0e38
+    got = kernels.linear_w4(x, w)
+    q, s, z = parts
+    x64 = x.double().cpu()
+    want, total = x64 @ ((q - z) * s).t(), x64.abs() @ ((q + z) * s).t()
+    assert want.abs().max() > 1e37 and want.abs().max() < 3.2e38
+    err = max(128 + K / 128 + 16, K + 3) * 2.0 ** -24 * total
+    err = err + 2.0 ** -8 * (want.abs() + err)
+    assert ((got.double().cpu() - want).abs() <= err).all()
