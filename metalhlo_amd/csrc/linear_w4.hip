@@ -243,42 +243,48 @@ __global__ __launch_bounds__(64 * WN * WK) void w4_rows_kernel(W4Args g) {
                     if (q0 + q < g.parts) sum[i] += v[q][i];
         }
     }
-    // Four neighbouring results by themselves, from row `first` of sixteen on: s (q - z) is a number, and x meets it as it is.  (A thread's own loop over K, a millisecond for 28672 columns, and over at once where x holds a NaN.)
+    // Four neighbouring results by themselves, from row `first` of sixteen on, by a wave whose lanes share K eight columns at a time: s (q - z) is a number, and x meets it as it is.  (us, one row of 4096 x 14336 with
+    // an infinity: 32, of which 10 are the product, and 826 with each lane by itself; a NaN ends it within 512 columns.)
     auto by_weights = [&](int row, int sixteen, int first) __attribute__((always_inline)) {
         f32x4 y = {0.f, 0.f, 0.f, 0.f};
         const uint32_t* words = reinterpret_cast<const uint32_t*>(g.words4 + (int64_t)sixteen * g.k128 * 64 + first);
         const uint32_t* pairs = g.scales + (int64_t)sixteen * g.k128 * (kGroups * 16) + first;
 #pragma unroll 1
-        for (int k = 0; k < g.K; k += 8) {
-            const u32x4 eight = piece(row, k);
-            const int64_t kb = k / kBlockK;
+        for (int k0 = 0; k0 < g.K; k0 += 512) {
+            const int k = k0 + 8 * lane;
+            if (k < g.K) {
+                const u32x4 eight = piece(row, k);
+                const int64_t kb = k / kBlockK;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const uint32_t word = words[(kb * 64 + 16 * (k / 8 % 4) + r) * 4 + k / 32 % 4], pair = pairs[(k / GROUP) * (int64_t)16 + r];
-                const float scale = low_half<T>(pair), zero = high_half<T>(pair);
+                for (int r = 0; r < 4; r++) {
+                    const uint32_t word = words[(kb * 64 + 16 * (k / 8 % 4) + r) * 4 + k / 32 % 4], pair = pairs[(k / GROUP) * (int64_t)16 + r];
+                    const float scale = low_half<T>(pair), zero = high_half<T>(pair);
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float q = (float)(word >> (8 * (e & 3) + 4 * (e >> 2)) & 15);
-                    y[r] = fmaf(scale * (q - zero), e & 1 ? high_half<T>(eight[e >> 1]) : low_half<T>(eight[e >> 1]), y[r]);
+                    for (int e = 0; e < 8; e++) {
+                        const float q = (float)(word >> (8 * (e & 3) + 4 * (e >> 2)) & 15);
+                        y[r] = fmaf(scale * (q - zero), e & 1 ? high_half<T>(eight[e >> 1]) : low_half<T>(eight[e >> 1]), y[r]);
+                    }
                 }
             }
-            if (y[0] != y[0] && y[1] != y[1] && y[2] != y[2] && y[3] != y[3]) break;
+            if (__any(y[0] != y[0]) && __any(y[1] != y[1]) && __any(y[2] != y[2]) && __any(y[3] != y[3])) break;
         }
+#pragma unroll
+        for (int r = 0; r < 4; r++) y[r] = wave_sum(y[r]);
         return y;
     };
 #pragma unroll
     for (int i = 0; i < kMine; i++) {
         const int t = threadIdx.x + i * kThreads, row = 16 * (t / 64 % MT) + (t & 15), col = (strip * WN + t / (64 * MT)) * 16 + 4 * (t >> 4 & 3);
-        if (t >= kItems || row >= rows || col >= g.N) continue;
-        bool finite = true;
-#pragma unroll
-        for (int e = 0; e < 4; e++) finite = finite && fabsf(sum[i][e]) < INFINITY;
-        if (!finite) {
-            const f32x4 y = by_weights(row, col / 16, col % 16);
+        const bool mine = t < kItems && row < rows && col < g.N;
+        auto wild = [&](int e) __attribute__((always_inline)) { return !(fabsf(sum[i][e]) < INFINITY); };
+        for (uint64_t left = __ballot(mine && (wild(0) || wild(1) || wild(2) || wild(3))); left; left &= left - 1) {
+            const int l = __builtin_ctzll(left), at = __builtin_amdgcn_readlane(col, l);
+            const f32x4 y = by_weights(__builtin_amdgcn_readlane(row, l), at / 16, at % 16);
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (!(fabsf(sum[i][e]) < INFINITY)) sum[i][e] = y[e];
+                if (lane == l && wild(e)) sum[i][e] = y[e];
         }
+        if (!mine) continue;
         const int64_t place = (int64_t)(m0 + row) * g.N + col;
         T* c = static_cast<T*>(g.c) + place;
         const T *res = static_cast<const T*>(g.residual) + place, *bias = static_cast<const T*>(g.bias) + col;

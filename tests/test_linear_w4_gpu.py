@@ -457,3 +457,18 @@ def test_great_numbers(M, K, group):
     err = max(128 + K / 128 + 16, K + 3) * 2.0 ** -24 * total
     err = err + 2.0 ** -8 * (want.abs() + err)
     assert ((got.double().cpu() - want).abs() <= err).all()
+
+
+@gpu
+@pytest.mark.parametrize("group", [32, 128])
+def test_as_many_rows_as_there_may_be(group):
+    from metalhlo_amd import _lib, kernels
+    M, K, N = 1 << 21, 40, 8
+    words, scales, parts = random_w4(N, K, group, torch.float16)
+    x, w = torch.randn(M, K, generator=torch.Generator("cuda").manual_seed(0), device="cuda").half(), layer(words, scales, parts, group)
+    out = torch.full((M, N), 7, dtype=torch.float16, device="cuda")
+    held = Held(w.words.data_ptr(), w.scales.data_ptr(), N, K, group)
+    _lib.check(_lib.load().mhip_linear_w4(torch.cuda.current_stream().cuda_stream, x.data_ptr(), ctypes.byref(held), None, None, out.data_ptr(), M, 0, kernels.DTYPE_CODE[x.dtype], None, 0))
+    some = [0, 31, 32, 63, 64, M // 2, M - 65, M - 64, M - 33, M - 32, M - 1]
+    check(out[some], x[some], parts)
+    check(kernels.linear_w4(x, w)[-200:], x[-200:], parts)
