@@ -335,6 +335,7 @@ int mhip_paged_attention(void* stream, const mhip_paged_cache* cache, const mhip
 /* The same for sequences that have a prefix in common, which is read once for all of them: o = softmax(scale * q [K_prefix; K_own]^T, causal) [V_prefix; V_own].  The prefix's first prefix_length[0] keys
  * lie in the pages prefix [prefix_width] of the same cache; all of it is device memory.  Every token sees all of them; its sequence's own keys, which seqs describes as ever (lengths count them alone), it sees by the causal rule.
  * An empty prefix, and a sequence without keys of its own, are allowed; a token without any keys yields zeros.  o may be q, and overlaps nothing else.
+ * mhip_paged_append turns by a sequence's own positions: tokens behind a prefix of P keys are appended with freqs from row P on.
  * The workspace is needed: mhip_paged_attention_shared_workspace says how much is of use and, in `least`, what suffices; 16-byte aligned, overwritten. */
 int64_t mhip_paged_attention_shared_workspace(const mhip_paged_cache* cache, int64_t prefix_width, const mhip_sequences* seqs, int64_t q_heads, int64_t* least);
 int mhip_paged_attention_shared(void* stream, const mhip_paged_cache* cache, const int32_t* prefix, int64_t prefix_width, const int32_t* prefix_length, const mhip_sequences* seqs, const void* q, void* o,
@@ -352,7 +353,8 @@ int mhip_paged_attention_weighed(void* stream, const mhip_paged_cache* cache, co
  * first, NaN above all); positions that the table names no page for hold none.  What stays moves to the front in its order, keys, values and weights: to the pages of `into` [sequences, into_width],
  * which holds min(keep + recent, width * page_size) keys at least and whose pages the call reads nothing from, or with NULL within the sequence's own.  left [sequences] (not lengths) gets how
  * many they are: the new lengths.  Slots behind the last one stay as they were.  A place whose page is none of the cache's takes no key.  8 bits: a page that takes keys gets the greatest of
- * the scales of the pages they come from, under which values are rounded anew.  seqs: table, lengths, sequences and width are used.  In place pages belong to one sequence; keys that are rotated stay so.
+ * the scales of the pages they come from, under which values are rounded anew.  seqs: table, lengths, sequences and width are used.  In place pages belong to one sequence.
+ * Keys that are rotated stay so, and mhip_paged_append turns by the places of what is left: tokens that follow an eviction are turned by their own positions in front of the append (rotated = 0).
  * The workspace is needed: mhip_paged_evict_workspace says how much is of use and, in `least`, what suffices; 16-byte aligned, overwritten. */
 int64_t mhip_paged_evict_workspace(const mhip_paged_cache* cache, const mhip_sequences* seqs, int64_t keep, int64_t recent, int in_place, int64_t* least);
 int mhip_paged_evict(void* stream, const mhip_paged_cache* cache, const mhip_sequences* seqs, float* weights, int64_t keep, int64_t recent, const int32_t* into, int64_t into_width,

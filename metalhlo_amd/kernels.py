@@ -245,7 +245,8 @@ def paged_attention(q, cache: PagedCache, table, lengths, starts, scale: Optiona
 def paged_attention_shared(q, cache: PagedCache, prefix, prefix_length, table, lengths, starts, scale: Optional[float] = None, is_causal: bool = True,
                            out: Optional[torch.Tensor] = None):
     """`paged_attention` of sequences that have a prefix in common, which is read once for all of them: the first `prefix_length` (int32 [1]) keys of the pages `prefix` (int32 [width]) of the same cache
-    lie in front of each sequence's own, which `table` and `lengths` describe alone.  Every token sees the whole prefix, and of its own sequence what `is_causal` says."""
+    lie in front of each sequence's own, which `table` and `lengths` describe alone.  Every token sees the whole prefix, and of its own sequence what `is_causal` says.
+    `paged_append` turns by a sequence's own positions: behind a prefix of P keys it is given `freqs[P:]`."""
     return (_native or _host()).paged_attention_shared(q, cache, prefix, prefix_length, table, lengths, starts, scale, is_causal, out)
 
 
@@ -260,7 +261,7 @@ def paged_evict(cache: PagedCache, weights, table, lengths, keep: int, recent: i
     as `paged_attention_weighed` adds it up; of equal ones the first, NaN above all).  They move to the front in their order, their weights along, within the sequence's own pages or to those of
     `into` [sequences, width] (room for all of them, and pages that the call reads nothing from); returns the new lengths.  In place a page belongs to one sequence.  Slots behind the new
     length stay as they were.  8 bits: a page takes the greatest scale of those its keys come from.  Keys keep the rotation they have been appended with: the tokens that follow
-    take the places behind what is left, and are turned by their own positions in front of the append."""
+    take the places behind what is left, by which `paged_append` would turn them, and so are turned by their own positions in front of an append without `freqs`."""
     return (_native or _host()).paged_evict(cache, weights, table, lengths, keep, recent, into)
 
 
