@@ -243,7 +243,7 @@ __global__ __launch_bounds__(kWindow) void evict_move_kernel(MoveArgs a) {
         // ---- keys, a piece of sixteen bytes a thread, so many turns at once
         constexpr int kTurn = 4;                                            // (us, 32 sequences, two | four | eight: 82.5 | 81 | 119)
         for (int p0 = 0; p0 < here * kPer; p0 += kTurn * kWindow) {
-            // (the row that a piece goes to is held and asked about where it is stored: with a token's number set to -1 in the first loop instead, the compiler stored pieces whose page is none)
+            // (where a piece goes, -1 for none, is formed once and decides about the load and about the store)
             u32x4 v[kTurn];
             int token[kTurn], into[kTurn];
 #pragma unroll
