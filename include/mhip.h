@@ -221,11 +221,12 @@ typedef struct {
     int64_t N, K, group;
 } mhip_w4;
 /* Writes `out`'s words and scales (dtype BF16 or F16) from w, whose element (n, k) is at n * stride_n + k * stride_k: F32, BF16 or F16, finite.  Of each group lo = min(w, 0) and hi = max(w, 0),
- * scale = (hi - lo) / 15 rounded to dtype, zero = round(-lo / scale), q = round(w / scale) + zero within 0 .. 15. */
+ * scale = (hi - lo) / 15 rounded to dtype (its greatest number at most), zero = round(-lo / scale), q = round(w / scale) + zero within 0 .. 15. */
 int mhip_quantize_w4(void* stream, const void* w, int64_t stride_n, int64_t stride_k, const mhip_w4* out, int w_dtype, int dtype);
 /* c [M, N] = act(x [M, K] . W^T + bias) (+ residual [M, N]); x, scales, bias [N], residual and c of dtype BF16 or F16, bias and residual may be NULL.  fp32 sums of exact products and
  * one rounding.  The workspace (mhip_linear_w4_workspace bytes, 0: of no use; 16-byte aligned, overwritten) lets few rows deal K over the device; from 129 rows on W is
- * rounded to dtype in it, once, and the product is mhip_gemm_residual's.  With less, or none, neither is done.  The last bits of a row may depend on the number of rows.
+ * rounded to dtype in it, once (to an infinity where it is beyond F16's range), and the product is mhip_gemm_residual's.  With less, or none, neither is done.  The last bits of a row may depend on the number of rows.
+ * An infinity in x yields what W x is, infinities, or NaN where they cancel or meet a weight of zero; a NaN its row of NaN.
  * The reference has no such layer (its matmul: Compiler/CodeGenerator.swift:4797-4850). */
 int64_t mhip_linear_w4_workspace(int64_t M, const mhip_w4* w, int dtype);
 int mhip_linear_w4(void* stream, const void* x, const mhip_w4* w, const void* bias, const void* residual, void* c, int64_t M, int activation, int dtype, void* workspace,

@@ -318,7 +318,9 @@ __global__ __launch_bounds__(64 * WN * WK) void w4_rows_kernel(W4Args g) {
     }
 }
 
-// W as 16-bit numbers [N][stride] (zeros behind K), each rounded once: a wave a kilobyte of words.
+// W as 16-bit numbers [N][stride] (zeros behind K), each rounded once: a wave a kilobyte of words.  The product's operands are of the tensors' type: exact ones would be q, and every
+// group's sums would have to leave the matrix unit to be scaled, as above, which is no quicker from 129 rows on.  Half a step of each weight is, of independent signs, as much of a result as its own rounding: relative to the
+// result's norm, against 64 bits, 1500 rows of 4000 -> 4104 in f16 are off by 2.5e-4 so and by 2.1e-4 with fp32 weights and one rounding.
 template <typename T, int GROUP>
 __global__ __launch_bounds__(256) void w4_widen_kernel(const u32x4* words, const uint32_t* scales, T* out, int N, int K, int n16, int k128, int stride) {
     constexpr int kGroups = kBlockK / GROUP;

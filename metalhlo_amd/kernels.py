@@ -155,7 +155,8 @@ def quantize_w4(weight, group: int = 128, dtype=torch.bfloat16, trans_b: bool = 
 
 
 def linear_w4(x, weight: W4, bias=None, activation: str = "none", residual=None):
-    """act(x [.., K] @ W^T + bias) (+ residual) with W in 4 bits; x, scales, bias and residual of one 16-bit type.  The last bits of a row may depend on how many there are."""
+    """act(x [.., K] @ W^T + bias) (+ residual) with W in 4 bits; x, scales, bias and residual of one 16-bit type.  The last bits of a row may depend on how many there are:
+    from 129 on W is rounded to the type."""
     return (_native or _host()).linear_w4(x, weight, bias, residual, ACTIVATION_CODE[activation])
 
 
