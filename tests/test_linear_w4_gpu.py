@@ -472,3 +472,23 @@ def test_as_many_rows_as_there_may_be(group):
     some = [0, 31, 32, 63, 64, M // 2, M - 65, M - 64, M - 33, M - 32, M - 1]
     check(out[some], x[some], parts)
     check(kernels.linear_w4(x, w)[-200:], x[-200:], parts)
+
+
+@gpu
+@TYPES
+@pytest.mark.parametrize("M,K", [(129, 1100), (140, 1096), (300, 264)])
+def test_infinities_of_many_rows(M, K, dtype):
+    """From 129 rows on, with the widened W, as of few."""
+    from metalhlo_amd import kernels
+    words, scales, parts = random_w4(50, K, 64, dtype, M)
+    w, x = layer(words, scales, parts, 64), normal((M, K), dtype, M)
+    clean, inf, rows = kernels.linear_w4(x, w), float("inf"), [0, M // 2, M - 1]
+    rest = [r for r in range(M) if r not in rows]
+    for places in ([(7, inf)], [(K - 1, -inf)], [(40, inf), (K - 70, inf)], [(50, inf), (51, -inf)]):
+        one = x.clone()
+        for row in rows:
+            for k, v in places:
+                one[row, k] = v
+        got = kernels.linear_w4(one, w)
+        same_as_infinite(got[rows], one[rows], parts)
+        assert torch.equal(got[rest], clean[rest])
