@@ -244,7 +244,7 @@ __global__ __launch_bounds__(64 * WN * WK) void w4_rows_kernel(W4Args g) {
         }
     }
     // Four neighbouring results by themselves, from row `first` of sixteen on, by a wave whose lanes share K eight columns at a time: s (q - z) is a number, and x meets it as it is.  (us, one row of 4096 x 14336 with
-    // an infinity: 32, of which 10 are the product, and 826 with each lane by itself; a NaN ends it within 512 columns.)
+    // an infinity: 32, of which 10 are the product, and 826 with each lane by itself; a NaN ends it where it is met.)
     auto by_weights = [&](int row, int sixteen, int first) __attribute__((always_inline)) {
         f32x4 y = {0.f, 0.f, 0.f, 0.f};
         const uint32_t* words = reinterpret_cast<const uint32_t*>(g.words4 + (int64_t)sixteen * g.k128 * 64 + first);
